@@ -372,6 +372,88 @@ int memopt_paged_attention_int4(const void* query, const uint8_t* kv_pages,
                                 void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Packed batches (no reference counterpart): sequences of different lengths  */
+/* in one batch, their tokens behind one another.                             */
+/* ------------------------------------------------------------------------ */
+#define MEMOPT_DTYPE_F16   0
+#define MEMOPT_DTYPE_BF16  1
+
+/* Page tables and slot maps built on the GPU.  The state is the caller's     */
+/* device memory: block_tables int32 [num_rows, max_blocks_per_seq] and       */
+/* context_lens int32 [num_rows] hold one sequence per row; free_pages int32  */
+/* [num_blocks] is a ring of free pages; pool_state int32 [4] = index of the  */
+/* oldest free page, number of free pages, status bits, internal (0).  A new  */
+/* state has every page in the ring, lengths 0 and state {0, num_blocks, 0, 0}. */
+/* The calls are asynchronous; a call that cannot be done changes nothing but  */
+/* the status word, where it sets (and keeps) the bits that say why:          */
+#define MEMOPT_PAGES_EXHAUSTED   1  /* more new pages than free ones           */
+#define MEMOPT_PAGES_ROW_FULL    2  /* a row would exceed max_blocks_per_seq   */
+#define MEMOPT_PAGES_BAD_ROW     4  /* a row out of range, or twice in a batch */
+#define MEMOPT_PAGES_BAD_LENGTH  8  /* negative, past max_tokens, or keep > length */
+#define MEMOPT_PAGES_CORRUPT    16  /* lengths, ring or table entries out of range */
+
+/* Appends new_lens[b] tokens to table row rows[b] (batch of them; a row at   */
+/* most once).  New pages are taken from the ring in batch order, as          */
+/* memopt_pool_allocate_block would hand them out.  Writes cu_seqlens         */
+/* [batch + 1] (exclusive scan of new_lens), for each new token its slot      */
+/* (page * block_size + offset) and its position in the sequence              */
+/* (slot_mapping and positions int32 [max_tokens], 16-byte aligned, -1 and 0  */
+/* past the last token), and the batch's own rows: batch_tables [batch,       */
+/* max_blocks_per_seq] and batch_lens [batch] with the new tokens.  A refused */
+/* call writes zero cu_seqlens and slots of -1 (which write_cache skips).     */
+/* batch <= 8192, num_rows <= 262144, num_blocks * block_size < 2^31.         */
+int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_rows, int max_blocks_per_seq,
+                         int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
+                         const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
+                         int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
+                         int32_t* batch_lens, void* stream);
+/* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none);   */
+/* the pages behind them go to the ring's end in row and page order and their */
+/* table entries become -1.  With freed page lists as block_tables, their     */
+/* counts as context_lens and block_size 1 it returns those pages.            */
+int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens, int num_rows, int max_blocks_per_seq,
+                         int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
+                         const int32_t* keep_lens, int batch, int block_size, void* stream);
+
+/* Rotary positions with 1 to 4 axes, fused with the cache write.  query      */
+/* [num_tokens, num_heads, head_dim], keys and values [num_tokens,            */
+/* num_kv_heads, head_dim], fp16 or bf16 (dtype), rows of a token contiguous, */
+/* tokens query_stride / key_stride / value_stride elements apart (multiples  */
+/* of 8; pointers 16-byte aligned).  The first 2 num_pairs dims of a head     */
+/* turn, the rest pass through: pair i = dims (i, i + num_pairs), or (2i,     */
+/* 2i + 1) if interleaved, by the angle positions[a][token] * inv_freq[i],    */
+/* a the axis whose section holds i (sections int32 [num_axes] on the HOST,   */
+/* summing to num_pairs; positions int32 [num_axes, num_tokens]; inv_freq     */
+/* fp64 [num_pairs]); angles are exact to fp32 at every int32 position.       */
+/* query_out and keys_out are contiguous and must not overlap the inputs.     */
+/* slot_mapping non-NULL: the rotated keys and the values are also written,   */
+/* as fp16, to key_pool / value_pool [num_blocks, block_size, num_kv_heads,   */
+/* head_dim]; slots outside the pool are skipped, as in write_cache.          */
+/* head_dim 64 or 128, num_pairs a multiple of 8.                             */
+int memopt_rotary_write_cache(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
+                              const void* values, int64_t value_stride, int dtype, int64_t num_tokens, int num_heads,
+                              int num_kv_heads, int head_dim, const int32_t* positions, int num_axes,
+                              const int32_t* sections, const double* inv_freq, int num_pairs, int interleaved,
+                              void* query_out, void* keys_out, const int32_t* slot_mapping, void* key_pool,
+                              void* value_pool, int64_t num_blocks, int block_size, void* stream);
+
+/* Attention inside each sequence of a packed batch.  Sequence s is the rows  */
+/* [cu_seqlens[s], cu_seqlens[s+1]) of query / out [total_tokens, num_heads,  */
+/* head_dim] and keys / values [total_tokens, num_kv_heads, head_dim] (fp16   */
+/* or bf16, layout and strides as above; out contiguous); query head h reads  */
+/* KV head h / (num_heads / num_kv_heads).  Row i of a sequence of n tokens   */
+/* sees its tokens [max(0, c - W), c), c = i + 1 (causal) or n; W = n when    */
+/* window_size <= 0 (the meaning of memopt_paged_attention_f16_ex).  Scores   */
+/* are scaled by 1 / sqrt(head_dim).  Tokens that a row does not see never    */
+/* reach it, whatever they hold.  Rows outside every sequence are not         */
+/* written.  max_seqlen (the longest sequence, or an upper bound) only helps  */
+/* to choose launch shapes.  head_dim 64 or 128.                              */
+int memopt_packed_attention(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
+                            const void* values, int64_t value_stride, int dtype, const int32_t* cu_seqlens,
+                            int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads, int num_kv_heads,
+                            int head_dim, int window_size, int causal, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,9 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(PKG, "libmemopt_b200.so")
 EXT = os.path.join(PKG, "memopt_C.so")
-CU_SOURCES = ["host.cu", "quant.cu", "write_cache.cu", "evict.cu", "decode.cu", "decode_static.cu", "prefill.cu", "compact.cu", "mdpool.cu"]
+CU_SOURCES = ["host.cu", "quant.cu", "write_cache.cu", "evict.cu", "decode.cu", "decode_static.cu", "prefill.cu", "compact.cu", "mdpool.cu",
+              "page_table.cu", "rotary.cu", "packed.cu"]
+EXT_SOURCES = ["memopt_C.cpp", "memopt_C_packed.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
@@ -74,8 +76,8 @@ def build_lib(verbose: bool = False) -> str:
 
 
 def build_ext(verbose: bool = False) -> str:
-    src = os.path.join(CSRC, "memopt_C.cpp")
-    if not _newer(EXT, [src, LIB, os.path.join(INCLUDE, "memopt_b200.h"), __file__]):
+    srcs = [os.path.join(CSRC, s) for s in EXT_SOURCES]
+    if not _newer(EXT, [*srcs, os.path.join(CSRC, "torch_common.h"), LIB, os.path.join(INCLUDE, "memopt_b200.h"), __file__]):
         return EXT
     # The image's /opt/gcc wrapper (picked up by torch's default CXX) produces
     # extensions that crash when a TORCH_CHECK message carries a number;
@@ -88,8 +90,8 @@ def build_ext(verbose: bool = False) -> str:
     os.makedirs(bdir, exist_ok=True)
     cpp_extension.load(
         name="memopt_C",
-        sources=[src],
-        extra_include_paths=[INCLUDE],
+        sources=srcs,
+        extra_include_paths=[INCLUDE, CSRC],
         extra_cflags=["-O2", "-std=c++17"],
         extra_ldflags=[f"-L{PKG}", "-lmemopt_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{PKG}"],
         build_directory=bdir,

@@ -11,9 +11,7 @@
 //   * optional compaction outputs of evict_tokens.
 // The pool tensors are allocated here (caching allocator, zero filled as in
 // kv_cache.cu:135-141); the free-list lives in the C library.
-#include <torch/extension.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
+#include "torch_common.h"
 
 #include <cstdlib>
 #include <map>
@@ -21,9 +19,11 @@
 #include <string>
 #include <vector>
 
-#include "memopt_b200.h"
-
 namespace {
+
+using memopt_torch::aligned_contig;
+using memopt_torch::check;
+using memopt_torch::cur_stream;
 
 struct Pool {
   std::mutex mu;
@@ -36,22 +36,6 @@ struct Pool {
 Pool& P() {
   static Pool p;
   return p;
-}
-
-void check(int st, const char* what) {
-  if (st != MEMOPT_OK) {
-    TORCH_CHECK(false, what, ": ", memopt_last_error(), " (", memopt_status_string(st), ")");
-  }
-}
-
-void* cur_stream() { return reinterpret_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }
-
-bool aligned16(const torch::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
-
-torch::Tensor aligned_contig(const torch::Tensor& t) {
-  auto c = t.contiguous();
-  if (c.numel() > 0 && !aligned16(c)) c = c.clone();
-  return c;
 }
 
 void require_pool(const char* who) {
@@ -645,4 +629,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("cache"), py::arg("group_size"));
   m.def("dequantize_kv_cache_int4", &dequantize_kv_cache_int4, "Dequantize packed INT4 KV cache to FP16",
         py::arg("q_cache"), py::arg("scales"), py::arg("group_size"));
+  bind_packed(m);
 }

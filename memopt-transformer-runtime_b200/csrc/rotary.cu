@@ -1,0 +1,262 @@
+// rotary.cu — rotary positions with several axes, fused with the cache write.
+//
+// A head of D dims has P rotary pairs (dims 2P..D-1 pass through).  Pair i
+// belongs to axis a(i) (the sections share the pairs out among the axes: time,
+// height, width; one axis for plain text) and turns by position[a(i)][token] *
+// inv_freq[i]:
+//   (x, y) -> (x cos - y sin, x sin + y cos),
+// with (x, y) = dims (i, i + P), or (2i, 2i + 1) when interleaved.
+//
+// Angles of far positions: fp32 would lose them (2^17 rad have a spacing of
+// 2^-7).  The frequency is held as a 64-bit fraction of a turn, so the integer
+// product with the position wraps modulo whole turns without rounding, and its
+// top 32 bits are the angle (error below 2^-24 of a half turn).  inv_freq is
+// fp64, so the fraction itself is off by 2^-52 of the frequency.
+//
+// Everything is held in fp32 and rounded once per output.  Bound by HBM: q and
+// k read and written once, v read once, the K and V rows written to the pool.
+// A lane owns 16 dims of a head (two 16-byte vectors holding 8 whole pairs),
+// D/16 lanes a head, a warp 512 / D heads at a time; a token's 8 cos/sin pairs
+// per lane are computed once, shared out over the lanes that need the same
+// ones, and used for every head of the token.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace memopt {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kMaxAxes = 4;
+
+struct RotaryArgs {
+  const void *q, *k, *v;
+  const int32_t* pos;   // [A, T]
+  const double* freq;   // [P]
+  const int32_t* slots;  // [T] or null: no cache write
+  void *q_out, *k_out;
+  __half *kc, *vc;
+  int64_t T, q_stride, k_stride, v_stride;  // strides in elements
+  int64_t num_slots;
+  int H, KVH, P, axes, split;
+  int ends[kMaxAxes];  // axis a owns the pairs below ends[a] and from ends[a - 1] on
+};
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 get(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static __device__ __forceinline__ uint32_t put(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 get(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t put(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = Pair<T>::get(w[i]);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(Pair<T>::put(f[0], f[1]), Pair<T>::put(f[2], f[3]), Pair<T>::put(f[4], f[5]),
+                    Pair<T>::put(f[6], f[7]));
+}
+
+// Both vectors of a lane's unit, rotated (in fp32).
+template <bool kInterleaved>
+__device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
+  if (kInterleaved) {  // a holds pairs 0..3 of the unit, b pairs 4..7
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+      a[2 * i] = x * c[i] - y * s[i];
+      a[2 * i + 1] = x * s[i] + y * c[i];
+      b[2 * i] = z * c[4 + i] - w * s[4 + i];
+      b[2 * i + 1] = z * s[4 + i] + w * c[4 + i];
+    }
+  } else {  // a holds the first dims of the 8 pairs, b the second ones
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = x * c[i] - y * s[i];
+      b[i] = x * s[i] + y * c[i];
+    }
+  }
+}
+
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryArgs p) {
+  constexpr int U = D / 16;         // units (lanes) per head
+  constexpr int HPW = 32 / U;       // heads per warp step
+  constexpr int OWN = 8 / HPW;      // cos/sin pairs a lane computes itself
+  const int lane = threadIdx.x & 31, u = lane % U, sub = lane / U;
+  const bool rotary = u < p.P / 8;
+  // Dims of the unit's two vectors; units past the rotary ones cover the rest of the head.
+  const int d0 = (!rotary || kInterleaved) ? 16 * u : 8 * u;
+  const int d1 = (!rotary || kInterleaved) ? 16 * u + 8 : p.P + 8 * u;
+
+  // This lane's own pairs: frequency in turns (64-bit fraction) and axis.
+  uint64_t turns[OWN];
+  int axis[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    turns[i] = 0;
+    axis[i] = 0;
+    if (rotary) {
+      const int pair = 8 * u + sub * OWN + i;
+      const double f = __ldg(p.freq + pair) * 0.15915494309189535;  // 1 / (2 pi)
+      turns[i] = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+      for (int a = 0; a + 1 < p.axes; ++a) axis[i] += pair >= p.ends[a];
+    }
+  }
+
+  const int heads = p.H + p.KVH;
+  const int steps = (heads + HPW - 1) / HPW;
+  const int64_t items = p.T * p.split;
+  const int64_t nwarps = static_cast<int64_t>(gridDim.x) * kWarps;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); it < items; it += nwarps) {
+    const int64_t t = it / p.split;
+    const int part = static_cast<int>(it - t * p.split);
+    float c[8], s[8];
+    {
+      float oc[OWN], os[OWN];
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const int64_t pos = __ldg(p.pos + axis[i] * p.T + t);
+        const uint64_t w = static_cast<uint64_t>(pos) * turns[i];
+        // the top 32 bits as a signed fraction of a turn, in half turns
+        sincospif(static_cast<float>(static_cast<int32_t>(w >> 32)) * 4.656612873077393e-10f, &os[i], &oc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = (i / OWN) * U + u;
+        c[i] = __shfl_sync(0xffffffffu, oc[i % OWN], from);
+        s[i] = __shfl_sync(0xffffffffu, os[i % OWN], from);
+      }
+    }
+    int64_t slot = -1;
+    if (p.slots) {
+      slot = __ldg(p.slots + t);
+      if (slot >= p.num_slots) slot = -1;
+    }
+    const int lo = static_cast<int>(static_cast<int64_t>(steps) * part / p.split);
+    const int hi = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.split);
+#pragma unroll 2
+    for (int st = lo; st < hi; ++st) {
+      const int h = st * HPW + sub;
+      if (h >= heads) continue;
+      const bool is_k = h >= p.H;
+      const int hk = h - p.H;
+      const T* src = is_k ? static_cast<const T*>(p.k) + t * p.k_stride + hk * D
+                          : static_cast<const T*>(p.q) + t * p.q_stride + h * D;
+      float a[8], b[8];
+      unpack8<T>(ld_stream_v4(src + d0), a);
+      unpack8<T>(ld_stream_v4(src + d1), b);
+      if (rotary) turn<kInterleaved>(a, b, c, s);
+      T* dst = is_k ? static_cast<T*>(p.k_out) + (t * p.KVH + hk) * D : static_cast<T*>(p.q_out) + (t * p.H + h) * D;
+      *reinterpret_cast<uint4*>(dst + d0) = pack8<T>(a);
+      *reinterpret_cast<uint4*>(dst + d1) = pack8<T>(b);
+      if (is_k && slot >= 0) {
+        __half* kd = p.kc + (slot * p.KVH + hk) * D;
+        *reinterpret_cast<uint4*>(kd + d0) = pack8<__half>(a);
+        *reinterpret_cast<uint4*>(kd + d1) = pack8<__half>(b);
+        const T* vs = static_cast<const T*>(p.v) + t * p.v_stride + hk * D;
+        __half* vd = p.vc + (slot * p.KVH + hk) * D;
+        unpack8<T>(ld_stream_v4(vs + d0), a);
+        unpack8<T>(ld_stream_v4(vs + d1), b);
+        *reinterpret_cast<uint4*>(vd + d0) = pack8<__half>(a);
+        *reinterpret_cast<uint4*>(vd + d1) = pack8<__half>(b);
+      }
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int D>
+int launch_rotary(const RotaryArgs& p, bool interleaved, int grid, cudaStream_t s) {
+  if (interleaved) rotary_kernel<T, D, true><<<grid, kWarps * 32, 0, s>>>(p);
+  else rotary_kernel<T, D, false><<<grid, kWarps * 32, 0, s>>>(p);
+  MEMOPT_LAUNCH_CHECK("rotary_kernel launch");
+  return MEMOPT_OK;
+}
+
+}  // namespace
+}  // namespace memopt
+
+using namespace memopt;
+
+extern "C" int memopt_rotary_write_cache(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
+                                         const void* values, int64_t value_stride, int dtype, int64_t num_tokens,
+                                         int num_heads, int num_kv_heads, int head_dim, const int32_t* positions,
+                                         int num_axes, const int32_t* sections, const double* inv_freq, int num_pairs,
+                                         int interleaved, void* query_out, void* keys_out,
+                                         const int32_t* slot_mapping, void* key_pool, void* value_pool,
+                                         int64_t num_blocks, int block_size, void* stream) {
+  if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_heads + num_kv_heads <= 0)
+    return fail(MEMOPT_ERR_INVALID_ARG, "rotary: invalid geometry");
+  if (dtype != MEMOPT_DTYPE_F16 && dtype != MEMOPT_DTYPE_BF16)
+    return fail(MEMOPT_ERR_UNSUPPORTED, "rotary: dtype must be fp16 or bf16");
+  if (head_dim != 64 && head_dim != 128) return fail(MEMOPT_ERR_UNSUPPORTED, "rotary: head_dim must be 64 or 128");
+  if (num_pairs <= 0 || num_pairs % 8 != 0 || 2 * num_pairs > head_dim)
+    return fail(MEMOPT_ERR_UNSUPPORTED, "rotary: the number of pairs must be a multiple of 8, at most head_dim / 2");
+  if (num_axes < 1 || num_axes > kMaxAxes || !sections)
+    return fail(MEMOPT_ERR_UNSUPPORTED, "rotary: between 1 and 4 axes");
+  RotaryArgs p{};
+  int end = 0;
+  for (int a = 0; a < num_axes; ++a) {
+    if (sections[a] < 0 || sections[a] > num_pairs)
+      return fail(MEMOPT_ERR_INVALID_ARG, "rotary: a section is negative or larger than the number of pairs");
+    end += sections[a];
+    p.ends[a] = end;
+  }
+  if (end != num_pairs) return fail(MEMOPT_ERR_INVALID_ARG, "rotary: the sections do not sum to the number of pairs");
+  if (num_tokens == 0) return MEMOPT_OK;
+  const bool cache = slot_mapping != nullptr;
+  if (!positions || !inv_freq || (num_heads > 0 && (!query || !query_out)) ||
+      (num_kv_heads > 0 && (!keys || !keys_out)) || (cache && num_kv_heads > 0 && (!values || !key_pool || !value_pool)))
+    return fail(MEMOPT_ERR_INVALID_ARG, "rotary: null pointer");
+  if (cache && (num_blocks < 0 || block_size <= 0)) return fail(MEMOPT_ERR_INVALID_ARG, "rotary: invalid pool geometry");
+  if (!aligned16(query) || !aligned16(keys) || !aligned16(values) || !aligned16(query_out) || !aligned16(keys_out) ||
+      !aligned16(key_pool) || !aligned16(value_pool) || (query_stride | key_stride | value_stride) % 8 != 0)
+    return fail(MEMOPT_ERR_INVALID_ARG, "rotary: pointers must be 16-byte aligned and strides multiples of 8 elements");
+  p.q = query, p.k = keys, p.v = values;
+  p.q_stride = query_stride, p.k_stride = key_stride, p.v_stride = value_stride;
+  p.pos = positions, p.freq = inv_freq, p.slots = slot_mapping;
+  p.q_out = query_out, p.k_out = keys_out;
+  p.kc = static_cast<__half*>(key_pool), p.vc = static_cast<__half*>(value_pool);
+  p.T = num_tokens, p.num_slots = cache ? num_blocks * block_size : 0;
+  p.H = num_heads, p.KVH = num_kv_heads, p.P = num_pairs, p.axes = num_axes;
+  // Few tokens: a token's heads are split over several warps, so that a decode
+  // step fills the GPU; the cos/sin are then computed once per part.
+  const int hpw = 512 / head_dim, steps = (num_heads + num_kv_heads + hpw - 1) / hpw;
+  const int64_t want = static_cast<int64_t>(sm_count()) * 16;
+  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(steps, want / num_tokens)));
+  const int64_t items = num_tokens * p.split;
+  const int grid = static_cast<int>(std::min<int64_t>((items + kWarps - 1) / kWarps, static_cast<int64_t>(sm_count()) * 8));
+  cudaStream_t s = as_stream(stream);
+  const bool il = interleaved != 0;
+  if (dtype == MEMOPT_DTYPE_F16)
+    return head_dim == 128 ? launch_rotary<__half, 128>(p, il, grid, s) : launch_rotary<__half, 64>(p, il, grid, s);
+  return head_dim == 128 ? launch_rotary<__nv_bfloat16, 128>(p, il, grid, s)
+                         : launch_rotary<__nv_bfloat16, 64>(p, il, grid, s);
+}

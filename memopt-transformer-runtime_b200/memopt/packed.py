@@ -1,0 +1,272 @@
+"""Packed batches: sequences of different lengths served in one step.
+
+The uniform path (:class:`~memopt.kv_cache.PagedKVCache`) takes the same number
+of tokens for every sequence and builds its tables in Python lists.  Here the
+tokens of a batch lie behind one another (``[num_tokens, heads, head_dim]``)
+and everything that depends on the lengths is built on the GPU:
+
+* :class:`DevicePageTable` — block tables, lengths and the ring of free pages
+  in device memory.  ``reserve`` appends tokens to rows and returns the
+  batch's ``cu_seqlens``, slot mapping, positions and tables; ``truncate``
+  gives pages back (a finished sequence, rejected draft tokens).  Pages are
+  handed out in the order of the host free-list (:class:`PageTable`).  Nothing
+  synchronises, so a step can be captured into a CUDA graph; ``check`` reports
+  refused calls.
+* :class:`RotaryPositions` — rotary positions with 1 to 4 axes (time, height,
+  width), applied to q and k and fused with the write into an fp16 pool.
+* :class:`PackedKVCache` — the process-wide pool behind both: ``admit`` /
+  ``prompt`` run a batch of whole prompts (causal attention over the packed
+  tokens), ``extend`` / ``decode`` the steps after them (paged attention).
+
+These operators serve; they carry no gradient and refuse inputs that ask for
+one.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+__all__ = ["DevicePageTable", "PackedBatch", "PackedKVCache", "RotaryPositions"]
+
+_STATUS = (
+    (1, "more new pages than free ones"),
+    (2, "a row would exceed its block table"),
+    (4, "a row out of range, or twice in a batch"),
+    (8, "a negative length, more tokens than max_tokens, or a kept length past the row's"),
+    (16, "lengths, ring or table entries out of range"),
+)
+
+Ints = Union[torch.Tensor, Sequence[int]]
+
+
+@dataclass
+class PackedBatch:
+    """What ``reserve`` built for a batch of rows (device tensors, int32)."""
+
+    rows: torch.Tensor          # [B] table rows
+    cu_seqlens: torch.Tensor    # [B + 1] first packed token of each sequence
+    slot_mapping: torch.Tensor  # [max_tokens] slot of each new token, -1 past the last
+    positions: torch.Tensor     # [max_tokens] position of each new token in its sequence
+    block_tables: torch.Tensor  # [B, max_blocks_per_seq]
+    context_lens: torch.Tensor  # [B] lengths with the new tokens
+    whole: bool = False         # the new tokens are the whole sequences
+
+
+class DevicePageTable:
+    """Block tables and free pages in device memory, one sequence per row."""
+
+    def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_len: int,
+                 device: Optional[torch.device] = None) -> None:
+        if min(num_blocks, block_size, max_seqs, max_seq_len) <= 0:
+            raise ValueError("DevicePageTable: num_blocks, block_size, max_seqs and max_seq_len must be > 0")
+        import memopt_C
+
+        self._C = memopt_C
+        self.num_blocks, self.block_size, self.max_seqs = num_blocks, block_size, max_seqs
+        self.max_seq_len = max_seq_len
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        width = (max_seq_len + block_size - 1) // block_size
+
+        def int32(value, *shape):
+            return torch.full(shape, value, dtype=torch.int32, device=self.device)
+
+        self.block_tables = int32(-1, max_seqs, width)
+        self.context_lens = int32(0, max_seqs)
+        self.free_pages = torch.arange(num_blocks, dtype=torch.int32, device=self.device)
+        self.pool_state = torch.tensor([0, num_blocks, 0, 0], dtype=torch.int32, device=self.device)
+
+    def ints(self, values: Ints) -> torch.Tensor:
+        """Whole numbers as an int32 tensor on the table's device."""
+        if isinstance(values, torch.Tensor):
+            return values.to(device=self.device, dtype=torch.int32)
+        return torch.tensor(list(values), dtype=torch.int32, device=self.device)
+
+    def reserve(self, rows: Ints, new_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
+        """Appends ``new_lens[b]`` tokens to row ``rows[b]``.  ``max_tokens``
+        sizes the per-token outputs (default: the sum of ``new_lens``, which
+        must then be a Python sequence); the sum may be smaller, a larger one
+        is refused.  A refused batch changes nothing (see :meth:`check`): its
+        ``cu_seqlens`` are zero and its slots -1."""
+        if max_tokens is None:
+            if isinstance(new_lens, torch.Tensor):
+                raise ValueError("reserve: max_tokens is needed when new_lens is a tensor")
+            max_tokens = sum(new_lens)
+        r = self.ints(rows)
+        cu, slots, pos, tables, lens = self._C.reserve_slots(
+            self.block_tables, self.context_lens, self.free_pages, self.pool_state, r, self.ints(new_lens),
+            self.block_size, max_tokens)
+        return PackedBatch(r, cu, slots, pos, tables, lens)
+
+    def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
+        """Cuts each row to its first ``keep_lens`` tokens (None: to nothing)
+        and gives the pages behind them back."""
+        keep = None if keep_lens is None else self.ints(keep_lens)
+        self._C.truncate_rows(self.block_tables, self.context_lens, self.free_pages, self.pool_state,
+                              self.ints(rows), keep, self.block_size)
+
+    def release_pages(self, pages: torch.Tensor, counts: torch.Tensor) -> None:
+        """Gives back the first ``counts[i]`` pages of each row of ``pages``
+        (the ``freed_pages`` and ``freed_count`` of an exact eviction; both
+        are cleared)."""
+        n = torch.arange(pages.shape[0], dtype=torch.int32, device=self.device)
+        self._C.truncate_rows(pages, counts, self.free_pages, self.pool_state, n, None, 1)
+
+    def free_count(self) -> int:
+        """Number of free pages (synchronises)."""
+        return int(self.pool_state[1].item())
+
+    def check(self) -> None:
+        """Raises if a call since the last check was refused (synchronises)."""
+        bits = int(self.pool_state[2].item())
+        if bits == 0:
+            return
+        self.pool_state[2] = 0
+        why = "; ".join(text for bit, text in _STATUS if bits & bit)
+        if bits == 1:
+            raise MemoryError(f"DevicePageTable: a call was refused: {why}")
+        raise RuntimeError(f"DevicePageTable: a call was refused: {why}")
+
+
+class RotaryPositions:
+    """Rotary positions of the heads: ``rotary_dim`` leading dims turn (all of
+    ``head_dim`` by default), pair i by ``base ** (-2i / rotary_dim)`` per
+    position of its axis (or by ``inv_freq[i]``); ``sections`` share the pairs
+    out among the axes, one axis by default."""
+
+    def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: Optional[int] = None,
+                 sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                 inv_freq: Optional[torch.Tensor] = None, device: Optional[torch.device] = None) -> None:
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        pairs = rotary_dim // 2
+        if rotary_dim <= 0 or rotary_dim > head_dim or rotary_dim % 16 != 0:
+            raise ValueError("RotaryPositions: rotary_dim must be a multiple of 16, at most head_dim")
+        self.sections: List[int] = [pairs] if sections is None else [int(s) for s in sections]
+        if min(self.sections, default=-1) < 0 or sum(self.sections) != pairs or len(self.sections) > 4:
+            raise ValueError(f"RotaryPositions: sections must be 1 to 4 counts that sum to {pairs}")
+        if inv_freq is None:
+            inv_freq = float(base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        if inv_freq.shape != (pairs,):
+            raise ValueError(f"RotaryPositions: inv_freq must hold {pairs} values")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, interleaved
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.inv_freq = inv_freq.to(device=self.device, dtype=torch.float64)
+
+    def apply(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """q [T, H, D] and k [T, KVH, D] turned by ``positions`` int32 [axes, T]
+        (or [T] for one axis)."""
+        import memopt_C
+
+        q2, k2 = memopt_C.apply_rotary(q, k, positions, self.inv_freq, self.sections, self.interleaved)
+        return q2, k2
+
+    def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+              slot_mapping: torch.Tensor, key_cache: torch.Tensor,
+              value_cache: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """:meth:`apply`, and the turned keys and the values written to the
+        fp16 pool at ``slot_mapping`` in the same pass."""
+        import memopt_C
+
+        q2, k2 = memopt_C.rotary_write_cache(q, k, v, positions, self.inv_freq, self.sections, slot_mapping,
+                                             key_cache, value_cache, self.interleaved)
+        return q2, k2
+
+
+class PackedKVCache:
+    """Packed-batch KV cache of one attention layer over the process-wide pool."""
+
+    def __init__(self, num_blocks: int, num_heads: int, head_dim: int, block_size: int = 16, max_seqs: int = 256,
+                 max_seq_len: int = 32768, kv_format: str = "fp16", rotary: Optional[RotaryPositions] = None,
+                 device: Optional[torch.device] = None) -> None:
+        import memopt_C
+
+        self._C = memopt_C
+        if rotary is not None and rotary.head_dim != head_dim:
+            raise ValueError("PackedKVCache: rotary.head_dim differs from head_dim")
+        self.num_heads, self.head_dim, self.block_size, self.rotary = num_heads, head_dim, block_size, rotary
+        memopt_C.init_pool(num_blocks, block_size, num_heads, head_dim, kv_format=kv_format)
+        self.table = DevicePageTable(num_blocks, block_size, max_seqs, max_seq_len, device)
+
+    @property
+    def kv_format(self) -> str:
+        return self._C.pool_format()
+
+    # ---- tables --------------------------------------------------------------
+    def admit(self, rows: Ints, prompt_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
+        """Starts a sequence in each row (what the row held is given back) and
+        reserves its prompt."""
+        r = self.table.ints(rows)
+        self.table.truncate(r)
+        batch = self.table.reserve(r, prompt_lens, max_tokens)
+        batch.whole = True
+        return batch
+
+    def extend(self, rows: Ints, tokens_per_row: int = 1) -> PackedBatch:
+        """Reserves the next ``tokens_per_row`` tokens of each row."""
+        r = self.table.ints(rows)
+        n = torch.full_like(r, tokens_per_row)
+        return self.table.reserve(r, n, int(r.numel()) * tokens_per_row)
+
+    def finish(self, rows: Ints) -> None:
+        """Gives the pages of finished rows back."""
+        self.table.truncate(rows)
+
+    # ---- data path -------------------------------------------------------------
+    def _store(self, q, k, v, batch: PackedBatch, positions):
+        if self.rotary is not None:
+            pos = batch.positions if positions is None else positions
+            if positions is None and len(self.rotary.sections) > 1:
+                pos = batch.positions.expand(len(self.rotary.sections), -1)
+            if self.kv_format == "fp16":
+                kc, vc = self._C.get_pool_tensors()
+                return self.rotary.write(q, k, v, pos, batch.slot_mapping, kc, vc)
+            q, k = self.rotary.apply(q, k, pos)
+        elif positions is not None:
+            raise ValueError("PackedKVCache: positions without rotary")
+        self._C.write_cache(k.to(torch.float16).contiguous(), v.to(torch.float16).contiguous(), batch.block_tables,
+                            batch.slot_mapping)
+        return q, k
+
+    def prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PackedBatch, max_seqlen: int,
+               window_size: int = -1, causal: bool = True, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Whole prompts (a batch of :meth:`admit`): rotary positions (the
+        tokens' own, or ``positions`` [axes, T]), the cache write, and
+        attention inside each prompt.  q [T, H, D], k and v [T, KVH, D]; rows
+        past the batch's last token come back as they are in memory."""
+        if not batch.whole:
+            raise ValueError("PackedKVCache.prompt: the batch must come from admit (whole sequences)")
+        q, k = self._store(q, k, v, batch, positions)
+        return self._C.packed_attention(q, k, v, batch.cu_seqlens, max_seqlen, window_size, causal)
+
+    def decode(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PackedBatch, window_size: int = -1,
+               positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next tokens of each row (a batch of :meth:`extend`, the same
+        number n of tokens per row): causal paged attention over the cached
+        context.  q [B * n, H, D]; the result has q's shape, in fp16."""
+        B = batch.rows.numel()
+        if B == 0 or q.shape[0] % B != 0:
+            raise ValueError(f"PackedKVCache.decode: {q.shape[0]} tokens for {B} rows")
+        q, _ = self._store(q, k, v, batch, positions)
+        q4 = q.to(torch.float16).reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])
+        reach = batch.block_tables.shape[1] * self.block_size
+        window = reach if window_size <= 0 else window_size
+        if self.kv_format == "int4":
+            out = self._C.dynamic_sparse_attention_int4(q4, self._C.get_int4_pages(), batch.block_tables,
+                                                        batch.context_lens, reach, window, True)
+        else:
+            kc, vc = self._C.get_pool_tensors()
+            out = self._C.dynamic_sparse_attention(q4, kc, vc, batch.block_tables, batch.context_lens, reach, window,
+                                                   True)
+        return out.reshape(q.shape)
+
+    def evict(self, scores: torch.Tensor, retain_ratio: float, num_sink_tokens: int = 4):
+        """``evict_topk_compact`` over every row of the table (scores fp32
+        [max_seqs, heads, L], L at least the longest row): kept tokens move to
+        the front, lengths shrink, emptied pages return to the ring.  Returns
+        (kept_idx, kept_count)."""
+        t = self.table
+        kept, count, freed, freed_count = self._C.evict_topk_compact(scores, t.block_tables, t.context_lens,
+                                                                     float(retain_ratio), int(num_sink_tokens))
+        t.release_pages(freed, freed_count)
+        return kept, count

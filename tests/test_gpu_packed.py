@@ -1,0 +1,550 @@
+"""Packed-batch operators on the GPU against plain implementations in 64 bits:
+attention over packed prompts, rotary positions with the cache write, device
+page tables, and the three together as a cache uses them."""
+from __future__ import annotations
+
+import math
+import random
+from collections import deque
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def C():
+    import memopt_C
+
+    return memopt_C
+
+
+def half_step(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+# ---- attention over packed prompts -------------------------------------------
+def attention_ref(q, k, v, lens, window, causal):
+    """(out, sum of p |v|, max |v|) per element, fp64; sequences in order."""
+    T, H, D = q.shape
+    G = H // k.shape[1]
+    out = torch.zeros(T, H, D, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    lo = 0
+    for n in lens:
+        if n:
+            i = torch.arange(n, device=q.device)
+            end = i + 1 if causal else torch.full_like(i, n)
+            start = (end - window).clamp(min=0) if window > 0 else torch.zeros_like(end)
+            hide = (i[None] >= end[:, None]) | (i[None] < start[:, None])
+            kk = k[lo:lo + n].double().repeat_interleave(G, 1)
+            vv = v[lo:lo + n].double().repeat_interleave(G, 1)
+            s = torch.einsum("qhd,khd->hqk", q[lo:lo + n].double(), kk) / math.sqrt(D)
+            p = torch.softmax(s.masked_fill(hide[None], float("-inf")), -1)
+            out[lo:lo + n] = torch.einsum("hqk,khd->qhd", p, vv)
+            mag[lo:lo + n] = torch.einsum("hqk,khd->qhd", p, vv.abs())
+        lo += n
+    return out, mag
+
+
+def attention_tol(out, mag, v, n, dtype):
+    """u = half a step of the type.  The final rounding is u |out|.  A weight p
+    is rounded to the type before P.V and the row sum may add rounded or exact
+    weights: 2 u sum p |v|.  Scores are fp32 sums of D products with |s| < 64
+    here, 2^-14 on a weight covers them and the exponential.  fp16 weights
+    below 2^-14 are subnormal: an absolute 2^-25 each, n of them."""
+    u = half_step(dtype)
+    tol = u * out.abs() + (2 * u + 2.0 ** -14) * mag + 1e-7
+    if dtype == torch.float16:
+        tol = tol + n * 2.0 ** -25 * v.abs().max().double()
+    return tol
+
+
+def make_qkv(lens, H, KVH, D, dtype, seed=0, tail=0, fused=False, spread=2.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    T = sum(lens) + tail
+    if fused:
+        x = torch.randn(T, H + 2 * KVH, D, generator=g, device=DEV)
+        x[:, :H] *= spread
+        x = x.to(dtype)
+        return x[:, :H], x[:, H:H + KVH], x[:, H + KVH:]
+    q = (spread * torch.randn(T, H, D, generator=g, device=DEV)).to(dtype)
+    k = torch.randn(T, KVH, D, generator=g, device=DEV).to(dtype)
+    v = torch.randn(T, KVH, D, generator=g, device=DEV).to(dtype)
+    return q, k, v
+
+
+def cu_of(lens):
+    return torch.tensor([0] + lens, device=DEV).cumsum(0).to(torch.int32)
+
+
+def check_attention(lens, H, KVH, D, dtype, causal=True, window=-1, fused=False, seed=0, spread=2.0, tail=0,
+                    max_seqlen=None):
+    q, k, v = make_qkv(lens, H, KVH, D, dtype, seed, tail, fused, spread)
+    out = C().packed_attention(q, k, v, cu_of(lens), max(lens) if max_seqlen is None else max_seqlen, window, causal)
+    T = sum(lens)
+    ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, window, causal)
+    err = (out[:T].double() - ref).abs()
+    bad = err > attention_tol(ref, mag, v, max(lens), dtype)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {err.max().item():.3g}"
+
+
+LENGTHS = [[1], [5], [64], [127, 128, 129], [255, 1, 0, 257], [0, 0, 33], [300, 2, 61, 0, 16, 128, 400], [1000],
+           [63, 65, 191, 193, 32, 31], [2049, 7]]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens", LENGTHS, ids=str)
+def test_attention_lengths(lens, causal):
+    check_attention(lens, 4, 2, 128, torch.float16, causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,KVH", [(1, 1), (3, 3), (8, 1), (5, 1), (12, 4), (6, 2), (32, 1), (7, 7), (24, 2)])
+def test_attention_heads(H, KVH, D, dtype):
+    check_attention([150, 1, 77, 300], H, KVH, D, dtype, fused=True, seed=3)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 128, 200, 511, 5000])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_window(window, causal):
+    check_attention([700, 90, 1, 333], 4, 2, 64, torch.bfloat16, causal, window, seed=5)
+    check_attention([700, 90, 1, 333], 4, 4, 128, torch.float16, causal, window, seed=6)
+
+
+def test_attention_long_and_peaked():
+    check_attention([5000, 3], 2, 1, 128, torch.float16, seed=7)
+    check_attention([3001], 2, 2, 64, torch.bfloat16, seed=8, spread=4.0)  # |s| < 64: q.k/8 of 64 products
+
+
+def test_attention_rising_scores():
+    """Every key scores above all earlier ones: the running maximum moves in each block."""
+    n, D = 1500, 128
+    q = torch.zeros(n, 1, D, device=DEV, dtype=torch.float16)
+    k = torch.zeros_like(q)
+    q[:, 0, 0] = 8.0
+    k[:, 0, 0] = torch.linspace(-40.0, 40.0, n, device=DEV).half()
+    v = torch.randn(n, 1, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).half()
+    for order in (torch.arange(n, device=DEV), torch.arange(n - 1, -1, -1, device=DEV)):
+        kk, vv = k[order].contiguous(), v[order].contiguous()
+        out = C().packed_attention(q, kk, vv, cu_of([n]), n)
+        ref, mag = attention_ref(q, kk, vv, [n], -1, True)
+        assert ((out.double() - ref).abs() <= attention_tol(ref, mag, v, n, torch.float16)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_hidden_tokens_never_reach_a_row(dtype, value):
+    """Non-finite keys and values of other sequences, of later tokens and of
+    tokens before the window leave the rows that do not see them unchanged."""
+    lens, H, KVH, D = [130, 200, 50], 4, 2, 128
+    q, k, v = make_qkv(lens, H, KVH, D, dtype, seed=11, tail=40)
+    cu = cu_of(lens)
+    at = 130 + 120  # a token of the second sequence
+    for window in (-1, 40):
+        ref = C().packed_attention(q, k, v, cu, 200, window, True)
+        for which in (k, v):
+            x = which.clone()
+            x[at], x[380:] = value, value  # and the rows behind the last sequence
+            kk, vv = (x, v) if which is k else (k, x)
+            out = C().packed_attention(q, kk, vv, cu, 200, window, True)
+            last = 330 if window < 0 else at + window
+            clean = torch.ones(380, dtype=torch.bool, device=DEV)
+            clean[at:last] = False
+            assert torch.equal(out[:380][clean], ref[:380][clean])
+            if which is v:  # the rows that see the value carry it
+                assert not torch.isfinite(out[at:last].float()).any()
+            elif math.isnan(value):
+                assert torch.isnan(out[at:last].float()).all()
+
+
+def test_attention_leaves_rows_behind_the_last_sequence():
+    lens = [100, 29]
+    q, k, v = make_qkv(lens, 4, 2, 128, torch.float16, tail=70)
+    out = torch.full_like(q, 7.0)
+    got = C().packed_attention(q, k, v, cu_of(lens), 100, -1, True, out)
+    assert got.data_ptr() == out.data_ptr()
+    assert (out[129:] == 7.0).all() and (out[:129] != 7.0).any()
+    # sequences need not begin at the first row either
+    out.fill_(7.0)
+    C().packed_attention(q, k, v, cu_of(lens) + 40, 100, -1, True, out)
+    assert (out[:40] == 7.0).all() and (out[169:] == 7.0).all()
+    again = C().packed_attention(q[40:169].contiguous(), k[40:169].contiguous(), v[40:169].contiguous(), cu_of(lens),
+                                 100)
+    assert torch.equal(out[40:169], again)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 64, 100000])
+def test_attention_length_hint_changes_nothing(hint):
+    check_attention([300, 70, 513], 4, 2, 128, torch.float16, max_seqlen=hint)
+
+
+def test_attention_lengths_out_of_range_stay_inside():
+    """cu_seqlens is device data that the host cannot check: decreasing or too
+    large values must not reach outside the tensors."""
+    q, k, v = make_qkv([200], 2, 2, 64, torch.float16)
+    out = torch.zeros_like(q)
+    C().packed_attention(q, k, v, torch.tensor([0, 120, 60, 500], dtype=torch.int32, device=DEV), 200, -1, True, out)
+    torch.cuda.synchronize()
+    ref = C().packed_attention(q, k, v, torch.tensor([0, 120], dtype=torch.int32, device=DEV), 200)
+    assert torch.equal(out[:60], ref[:60])
+
+
+def test_attention_many_sequences():
+    rng = random.Random(0)
+    lens = [rng.choice([0, 1, 2, 3, 7, 20, 33]) for _ in range(1500)]
+    check_attention(lens, 2, 1, 64, torch.float16, seed=13)
+
+
+def test_attention_same_bits_again_and_on_another_stream():
+    lens = [500, 3, 130]
+    q, k, v = make_qkv(lens, 8, 2, 128, torch.bfloat16, fused=True)
+    cu = cu_of(lens)
+    ref = C().packed_attention(q, k, v, cu, 500)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [C().packed_attention(q, k, v, cu, 500) for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)
+
+
+def test_attention_in_a_graph_with_new_lengths():
+    q, k, v = make_qkv([600], 4, 4, 128, torch.float16)
+    cu = cu_of([100, 200, 300])
+    out = torch.zeros_like(q)
+    C().packed_attention(q, k, v, cu, 600, -1, True, out)  # warm-up
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        C().packed_attention(q, k, v, cu, 600, -1, True, out)
+    for lens in ([100, 200, 300], [0, 599, 1], [600, 0, 0], [1, 1, 1]):
+        cu.copy_(cu_of(lens))
+        out.zero_()
+        graph.replay()
+        T = sum(lens)
+        ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, -1, True)
+        assert ((out[:T].double() - ref).abs() <= attention_tol(ref, mag, v, max(lens), torch.float16)).all()
+        assert (out[T:] == 0).all()
+
+
+# ---- rotary positions ----------------------------------------------------------
+def rotary_ref(x, pos, freq, sections, interleaved):
+    """(turned, |x| + |y| of the pair) in fp64."""
+    P = freq.numel()
+    axis = torch.repeat_interleave(torch.arange(len(sections), device=DEV), torch.tensor(sections, device=DEV))
+    a = (pos.double().reshape(len(sections), -1)[axis].T * freq[None])[:, None]  # [T, 1, P]
+    y, m = x.double().clone(), x.double().abs()
+    one = torch.arange(P, device=DEV) * (2 if interleaved else 1)
+    two = one + 1 if interleaved else one + P
+    u, w = x.double()[..., one], x.double()[..., two]
+    y[..., one], y[..., two] = u * a.cos() - w * a.sin(), u * a.sin() + w * a.cos()
+    m[..., one] = m[..., two] = u.abs() + w.abs()
+    return y, m
+
+
+def rotary_close(got, ref, mag):
+    """Half a step of the type, plus fp32 arithmetic: the angle is off by at
+    most pi 2^-24, cos and sin by 2 ulp and two products and a sum round:
+    below 2^-20 of |x| + |y|; fp16 subnormals 2^-25."""
+    tol = half_step(got.dtype) * ref.abs() + 2.0 ** -20 * mag + 2.0 ** -25
+    return bool(((got.double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,H,KVH,D,P,sections,interleaved", [
+    (1, 32, 8, 128, 64, [64], False), (1, 1, 1, 64, 32, [32], True), (33, 32, 8, 128, 64, [16, 24, 24], False),
+    (700, 5, 1, 64, 24, [10, 14], True), (257, 3, 3, 128, 8, [8], False), (64, 40, 8, 128, 48, [1, 0, 40, 7], True),
+    (5000, 8, 2, 64, 32, [32], False), (19, 7, 7, 64, 16, [3, 13], False)])
+def test_rotary(T, H, KVH, D, P, sections, interleaved, dtype):
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, H + 2 * KVH, D, generator=g, device=DEV).to(dtype)
+    q, k, v = x[:, :H], x[:, H:H + KVH], x[:, H + KVH:]
+    pos = torch.randint(-(1 << 20), 1 << 24, (len(sections), T), generator=g, device=DEV, dtype=torch.int32)
+    pos[:, 0] = torch.tensor([0, 2 ** 31 - 1, -2 ** 31, 131071][:len(sections)], dtype=torch.int32, device=DEV)
+    freq = 500000.0 ** (-torch.arange(P, device=DEV, dtype=torch.float64) / P)
+    q2, k2 = C().apply_rotary(q, k, pos, freq, sections, interleaved)
+    assert rotary_close(q2, *rotary_ref(q, pos, freq, sections, interleaved))
+    assert rotary_close(k2, *rotary_ref(k, pos, freq, sections, interleaved))
+    assert torch.equal(q2[..., 2 * P:], q[..., 2 * P:])  # the rest of the head passes through
+    # the same with the cache write: shuffled slots, some tokens without one
+    BS = 16
+    NB = T // BS + 4
+    kc = torch.full((NB, BS, KVH, D), 3.0, dtype=torch.float16, device=DEV)
+    vc = kc.clone()
+    slots = torch.randperm(NB * BS, generator=g, device=DEV)[:T].to(torch.int32)
+    if T > 4:
+        slots[2], slots[3], slots[4] = -1, NB * BS, 2 ** 31 - 1
+    q3, k3 = C().rotary_write_cache(q, k, v, pos, freq, sections, slots, kc, vc, interleaved)
+    assert torch.equal(q3, q2) and torch.equal(k3, k2)
+    ok = (slots >= 0) & (slots < NB * BS)
+    at = slots[ok].long()
+    ref, mag = rotary_ref(k, pos, freq, sections, interleaved)
+    assert rotary_close(kc.view(-1, KVH, D)[at], ref[ok], mag[ok])
+    assert torch.equal(vc.view(-1, KVH, D)[at], v[ok].half())
+    rest = torch.ones(NB * BS, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert (kc.view(-1, KVH, D)[rest] == 3.0).all() and (vc.view(-1, KVH, D)[rest] == 3.0).all()
+
+
+def test_rotary_relative_positions():
+    """Turned by p and by p + s, a pair's inner product depends on s alone."""
+    D, P = 128, 64
+    freq = 10000.0 ** (-torch.arange(P, device=DEV, dtype=torch.float64) / P)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(1, 1, D, generator=g, device=DEV).half().expand(64, 1, D).contiguous()
+    y = torch.randn(1, 1, D, generator=g, device=DEV).half().expand(64, 1, D).contiguous()
+    pos = torch.arange(64, device=DEV, dtype=torch.int32) * 65521
+    a, _ = C().apply_rotary(x, x, pos, freq, [P])
+    b, _ = C().apply_rotary(y, y, pos + 17, freq, [P])
+    dots = (a.double() * b.double()).sum(-1)
+    # two fp16 roundings of each of D products
+    assert (dots - dots[0]).abs().max() <= 4 * 2.0 ** -11 * (a.double() * b.double()).abs().sum(-1).max()
+
+
+# ---- device page tables -----------------------------------------------------------
+class Host:
+    """The same bookkeeping on the host: a FIFO of pages and a list per row."""
+
+    def __init__(self, NB, BS, R, MB):
+        self.NB, self.BS, self.R, self.MB = NB, BS, R, MB
+        self.free = deque(range(NB))
+        self.pages = [[] for _ in range(R)]
+        self.lens = [0] * R
+
+    def need(self, tokens):
+        return -(-tokens // self.BS)
+
+    def refusal(self, rows, new, cap):
+        if len(set(rows)) < len(rows) or any(not 0 <= r < self.R for r in rows):
+            return 4
+        if any(n < 0 for n in new) or sum(new) > cap:
+            return 8
+        if any(self.need(self.lens[r] + n) > self.MB for r, n in zip(rows, new)):
+            return 2
+        if sum(self.need(self.lens[r] + n) - len(self.pages[r]) for r, n in zip(rows, new)) > len(self.free):
+            return 1
+        return 0
+
+    def reserve(self, rows, new):
+        slots, pos = [], []
+        for r, n in zip(rows, new):
+            while len(self.pages[r]) < self.need(self.lens[r] + n):
+                self.pages[r].append(self.free.popleft())
+            for t in range(self.lens[r], self.lens[r] + n):
+                slots.append(self.pages[r][t // self.BS] * self.BS + t % self.BS)
+                pos.append(t)
+            self.lens[r] += n
+        return slots, pos
+
+    def truncate(self, rows, keep):
+        for r, n in zip(rows, keep):
+            m = self.need(n)
+            self.free.extend(self.pages[r][m:])
+            self.pages[r] = self.pages[r][:m]
+            self.lens[r] = n
+
+    def same(self, table):
+        head, count, status, ticket = table.pool_state.tolist()
+        assert (status, ticket) == (0, 0)
+        ring = table.free_pages.tolist()
+        assert [ring[(head + i) % self.NB] for i in range(count)] == list(self.free)
+        assert table.context_lens.tolist() == self.lens
+        assert table.block_tables.tolist() == [p + [-1] * (self.MB - len(p)) for p in self.pages]
+
+
+@pytest.mark.parametrize("NB,BS,R,width,batch,most", [(64, 16, 8, 7, 5, 40), (5000, 16, 300, 300, 280, 300),
+                                                     (900, 32, 3, 300, 2, 6000), (40, 1, 9, 11, 4, 3),
+                                                     (20000, 16, 1200, 40, 1100, 60)])
+def test_page_table_against_the_host(NB, BS, R, width, batch, most):
+    from memopt import DevicePageTable
+
+    rng = random.Random(NB)
+    host, table = Host(NB, BS, R, width), DevicePageTable(NB, BS, R, width * BS)
+    refused = 0
+    for step in range(30):
+        rows = rng.sample(range(R), rng.randint(0, batch))
+        new = [rng.choice([0, 1, 1, rng.randint(0, most)]) for _ in rows]
+        cap = sum(new) + rng.choice([0, 0, 1, 70])
+        why = host.refusal(rows, new, cap)
+        got = table.reserve(rows, new, cap)
+        if why:
+            refused += 1
+            assert table.pool_state[2].item() == why
+            with pytest.raises(MemoryError if why == 1 else RuntimeError):
+                table.check()
+            assert (got.slot_mapping == -1).all() and (got.cu_seqlens == 0).all()
+            slots, pos, new = [], [], [0] * len(rows)
+        else:
+            slots, pos = host.reserve(rows, new)
+            assert got.cu_seqlens.tolist() == [sum(new[:i]) for i in range(len(new) + 1)]
+        pad = cap - len(slots)
+        assert got.slot_mapping.tolist() == slots + [-1] * pad
+        assert got.positions.tolist() == pos + [0] * pad
+        assert got.context_lens.tolist() == [host.lens[r] for r in rows]
+        assert got.block_tables.tolist() == [host.pages[r] + [-1] * (width - len(host.pages[r])) for r in rows]
+        host.same(table)
+        rows = rng.sample(range(R), rng.randint(0, R // 2))
+        keep = [rng.choice([0, host.lens[r], rng.randint(0, host.lens[r])]) for r in rows]
+        if rng.random() < 0.3:
+            keep = [0] * len(rows)
+            table.truncate(rows)
+        else:
+            table.truncate(rows, keep)
+        host.truncate(rows, keep)
+        host.same(table)
+    assert refused < 30
+
+
+def test_page_table_takes_pages_as_the_host_table_does():
+    from memopt import DevicePageTable, PageTable
+
+    free = deque(range(50))
+    host = PageTable(16, lambda: free.popleft() if free else -1, free.append)
+    table = DevicePageTable(50, 16, 4, 400)
+    ids = [host.add_sequence() for _ in range(4)]
+    for new in ([30, 1, 0, 16], [2, 15, 1, 1], [100, 17, 33, 0]):
+        want = [s for i, n in zip(ids, new) for s in host.reserve(i, n)]
+        assert table.reserve(range(4), new).slot_mapping.tolist() == want
+    assert table.block_tables.tolist() == host.block_table(ids, 25)
+    table.check()
+
+
+def test_page_table_refusals_change_nothing():
+    from memopt import DevicePageTable
+
+    table = DevicePageTable(10, 16, 4, 96)  # six pages a row
+    table.reserve([0, 2], [20, 90])
+    before = [t.clone() for t in (table.block_tables, table.context_lens, table.free_pages, table.pool_state[:2])]
+    calls = [(lambda: table.reserve([1, 1], [1, 1]), 4), (lambda: table.reserve([4], [1]), 4),
+             (lambda: table.reserve([-1], [1]), 4), (lambda: table.reserve([0], [-3], 5), 8),
+             (lambda: table.reserve([0, 1], [9, 9], 17), 8), (lambda: table.reserve([2], [7]), 2),
+             (lambda: table.reserve([1, 3], [17, 1]), 1), (lambda: table.truncate([0, 0]), 4),
+             (lambda: table.truncate([0], [21]), 8), (lambda: table.truncate([0], [-1]), 8),
+             (lambda: table.truncate([7]), 4),
+             (lambda: table.reserve([0, 1], [2 ** 31 - 1, 2 ** 31 - 1], 64), 2 + 8)]
+    for call, why in calls:
+        call()
+        assert table.pool_state[2].item() & why
+        with pytest.raises((MemoryError, RuntimeError)):
+            table.check()
+        after = [table.block_tables, table.context_lens, table.free_pages, table.pool_state[:2]]
+        assert all(torch.equal(a, b) for a, b in zip(before, after))
+    table.reserve([1], [1])
+    table.check()
+
+
+def test_page_table_step_in_a_graph():
+    """A captured decode step: one token per row, replayed; half of the rows are cut back in between."""
+    from memopt import DevicePageTable
+
+    host, table = Host(400, 16, 6, 60), DevicePageTable(400, 16, 6, 960)
+    rows = torch.arange(6, dtype=torch.int32, device=DEV)
+    one = torch.ones_like(rows)
+    args = (table.block_tables, table.context_lens, table.free_pages, table.pool_state, rows, one, 16, 8)
+    C().reserve_slots(*args)
+    host.reserve(range(6), [1] * 6)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cu, slots, pos, tables, lens = C().reserve_slots(*args)
+    for step in range(40):
+        graph.replay()
+        want, at = host.reserve(range(6), [1] * 6)
+        assert slots.tolist() == want + [-1, -1] and pos.tolist() == at + [0, 0]
+        assert lens.tolist() == host.lens
+        if step % 7 == 3:
+            table.truncate([1, 3, 5], [3, 0, 1])
+            host.truncate([1, 3, 5], [3, 0, 1])
+    host.same(table)
+
+
+# ---- together -----------------------------------------------------------------------
+@pytest.mark.parametrize("kv_format", ["fp16", "int4"])
+def test_cache_prompt_decode_draft_evict(kv_format):
+    """Prompts of different lengths, decode steps, rejected drafts, a finished
+    row and an exact eviction: attention stays that over the tokens that are
+    cached (read back from the pool) and no page is lost."""
+    from memopt import PackedKVCache, RotaryPositions
+
+    H, KVH, D, BS = 8, 2, 128, 16
+    rot = RotaryPositions(D, sections=[16, 24, 24])
+    cache = PackedKVCache(200, KVH, D, BS, max_seqs=4, max_seq_len=640, kv_format=kv_format, rotary=rot)
+    g = torch.Generator(device=DEV).manual_seed(2)
+
+    def tokens(n):
+        x = torch.randn(n, H + 2 * KVH, D, generator=g, device=DEV).half()
+        return x[:, :H], x[:, H:H + KVH], x[:, H + KVH:]
+
+    lens = [70, 1, 300]
+    batch = cache.admit([0, 3, 1], lens)
+    q, k, v = tokens(371)
+    grid = torch.randint(0, 50, (3, 371), generator=g, device=DEV, dtype=torch.int32)
+    out = cache.prompt(q, k, v, batch, 300, positions=grid)
+    q64, _ = rotary_ref(q, grid, rot.inv_freq, rot.sections, False)
+    k64, _ = rotary_ref(k, grid, rot.inv_freq, rot.sections, False)
+    ref, mag = attention_ref(q64, k64, v, lens, -1, True)
+    # q and k are rounded to fp16: half a step of each of the products of a score
+    size = (q64.abs().amax() * k64.abs().amax() * math.sqrt(D)).item()
+    assert ((out.double() - ref).abs() <= attention_tol(ref, mag, v, 300, torch.float16) +
+            2.0 ** -10 * min(size, 64.0) * mag).all()
+
+    def rows_of(row):  # this row's cached keys and values, fp32 [n, KVH, D]
+        n = int(cache.table.context_lens[row])
+        pages = cache.table.block_tables[row, : -(-n // BS)].long()
+        if kv_format == "fp16":
+            return [c[pages].reshape(-1, KVH, D)[:n].double() for c in C().get_pool_tensors()]
+        import oracle as O
+
+        kv = O.int4_dense(C().get_int4_pages().cpu().numpy(), BS, D) if hasattr(O, "int4_dense") else None
+        return kv
+
+    def step(n):
+        batch = cache.extend([0, 1, 3], n)
+        q, k, v = tokens(3 * n)
+        out = cache.decode(q, k, v, batch)
+        if kv_format == "fp16":
+            pos = batch.positions.expand(3, -1)
+            q64, _ = rotary_ref(q, pos, rot.inv_freq, rot.sections, False)
+            for i, row in enumerate([0, 1, 3]):
+                kk, vv = rows_of(row)
+                m = kk.shape[0]
+                full = torch.zeros(m, H, D, dtype=torch.float64, device=DEV)
+                full[m - n:] = q64[i * n:(i + 1) * n].half().double()
+                ref, mag = attention_ref(full, kk, vv, [m], -1, True)
+                err = (out[i * n:(i + 1) * n].double() - ref[m - n:]).abs()
+                assert (err <= 2e-3 + 1e-2 * ref[m - n:].abs()).all()  # the paged kernels' own tolerance
+        assert torch.isfinite(out.float()).all()
+        return batch
+
+    for _ in range(20):
+        step(1)
+    step(4)
+    cache.table.truncate([0, 1, 3], [91, 321, 22])  # three of four drafts rejected
+    step(1)
+    assert cache.table.context_lens.tolist() == [92, 322, 0, 23]
+    cache.finish([3])
+    scores = torch.rand(4, KVH, 322, generator=g, device=DEV)
+    kept, count = cache.evict(scores, 0.5)
+    assert count.tolist() == [46, 161, 0, 0]
+    batch = cache.extend([0, 1])
+    q, k, v = tokens(2)
+    assert torch.isfinite(cache.decode(q, k, v, batch).float()).all()
+    assert cache.table.context_lens.tolist() == [47, 162, 0, 0]
+    cache.finish([0, 1])
+    cache.table.check()
+    assert cache.table.free_count() == 200
+    assert sorted(cache.table.free_pages.tolist()) == list(range(200))
+
+
+def test_grad_inputs_are_refused():
+    q, k, v = make_qkv([8], 2, 2, 64, torch.float16)
+    q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        C().packed_attention(q, k, v, cu_of([8]), 8)
+    with torch.no_grad():
+        C().packed_attention(q, k, v, cu_of([8]), 8)
+    freq = torch.ones(32, dtype=torch.float64, device=DEV)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        C().apply_rotary(q, k, torch.zeros(8, dtype=torch.int32, device=DEV), freq, [32])
