@@ -1,81 +1,668 @@
 // packed.cu — attention over packed prompts of different lengths, with
-// grouped heads (simple form: one warp per query row and head).
+// grouped heads, on the 5th-generation tensor cores.
+//
+// Row i of a sequence of n tokens sees its tokens [max(0, c - W), c), c = i + 1
+// (causal) or n; out = softmax(q k^T / sqrt(D)) v over them.
+//
+// Work item = (sequence, block of tokens, head unit).  A head unit is Gp query
+// heads that share a KV head (the largest power of two dividing the group, at
+// most 16), and a tile is 128 rows = 128 / Gp tokens x Gp heads: one TMA box of
+// the query tensor lays them out token by token, so grouped heads share every
+// K and V tile and a short prompt still fills rows.  An item has two tiles of
+// consecutive tokens over the same key blocks of 128.
+//
+// A persistent CTA per SM walks the items, long ones first (token blocks by
+// descending index: under a causal mask the work grows with it), 12 warps:
+//   * warps 0-3 / 4-7: softmax of tile 0 / 1, one thread per row (= TMEM lane);
+//   * warp 8 issues the tcgen05.mma: S = Q K^T (128 x 128 x D) into a tile's 128
+//     score columns, O += P V (128 x D x 128) with P read from tensor memory;
+//   * warp 9 loads Q and the K/V blocks by TMA (128-byte swizzle) into a ring;
+//   * warp 10 finds the next item from cu_seqlens while the others work (warp 11
+//     only completes the warpgroup that hands its registers over).
+// The tiles alternate on the tensor pipe: while one tile's scores become
+// weights, the other's products run.  P (16-bit pairs) overwrites the scores it
+// came from; P.V starts on its first 64 keys while the weights of the other 64
+// are being computed.  O is rescaled only when the running maximum grows by
+// more than 2^8 (weights stay <= 2^8 and the sums fp32), which is rare.
+//
+// Masked scores are replaced, so a hidden key never matters.  A hidden value
+// meets a weight of exactly 0, which only a non-finite value survives: rows
+// behind the sequence's end are zeroed in shared memory, and a row whose result is not finite
+// is computed again over its visible tokens alone (row_by_row), so a NaN or an
+// infinity reaches exactly the rows that see it.
+//
+// Every wait is bounded; a wait that runs out ends the CTA with NaN in the rows
+// of the item at hand.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace memopt {
-namespace {
+namespace packed {
 
-constexpr int kWarps = 8;
+constexpr int kBN = 128;       // keys per block
+constexpr int kMaxGp = 16;     // query heads packed into a tile
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kSchedWarp = 10;
+constexpr int kThreads = 384;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 72;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "register split within the launch's registers");
 
-struct PackedArgs {
+struct Params {
   const void *q, *k, *v;
   void* out;
   const int32_t* cu;
-  int64_t q_stride, k_stride, v_stride;
-  int T, S, H, group, window, causal;
-  float qscale;
+  int64_t q_stride, k_stride, v_stride;  // elements between tokens
+  int T, S, H, group;
+  int gshift;       // log2 of the heads packed into a tile
+  int units;        // head units: H >> gshift
+  int tiles;        // tiles per item, 1 or 2
+  int window, causal;
+  float qscale;     // log2(e) / sqrt(D)
 };
 
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <int D>
+struct Cfg {
+  static constexpr int HALVES = D / 64;
+  static constexpr int HALF = kBN * 128;          // 128 rows x 128 B
+  static constexpr int TILE = HALVES * HALF;      // a Q tile, a K block or a V block
+  static constexpr int STAGES = D == 128 ? 5 : 8;
+  static constexpr int KV_OFF = 2 * TILE;
+  static constexpr int SMEM = KV_OFF + STAGES * TILE + 1024;  // + alignment slack
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(2 * (kBN + D) <= 512, "tensor memory columns");
+};
+
+struct Item {
+  int start, n, t0, unit;  // first packed row, length, first token, head unit (n < 0: no more items)
+};
+
+// Bounded wait: at most 2^22 polls of at most 1 us each.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+  uint32_t polls = 0;
+  while (!mbar_try_wait_hint(bar, parity, 1000)) {
+    if (++polls >= (1u << 22)) return false;
+  }
+  return true;
+}
+
+// Key blocks [lo, hi) of an item's tile.
+struct Range {
+  int lo, hi;
+  int last;  // keys below this index are the tile's (visible to some row)
+};
+__device__ __forceinline__ Range tile_range(const Params& p, const Item& it, int t) {
+  const int tokens = 128 >> p.gshift;
+  const int first = it.t0 + t * tokens;
+  if (t >= p.tiles || first >= it.n) return {0, 0, 0};
+  const int end = min(first + tokens, it.n);
+  const int c_last = p.causal ? end : it.n, c_first = p.causal ? first + 1 : it.n;
+  const int from = p.window > 0 && c_first > p.window ? c_first - p.window : 0;
+  return {from / kBN, (c_last + kBN - 1) / kBN, c_last};
+}
+
 template <typename T>
-__device__ __forceinline__ T from_f(float x);
+__device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// One row from its definition, by one warp: lane l holds dims [l D/32, (l+1) D/32),
+// four keys at a time.  Only rows whose fast result is not finite come here.
+template <typename T, int D>
+__device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int64_t key0, int begin, int end) {
+  constexpr int E = D / 64;  // 32-bit words per lane
+  const int lane = threadIdx.x & 31, hk = h / p.group;
+  auto words = [&](const void* base, int64_t at, uint32_t (&w)[E]) {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(base) + at) + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = __ldg(src + e);
+  };
+  float q[2 * E], acc[2 * E], m = -INFINITY, l = 0.f;
+  {
+    uint32_t w[E];
+    words(p.q, row * p.q_stride + static_cast<int64_t>(h) * D, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float2 f = unpack2<T>(w[e]);
+      q[2 * e] = f.x * p.qscale;
+      q[2 * e + 1] = f.y * p.qscale;
+      acc[2 * e] = acc[2 * e + 1] = 0.f;
+    }
+  }
+  for (int j0 = begin; j0 < end; j0 += 4) {
+    uint32_t kw[4][E], vw[4][E];
+    float s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t j = key0 + min(j0 + u, end - 1);
+      words(p.k, j * p.k_stride + static_cast<int64_t>(hk) * D, kw[u]);
+      words(p.v, j * p.v_stride + static_cast<int64_t>(hk) * D, vw[u]);
+      s[u] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float2 f = unpack2<T>(kw[u][e]);
+        s[u] += q[2 * e] * f.x + q[2 * e + 1] * f.y;
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (j0 + u < end) {
+        const float mn = fmaxf(m, s[u]), a = l > 0.f ? exp2f(m - mn) : 0.f;
+        const float w = s[u] == -INFINITY ? 0.f : exp2f(s[u] - mn);
+        l = l > 0.f ? l * a + w : l + w;  // NaN stays: l > 0 is false then and w is added to it
+        m = mn;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 f = unpack2<T>(vw[u][e]);
+          acc[2 * e] = (l > 0.f ? acc[2 * e] * a : acc[2 * e]) + w * f.x;
+          acc[2 * e + 1] = (l > 0.f ? acc[2 * e + 1] * a : acc[2 * e + 1]) + w * f.y;
+        }
+      }
+    }
+  }
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (row * p.H + h) * D) + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = pack2<T>(acc[2 * e] / l, acc[2 * e + 1] / l);
+}
+
+// Barriers: items (2 slots: filled by the scheduler, read by the 10 warps
+// that work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
+// ready (commit), first and second half of P ready (4 warps), P.V done
+// (commit).
+template <int D>
+struct Bars {
+  uint64_t item_full[2], item_free[2], q_full, q_free, kv_full[Cfg<D>::STAGES], kv_free[Cfg<D>::STAGES];
+  uint64_t s_full[2], p_half[2][2], pv_done[2];
+};
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) packed_simple_kernel(const PackedArgs p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int t = static_cast<int>(item / p.H), h = static_cast<int>(item % p.H);
-  if (t >= p.T) return;
-  int lo = 0, hi = p.S;  // the last s with cu[s] <= t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (p.cu[mid] <= t) lo = mid;
-    else hi = mid;
+__global__ void __launch_bounds__(kThreads, 1)
+packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qmap,
+                        const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kIdescS = tc::idesc_f16(128, kBN, false, false, kBf16);
+  constexpr uint32_t kIdescPV = tc::idesc_f16(128, D, false, true, kBf16);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) Bars<D> bars;
+  __shared__ Item items[2];
+  __shared__ uint32_t tmem_slot;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(base);
+  auto at = [](const uint64_t& b) { return smem_u32(&b); };
+  const int tile_tokens = 128 >> p.gshift;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(at(bars.item_full[i]), 1);
+      mbar_init(at(bars.item_free[i]), 10);
+      mbar_init(at(bars.s_full[i]), 1);
+      mbar_init(at(bars.p_half[i][0]), 4);
+      mbar_init(at(bars.p_half[i][1]), 4);
+      mbar_init(at(bars.pv_done[i]), 1);
+    }
+    mbar_init(at(bars.q_full), 1);
+    mbar_init(at(bars.q_free), 1);
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(at(bars.kv_full[i]), 1);
+      mbar_init(at(bars.kv_free[i]), 1);
+    }
+    fence_mbar_init();
   }
-  const int first = max(p.cu[lo], 0), last = min(p.cu[lo + 1], p.T);
-  if (t < first || t >= last) return;
-  const int end = p.causal ? t + 1 : last;
-  const int begin = p.window > 0 && end - first > p.window ? end - p.window : first;
-  const T* q = static_cast<const T*>(p.q) + t * p.q_stride + h * D;
-  const T* k = static_cast<const T*>(p.k) + (h / p.group) * D;
-  const T* v = static_cast<const T*>(p.v) + (h / p.group) * D;
-  float qr[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qr[e] = to_f(q[lane + 32 * e]) * p.qscale;
-    acc[e] = 0.f;
+  if (warp == 0) {
+    tc::tmem_alloc(smem_u32(&tmem_slot), 512);
+    tc::tmem_relinquish();
   }
-  for (int j = begin; j < end; ++j) {
-    float s = 0.f;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  // Tile t: scores (and P) at columns 128 t, O at 256 + D t.
+  auto tS = [&](int t) { return tmem + 128u * t; };
+  auto tO = [&](int t) { return tmem + 256u + static_cast<uint32_t>(D) * t; };
+
+  // The k-th item of this CTA (read by every warp but the scheduler).
+  auto next_item = [&](int k, Item& it) -> bool {
+    const bool ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_full[k & 1]), (k >> 1) & 1));
+    if (!ok) return false;
+    it = items[k & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(at(bars.item_free[k & 1]));
+    return it.n >= 0;
+  };
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // =========================== softmax warps ===========================
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint64_t qs2 = f32x2_pack(p.qscale, p.qscale);
+    uint32_t blocks = 0;  // key blocks of this tile so far (phases of its barriers)
+    bool ok = true;
+    Item it;
+    for (int k = 0; ok && next_item(k, it); ++k) {
+      const Range r = tile_range(p, it, t);
+      if (r.hi == 0) continue;
+      const int tok = it.t0 + t * tile_tokens + (row >> p.gshift);
+      const int h = (it.unit << p.gshift) + (row & ((1 << p.gshift) - 1));
+      const int c = p.causal ? min(tok + 1, it.n) : it.n;
+      const int ws = p.window > 0 && c > p.window ? c - p.window : 0;
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = r.lo; j < r.hi && ok; ++j, ++blocks) {
+        ok = __all_sync(0xffffffffu, wait_bar(at(bars.s_full[t]), blocks & 1));
+        if (!ok) break;
+        tc::fence_after_sync();
+        float s[kBN];
+        {
+          float v0[32], v1[32], v2[32], v3[32];
+          tc::ld32(tS(t) + lane_base, v0);
+          tc::ld32(tS(t) + lane_base + 32, v1);
+          tc::ld32(tS(t) + lane_base + 64, v2);
+          tc::ld32(tS(t) + lane_base + 96, v3);
+          tc::wait_ld(v0);
+          tc::wait_ld(v1);
+          tc::wait_ld(v2);
+          tc::wait_ld(v3);
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += qr[e] * to_f(k[j * p.k_stride + lane + 32 * e]);
+          for (int i = 0; i < 32; ++i) {
+            s[i] = v0[i];
+            s[32 + i] = v1[i];
+            s[64 + i] = v2[i];
+            s[96 + i] = v3[i];
+          }
+        }
+        const int lo = ws - j * kBN, hi = c - j * kBN;  // visible columns [lo, hi)
+        if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float mn = fmaxf(m, s), a = exp2f(m - mn), w = exp2f(s - mn);
-    l = l * a + w;
-    m = mn;
+          for (int i = 0; i < kBN; ++i) s[i] = (i >= lo && i < hi) ? s[i] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + w * to_f(v[j * p.v_stride + lane + 32 * e]);
+        for (int i = 4; i < kBN; i += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[i + e]), i + 4 + e < kBN ? s[i + 4 + e] : s[i + e]);
+        }
+        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.qscale);
+        float alpha = 1.f;
+        bool rescale = false;
+        if (m_run == -INFINITY) {
+          m_run = m_new;  // nothing accumulated yet
+        } else if (m_new > m_run + 8.f) {
+          alpha = tc::ex2(m_run - m_new);
+          m_run = m_new;
+          rescale = true;
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds the earlier blocks only once P.V of the last one completed.
+          if (j > r.lo) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
+          if (!ok) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            float v[32];
+            tc::ld32(tO(t) + lane_base + cc * 32, v);
+            tc::wait_ld(v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= alpha;
+            tc::st32(tO(t) + lane_base + cc * 32, v);
+          }
+          tc::wait_st();
+          l_run *= alpha;
+        }
+        const float msub = m_run == -INFINITY ? 0.f : m_run;  // nothing visible yet: every weight is 2^-inf = 0
+        const uint64_t nm2 = f32x2_pack(-msub, -msub);
+        uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t ph[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int e = half * 64 + 2 * i;
+            float x0, x1;
+            f32x2_unpack(f32x2_fma(f32x2_pack(s[e], s[e + 1]), qs2, nm2), x0, x1);
+            x0 = tc::ex2(x0);
+            x1 = tc::ex2(x1);
+            sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
+            ph[i] = pack2<T>(x0, x1);
+          }
+          tc::st32u(tS(t) + lane_base + half * 32, ph);
+          tc::wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(at(bars.p_half[t][half]));
+        }
+        float a0, a1, b0, b1;
+        f32x2_unpack(f32x2_add(sum2[0], sum2[1]), a0, a1);
+        f32x2_unpack(f32x2_add(sum2[2], sum2[3]), b0, b1);
+        l_run += (a0 + a1) + (b0 + b1);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
+      tc::fence_after_sync();
+      const bool mine = tok < it.n;
+      T* orow = static_cast<T*>(p.out) + (static_cast<int64_t>(it.start + tok) * p.H + h) * D;
+      const float inv = ok ? 1.f / l_run : __int_as_float(0x7fffffff);
+      float odd = 0.f;  // becomes NaN when an element is not finite
+#pragma unroll
+      for (int cc = 0; cc < D / 32; ++cc) {
+        float v[32];
+        tc::ld32(tO(t) + lane_base + cc * 32, v);
+        tc::wait_ld(v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) odd = fmaf(v[i], 0.f, odd);
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack2<T>(v[8 * e + 2 * i] * inv, v[8 * e + 2 * i + 1] * inv);
+            *reinterpret_cast<uint4*>(orow + cc * 32 + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc::fence_before_sync();
+      uint32_t redo = __ballot_sync(0xffffffffu, ok && mine && !(odd == 0.f && l_run > 0.f && l_run < INFINITY));
+      __syncwarp();
+      while (redo) {
+        const int from = __ffs(redo) - 1;
+        redo &= redo - 1;
+        const int rt = __shfl_sync(0xffffffffu, tok, from), rh = __shfl_sync(0xffffffffu, h, from);
+        const int rb = __shfl_sync(0xffffffffu, ws, from), re = __shfl_sync(0xffffffffu, c, from);
+        row_by_row<T, D>(p, it.start + rt, rh, it.start, rb, re);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kMmaWarp) {
+      // ============================== MMA warp ==============================
+      // Warp-uniform code; elect.sync issues each instruction once.
+      const uint64_t dq0 = tc::sdesc_sw128(sbase, 16, 1024);
+      const uint64_t dk0 = tc::sdesc_sw128(sbase + C::KV_OFF, 16, 1024);
+      const uint64_t dv0 = tc::sdesc_sw128(sbase + C::KV_OFF, C::HALF, 1024);
+      auto wait_all = [&](const uint64_t& b, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_bar(at(b), parity & 1));
+      };
+      uint32_t loads = 0;                // K/V blocks consumed before this item
+      uint32_t blocks[2] = {0, 0};       // P blocks of each tile so far
+      bool ok = true;
+      Item it;
+      for (int k = 0; ok && next_item(k, it); ++k) {
+        const Range r[2] = {tile_range(p, it, 0), tile_range(p, it, 1)};
+        const int LO = r[0].lo, HI = max(r[0].hi, r[1].hi);  // tile 0 exists and starts first
+        auto stage_of = [&](int j, int v) { return static_cast<int>((loads + 2u * (j - LO) + v) % C::STAGES); };
+        auto phase_of = [&](int j, int v) { return (loads + 2u * (j - LO) + v) / C::STAGES; };
+        auto in = [&](int t, int j) { return j >= r[t].lo && j < r[t].hi; };
+        auto issue_s = [&](int t, int j) {
+          const uint64_t dk = dk0 + static_cast<uint64_t>((stage_of(j, 0) * C::TILE) >> 4);
+          const uint64_t dq = dq0 + static_cast<uint64_t>((t * C::TILE) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = static_cast<uint64_t>(((kk / 4) * C::HALF + (kk % 4) * 32) >> 4);
+            tc::mma_f16_elect(tS(t), dq + off, dk + off, kIdescS, kk > 0);
+          }
+          tc::commit_elect(at(bars.s_full[t]));
+        };
+        // K(j) is there, S(j) of both tiles; then the block and, after the last one, Q are free.
+        auto after_s = [&](int j) {
+          tc::commit_elect(at(bars.kv_free[stage_of(j, 0)]));
+          if (j == HI - 1) tc::commit_elect(at(bars.q_free));
+        };
+        ok = wait_all(bars.q_full, k) && wait_all(bars.kv_full[stage_of(LO, 0)], phase_of(LO, 0));
+        if (!ok) break;
+        tc::fence_after_sync();
+        for (int t = 0; t < 2; ++t)
+          if (in(t, LO)) issue_s(t, LO);
+        after_s(LO);
+        const bool tail = HI * kBN > it.n && (it.n & 15);  // the last block runs past the sequence's end
+        for (int j = LO; j < HI && ok; ++j) {
+          ok = wait_all(bars.kv_full[stage_of(j, 1)], phase_of(j, 1));
+          if (ok && tail && j == HI - 1) {
+            // Rows behind the sequence's end, up to the 16 keys of an instruction, become zero.
+            const int first = it.n - j * kBN, rows = 16 - (first & 15);
+            uint8_t* v0 = base + C::KV_OFF + stage_of(j, 1) * C::TILE + first * 128;
+            for (int i = lane; i < rows * C::HALVES * 8; i += 32)
+              *reinterpret_cast<uint4*>(v0 + (i % C::HALVES) * C::HALF + (i / C::HALVES) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (in(t, j)) {
+              const uint64_t dv = dv0 + static_cast<uint64_t>((stage_of(j, 1) * C::TILE) >> 4);
+              const int steps = min(kBN, r[t].last - j * kBN + 15) / 16;  // of 16 keys, up to the last one seen
+              for (int half = 0; half < 2 && ok; ++half) {
+                ok = wait_all(bars.p_half[t][half], blocks[t]);
+                if (!ok) break;
+                tc::fence_after_sync();
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk) {
+                  if (kk < steps)
+                    tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4),
+                                             kIdescPV, (j > r[t].lo || kk > 0) ? 1u : 0u);
+                }
+              }
+              if (!ok) break;
+              tc::commit_elect(at(bars.pv_done[t]));
+              ++blocks[t];
+            }
+            if (j + 1 < HI) {
+              if (t == 0) ok = wait_all(bars.kv_full[stage_of(j + 1, 0)], phase_of(j + 1, 0));
+              if (!ok) break;
+              if (in(t, j + 1)) issue_s(t, j + 1);
+            }
+          }
+          if (!ok) break;
+          tc::commit_elect(at(bars.kv_free[stage_of(j, 1)]));
+          if (j + 1 < HI) after_s(j + 1);
+        }
+        loads += 2u * (HI - LO);
+      }
+      // The last commit's arrival lands before the CTA ends.
+      if (ok && loads > 0) wait_all(bars.kv_free[(loads - 1) % C::STAGES], (loads - 1) / C::STAGES);
+    } else if (warp == kLoadWarp) {
+      // ============================== loads ==============================
+      if (lane == 0) {
+        prefetch_tensormap(&qmap);
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+      }
+      uint32_t loads = 0;
+      bool ok = true;
+      Item it;
+      for (int k = 0; ok && next_item(k, it); ++k) {
+        const Range r0 = tile_range(p, it, 0), r1 = tile_range(p, it, 1);
+        const int LO = r0.lo, HI = max(r0.hi, r1.hi);
+        const int h0 = it.unit << p.gshift, hk = h0 / p.group;
+        if (lane == 0) {
+          if (k > 0) ok = wait_bar(at(bars.q_free), (k - 1) & 1);
+          if (ok) {
+            const int ntiles = r1.hi > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(at(bars.q_full), ntiles * C::TILE);
+            for (int t = 0; t < ntiles; ++t)
+              for (int hh = 0; hh < C::HALVES; ++hh)
+                tma_load_3d(sbase + t * C::TILE + hh * C::HALF, &qmap, hh * 64, h0,
+                            it.start + it.t0 + t * tile_tokens, at(bars.q_full));
+          }
+          for (int j = LO; j < HI && ok; ++j) {
+            for (int v = 0; v < 2 && ok; ++v, ++loads) {
+              const int st = loads % C::STAGES;
+              const uint32_t use = loads / C::STAGES;
+              if (use > 0) ok = wait_bar(at(bars.kv_free[st]), (use - 1) & 1);
+              if (!ok) break;
+              mbar_arrive_expect_tx(at(bars.kv_full[st]), C::TILE);
+              for (int hh = 0; hh < C::HALVES; ++hh)
+                tma_load_3d(sbase + C::KV_OFF + st * C::TILE + hh * C::HALF, v ? &vmap : &kmap, hh * 64, hk,
+                            it.start + j * kBN, at(bars.kv_full[st]));
+            }
+          }
+          if (!ok) {  // nothing may be in flight when the CTA ends
+            for (uint32_t u = loads > C::STAGES ? loads - C::STAGES : 0; u < loads; ++u)
+              wait_bar(at(bars.kv_full[u % C::STAGES]), (u / C::STAGES) & 1);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        loads = __shfl_sync(0xffffffffu, loads, 0);
+      }
+    } else if (warp == kSchedWarp) {
+      // ============================ scheduler ============================
+      // Items in descending order of token block index L, within one index the
+      // sequences that have it in order, within a sequence the head units.
+      const int tokens = tile_tokens * p.tiles;
+      auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
+        lo = min(max(__ldg(p.cu + s), 0), p.T);
+        hi = min(max(__ldg(p.cu + s + 1), lo), p.T);
+      };
+      auto nblocks = [&](int s) {
+        int lo = 0, hi = 0;
+        if (s < p.S) bounds(s, lo, hi);
+        return (hi - lo + tokens - 1) / tokens;
+      };
+      int most = 0;
+      int64_t all = 0;
+      for (int s = lane; s < p.S; s += 32) {
+        const int nb = nblocks(s);
+        most = max(most, nb);
+        all += nb;
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+      auto count_above = [&](int L) {  // sequences with a token block of index L
+        int n = 0;
+        for (int s = lane; s < p.S; s += 32) n += nblocks(s) > L;
+        return __reduce_add_sync(0xffffffffu, n);
+      };
+      const int64_t total = all * p.units;
+      int L = most - 1, here = total > 0 ? count_above(L) : 0;
+      int64_t above = 0;  // token blocks of a larger index
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        // every other round in reverse: the sums of work differ less between CTAs
+        const int64_t i = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        Item it{0, -1, 0, 0};
+        if (i < total) {
+          const int64_t b = i / p.units;
+          while (b >= above + here) {
+            above += here;
+            here = count_above(--L);
+          }
+          int skip = static_cast<int>(b - above);
+          for (int s0 = 0; s0 < p.S; s0 += 32) {
+            const uint32_t has = __ballot_sync(0xffffffffu, nblocks(s0 + lane) > L);
+            const int n = __popc(has);
+            if (skip < n) {
+              const int s = s0 + static_cast<int>(__fns(has, 0, skip + 1));
+              int lo, hi;
+              bounds(s, lo, hi);
+              it = Item{lo, hi - lo, L * tokens, static_cast<int>(i - b * p.units)};
+              break;
+            }
+            skip -= n;
+          }
+        }
+        if (k >= 2) ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_free[k & 1]), ((k >> 1) - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          items[k & 1] = it;
+          mbar_arrive(at(bars.item_full[k & 1]));
+        }
+        __syncwarp();
+        if (it.n < 0) break;
+      }
+    }
   }
-  T* o = static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.H + h) * D;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[lane + 32 * e] = from_f<T>(acc[e] / l);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, 512);
+}
+
+namespace {
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [rows][heads][D] with `stride` elements between rows; a box is 64 dims x
+// box_heads x box_rows, 128-byte swizzle, token-major rows.  Rows past the
+// tensor read as zero.
+int map_rows(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t stride, int heads, int D,
+             int box_heads, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return fail(MEMOPT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MEMOPT_ERR_CUDA, "packed_attention: cuTensorMapEncodeTiled failed: " + std::to_string(static_cast<int>(r)));
+  return MEMOPT_OK;
+}
+
+template <typename T, int D>
+int launch(const Params& p, int KVH, int grid, cudaStream_t s) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  alignas(64) CUtensorMap qm, km, vm;
+  const int Gp = 1 << p.gshift;
+  int st = map_rows(&qm, p.q, bf16, p.T, p.q_stride, p.H, D, Gp, 128 / Gp);
+  if (st == MEMOPT_OK) st = map_rows(&km, p.k, bf16, p.T, p.k_stride, KVH, D, 1, kBN);
+  if (st == MEMOPT_OK) st = map_rows(&vm, p.v, bf16, p.T, p.v_stride, KVH, D, 1, kBN);
+  if (st != MEMOPT_OK) return st;
+  auto kern = packed_attention_kernel<T, D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed_attention)");
+  kern<<<grid, kThreads, Cfg<D>::SMEM, s>>>(p, qm, km, vm);
+  MEMOPT_LAUNCH_CHECK("packed_attention_kernel launch");
+  return MEMOPT_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
+}  // namespace packed
 }  // namespace memopt
 
 using namespace memopt;
@@ -95,24 +682,30 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   if (num_seqs == 0 || total_tokens == 0) return MEMOPT_OK;
   if (!query || !keys || !values || !cu_seqlens || !out)
     return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: null pointer");
-  if (!aligned16(query) || !aligned16(keys) || !aligned16(values) || !aligned16(out) ||
-      (query_stride | key_stride | value_stride) % 8 != 0)
+  if (!packed::aligned16(query) || !packed::aligned16(keys) || !packed::aligned16(values) ||
+      !packed::aligned16(out) || (query_stride | key_stride | value_stride) % 8 != 0)
     return fail(MEMOPT_ERR_INVALID_ARG,
                 "packed_attention: pointers must be 16-byte aligned and strides multiples of 8 elements");
-  PackedArgs p{query, keys, values, out, cu_seqlens, query_stride, key_stride, value_stride,
-               static_cast<int>(total_tokens), num_seqs, num_heads, num_heads / num_kv_heads, window_size, causal,
-               (1.0f / sqrtf(static_cast<float>(head_dim))) * 1.4426950408889634f};
+  packed::Params p{};
+  p.q = query, p.k = keys, p.v = values, p.out = out, p.cu = cu_seqlens;
+  p.q_stride = query_stride, p.k_stride = key_stride, p.v_stride = value_stride;
+  p.T = static_cast<int>(total_tokens), p.S = num_seqs, p.H = num_heads, p.group = num_heads / num_kv_heads;
+  while ((2 << p.gshift) <= packed::kMaxGp && p.group % (2 << p.gshift) == 0) ++p.gshift;
+  p.units = num_heads >> p.gshift;
+  p.window = window_size > 0 ? window_size : 0, p.causal = causal ? 1 : 0;
+  p.qscale = (1.0f / sqrtf(static_cast<float>(head_dim))) * 1.4426950408889634f;
+  // At most this many items (each sequence has one partial token block at most):
+  // with fewer than the SMs, an item takes one tile instead of two, so that twice
+  // as many SMs work.
+  const int64_t tokens = 128 >> p.gshift;
+  auto most_items = [&](int tiles) { return (total_tokens / (tokens * tiles) + num_seqs) * p.units; };
+  p.tiles = most_items(2) < sm_count() ? 1 : 2;
   (void)max_seqlen;
-  const int64_t items = total_tokens * num_heads;
-  const int grid = static_cast<int>((items + kWarps - 1) / kWarps);
+  const int grid = static_cast<int>(std::min<int64_t>(most_items(p.tiles), sm_count()));
   cudaStream_t s = as_stream(stream);
-  if (dtype == MEMOPT_DTYPE_F16) {
-    if (head_dim == 128) packed_simple_kernel<__half, 128><<<grid, kWarps * 32, 0, s>>>(p);
-    else packed_simple_kernel<__half, 64><<<grid, kWarps * 32, 0, s>>>(p);
-  } else {
-    if (head_dim == 128) packed_simple_kernel<__nv_bfloat16, 128><<<grid, kWarps * 32, 0, s>>>(p);
-    else packed_simple_kernel<__nv_bfloat16, 64><<<grid, kWarps * 32, 0, s>>>(p);
-  }
-  MEMOPT_LAUNCH_CHECK("packed_attention launch");
-  return MEMOPT_OK;
+  if (dtype == MEMOPT_DTYPE_F16)
+    return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, grid, s)
+                           : packed::launch<__half, 64>(p, num_kv_heads, grid, s);
+  return head_dim == 128 ? packed::launch<__nv_bfloat16, 128>(p, num_kv_heads, grid, s)
+                         : packed::launch<__nv_bfloat16, 64>(p, num_kv_heads, grid, s);
 }

@@ -145,7 +145,7 @@ def test_attention_hidden_tokens_never_reach_a_row(dtype, value):
     cu = cu_of(lens)
     at = 130 + 120  # a token of the second sequence
     for window in (-1, 40):
-        ref = C().packed_attention(q, k, v, cu, 200, window, True)
+        ref, mag = attention_ref(q[:380], k[:380], v[:380], lens, window, True)
         for which in (k, v):
             x = which.clone()
             x[at], x[380:] = value, value  # and the rows behind the last sequence
@@ -154,7 +154,8 @@ def test_attention_hidden_tokens_never_reach_a_row(dtype, value):
             last = 330 if window < 0 else at + window
             clean = torch.ones(380, dtype=torch.bool, device=DEV)
             clean[at:last] = False
-            assert torch.equal(out[:380][clean], ref[:380][clean])
+            tol = attention_tol(ref, mag, v, 200, dtype)
+            assert ((out[:380].double() - ref).abs() <= tol)[clean].all()
             if which is v:  # the rows that see the value carry it
                 assert not torch.isfinite(out[at:last].float()).any()
             elif math.isnan(value):
