@@ -11,14 +11,15 @@
 // K and V tile and a short prompt still fills rows.  An item has two tiles of
 // consecutive tokens over the same key blocks of 128.
 //
-// A persistent CTA per SM walks the items, long ones first (token blocks by
-// descending index: under a causal mask the work grows with it), 12 warps:
+// The launch has a CTA per item at most, long items first (token blocks by
+// descending index: under a causal mask the work grows with it).  A CTA that has
+// done its item takes over one that has not begun (cluster launch control), so
+// about one CTA per SM runs and the SMs stay balanced.  12 warps:
 //   * warps 0-3 / 4-7: softmax of tile 0 / 1, one thread per row (= TMEM lane);
-//   * warp 8 issues the tcgen05.mma: S = Q K^T (128 x 128 x D) into a tile's 128
-//     score columns, O += P V (128 x D x 128) with P read from tensor memory;
-//   * warp 9 loads Q and the K/V blocks by TMA (128-byte swizzle) into a ring;
-//   * warp 10 finds the next item from cu_seqlens while the others work (warp 11
-//     only completes the warpgroup that hands its registers over).
+//   * warps 8 / 9 issue the tcgen05.mma of tile 0 / 1: S = Q K^T (128 x 128 x D)
+//     into its 128 score columns, O += P V (128 x D x 128), P from tensor memory;
+//   * warp 10 loads Q and the K/V blocks by TMA (128-byte swizzle) into a ring;
+//   * warp 11 finds the next item from cu_seqlens while the others work.
 // The tiles alternate on the tensor pipe: while one tile's scores become
 // weights, the other's products run.  P (16-bit pairs) overwrites the scores it
 // came from; P.V starts on its first 64 keys while the weights of the other 64
@@ -36,6 +37,7 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -47,7 +49,7 @@ namespace packed {
 
 constexpr int kBN = 128;       // keys per block
 constexpr int kMaxGp = 16;     // query heads packed into a tile
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kSchedWarp = 10;
+constexpr int kMmaWarp = 8, kLoadWarp = 10;  // MMA warps 8 and 9, scheduler warp 11
 constexpr int kThreads = 384;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "register split within the launch's registers");
@@ -61,6 +63,7 @@ struct Params {
   int gshift;       // log2 of the heads packed into a tile
   int units;        // head units: H >> gshift
   int tiles;        // tiles per item, 1 or 2
+  int chunk;        // head units walked together
   int window, causal;
   float qscale;     // log2(e) / sqrt(D)
 };
@@ -83,6 +86,7 @@ struct Item {
 
 // Bounded wait: at most 2^22 polls of at most 1 us each.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
   uint32_t polls = 0;
   while (!mbar_try_wait_hint(bar, parity, 1000)) {
     if (++polls >= (1u << 22)) return false;
@@ -126,6 +130,27 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
 template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// Position in the K/V ring: stage and phase of its barriers.
+template <int N>
+struct Slot {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// The exponential unit's 2^x, kept in program order: left free, the compiler
+// moves the second half of a block's exponentials before the first half's store.
+__device__ __forceinline__ float ex2_mufu(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // One row from its definition, by one warp: lane l holds dims [l D/32, (l+1) D/32),
@@ -195,14 +220,14 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
   for (int e = 0; e < E; ++e) dst[e] = pack2<T>(acc[2 * e] / l, acc[2 * e + 1] / l);
 }
 
-// Barriers: items (2 slots: filled by the scheduler, read by the 10 warps
+// Barriers: items (2 slots: filled by the scheduler, read by the 11 warps
 // that work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
 // ready (commit), first and second half of P ready (4 warps), P.V done
 // (commit).
 template <int D>
 struct Bars {
   uint64_t item_full[2], item_free[2], q_full, q_free, kv_full[Cfg<D>::STAGES], kv_free[Cfg<D>::STAGES];
-  uint64_t s_full[2], p_half[2][2], pv_done[2];
+  uint64_t s_full[2], p_half[2][2], pv_done[2], end[2], next, loaded;
 };
 
 template <typename T, int D>
@@ -212,13 +237,16 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   using C = Cfg<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = tc::idesc_f16(128, kBN, false, false, kBf16);
+  constexpr uint32_t kIdescS64 = tc::idesc_f16(128, 64, false, false, kBf16);
   constexpr uint32_t kIdescPV = tc::idesc_f16(128, D, false, true, kBf16);
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) Bars<D> bars;
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) uint4 next_cta;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(base);
   auto at = [](const uint64_t& b) { return smem_u32(&b); };
@@ -227,17 +255,20 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(at(bars.item_full[i]), 1);
-      mbar_init(at(bars.item_free[i]), 10);
+      mbar_init(at(bars.item_free[i]), 11);
       mbar_init(at(bars.s_full[i]), 1);
       mbar_init(at(bars.p_half[i][0]), 4);
       mbar_init(at(bars.p_half[i][1]), 4);
       mbar_init(at(bars.pv_done[i]), 1);
+      mbar_init(at(bars.end[i]), 1);
     }
+    mbar_init(at(bars.next), 1);
+    mbar_init(at(bars.loaded), 1);
     mbar_init(at(bars.q_full), 1);
-    mbar_init(at(bars.q_free), 1);
+    mbar_init(at(bars.q_free), 2);
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(at(bars.kv_full[i]), 1);
-      mbar_init(at(bars.kv_free[i]), 1);
+      mbar_init(at(bars.kv_free[i]), 2);
     }
     fence_mbar_init();
   }
@@ -257,8 +288,13 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   auto next_item = [&](int k, Item& it) -> bool {
     const bool ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_full[k & 1]), (k >> 1) & 1));
     if (!ok) return false;
-    it = items[k & 1];
-    __syncwarp();
+    // Broadcast from one lane: the compiler then keeps what follows from the
+    // item (descriptors, loop bounds) in uniform registers.
+    const Item& src = items[k & 1];
+    it.start = __shfl_sync(0xffffffffu, src.start, 0);
+    it.n = __shfl_sync(0xffffffffu, src.n, 0);
+    it.t0 = __shfl_sync(0xffffffffu, src.t0, 0);
+    it.unit = __shfl_sync(0xffffffffu, src.unit, 0);
     if (lane == 0) mbar_arrive(at(bars.item_free[k & 1]));
     return it.n >= 0;
   };
@@ -281,41 +317,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       const int c = p.causal ? min(tok + 1, it.n) : it.n;
       const int ws = p.window > 0 && c > p.window ? c - p.window : 0;
       float m_run = -INFINITY, l_run = 0.f;
-      for (int j = r.lo; j < r.hi && ok; ++j, ++blocks) {
-        ok = __all_sync(0xffffffffu, wait_bar(at(bars.s_full[t]), blocks & 1));
-        if (!ok) break;
-        tc::fence_after_sync();
-        float s[kBN];
-        {
-          float v0[32], v1[32], v2[32], v3[32];
-          tc::ld32(tS(t) + lane_base, v0);
-          tc::ld32(tS(t) + lane_base + 32, v1);
-          tc::ld32(tS(t) + lane_base + 64, v2);
-          tc::ld32(tS(t) + lane_base + 96, v3);
-          tc::wait_ld(v0);
-          tc::wait_ld(v1);
-          tc::wait_ld(v2);
-          tc::wait_ld(v3);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] = v0[i];
-            s[32 + i] = v1[i];
-            s[64 + i] = v2[i];
-            s[96 + i] = v3[i];
-          }
-        }
-        const int lo = ws - j * kBN, hi = c - j * kBN;  // visible columns [lo, hi)
-        if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
-#pragma unroll
-          for (int i = 0; i < kBN; ++i) s[i] = (i >= lo && i < hi) ? s[i] : -INFINITY;
-        }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < kBN; i += 8) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[i + e]), i + 4 + e < kBN ? s[i + 4 + e] : s[i + e]);
-        }
-        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.qscale);
+      // The running maximum takes a block's maximum in: it moves only when it
+      // grows by more than 2^8, and then O and the sum are rescaled.
+      auto take_max = [&](float mx, int j) -> bool {
+        const float m_new = fmaxf(m_run, mx * p.qscale);  // qscale > 0
         float alpha = 1.f;
         bool rescale = false;
         if (m_run == -INFINITY) {
@@ -327,42 +332,113 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the earlier blocks only once P.V of the last one completed.
-          if (j > r.lo) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
-          if (!ok) break;
+          if (j > r.lo && !__all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1))) return false;
           tc::fence_after_sync();
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t v[16];
+            tc::ld16_wait(tO(t) + lane_base + cc * 16, v);
 #pragma unroll
-          for (int cc = 0; cc < D / 32; ++cc) {
-            float v[32];
-            tc::ld32(tO(t) + lane_base + cc * 32, v);
-            tc::wait_ld(v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= alpha;
-            tc::st32(tO(t) + lane_base + cc * 32, v);
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+            tc::st16(tO(t) + lane_base + cc * 16, v);
           }
           tc::wait_st();
           l_run *= alpha;
         }
-        const float msub = m_run == -INFINITY ? 0.f : m_run;  // nothing visible yet: every weight is 2^-inf = 0
-        const uint64_t nm2 = f32x2_pack(-msub, -msub);
+        return true;
+      };
+      auto p_ready = [&](int half) {
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(at(bars.p_half[t][half]));
+      };
+      for (int j = r.lo; j < r.hi && ok; ++j, ++blocks) {
+        ok = __all_sync(0xffffffffu, wait_bar(at(bars.s_full[t]), blocks & 1));
+        if (!ok) break;
+        tc::fence_after_sync();
+        const int lo = ws - j * kBN, hi = c - j * kBN;  // visible columns [lo, hi)
         uint64_t sum2[4] = {0, 0, 0, 0};
+        if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
+          // An edge of the mask: 32 columns at a time up to the last one that the
+          // tile sees, the maximum first, then the weights from the scores read
+          // again (P of a chunk lies below the scores of the next one).
+          const int chunks = (min(kBN, r.last - j * kBN) + 31) / 32;
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int cc = 0; cc < chunks; ++cc) {
+            float v[32];
+            tc::ld32(tS(t) + lane_base + cc * 32, v);
+            tc::wait_ld(v);
+            const int l = lo - cc * 32, u = hi - cc * 32;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t ph[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int e = half * 64 + 2 * i;
-            float x0, x1;
-            f32x2_unpack(f32x2_fma(f32x2_pack(s[e], s[e + 1]), qs2, nm2), x0, x1);
-            x0 = tc::ex2(x0);
-            x1 = tc::ex2(x1);
-            sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
-            ph[i] = pack2<T>(x0, x1);
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (i >= l && i < u) ? v[i] : -INFINITY);
           }
-          tc::st32u(tS(t) + lane_base + half * 32, ph);
-          tc::wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(at(bars.p_half[t][half]));
+          ok = take_max(mx, j);
+          if (!ok) break;
+          const float msub = m_run == -INFINITY ? 0.f : m_run;  // nothing visible yet: every weight is 2^-inf = 0
+          const uint64_t nm2 = f32x2_pack(-msub, -msub);
+#pragma unroll 1
+          for (int cc = 0; cc < chunks; ++cc) {
+            float v[32];
+            tc::ld32(tS(t) + lane_base + cc * 32, v);
+            tc::wait_ld(v);
+            const int l = lo - cc * 32, u = hi - cc * 32;
+            uint32_t ph[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              f32x2_unpack(f32x2_fma(f32x2_pack((i >= l && i < u) ? v[i] : -INFINITY,
+                                                (i + 1 >= l && i + 1 < u) ? v[i + 1] : -INFINITY), qs2, nm2), x0, x1);
+              x0 = tc::ex2(x0);
+              x1 = tc::ex2(x1);
+              sum2[(i / 2) & 3] = f32x2_add(sum2[(i / 2) & 3], f32x2_pack(x0, x1));
+              ph[i / 2] = pack2<T>(x0, x1);
+            }
+            tc::st16(tS(t) + lane_base + cc * 16, ph);
+            if (cc == 1) p_ready(0);
+          }
+          if (chunks < 2) p_ready(0);
+          p_ready(1);
+        } else {
+          float s[kBN];
+          {
+            float v[4][32];
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) tc::ld32(tS(t) + lane_base + cc * 32, v[cc]);
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+              tc::wait_ld(v[cc]);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[cc * 32 + i] = v[cc][i];
+            }
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < kBN; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[i + e]), s[i + 4 + e < kBN ? i + 4 + e : i + e]);
+          }
+          ok = take_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), j);
+          if (!ok) break;
+          const float msub = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t nm2 = f32x2_pack(-msub, -msub);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t ph[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int e = half * 64 + 2 * i;
+              float x0, x1;
+              f32x2_unpack(f32x2_fma(f32x2_pack(s[e], s[e + 1]), qs2, nm2), x0, x1);
+              x0 = ex2_mufu(x0);
+              x1 = ex2_mufu(x1);
+              sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
+              ph[i] = pack2<T>(x0, x1);
+            }
+            tc::st32u(tS(t) + lane_base + half * 32, ph);
+            p_ready(half);
+          }
         }
         float a0, a1, b0, b1;
         f32x2_unpack(f32x2_add(sum2[0], sum2[1]), a0, a1);
@@ -371,29 +447,54 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       }
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
       tc::fence_after_sync();
-      const bool mine = tok < it.n;
-      T* orow = static_cast<T*>(p.out) + (static_cast<int64_t>(it.start + tok) * p.H + h) * D;
+      // Epilogue: 32 dims of a row are four 16-byte pieces of its thread; the four
+      // threads of neighbouring rows exchange pieces, so that a store writes 64
+      // contiguous bytes of each of 8 rows instead of 16 bytes of 32 rows.
       const float inv = ok ? 1.f / l_run : __int_as_float(0x7fffffff);
       float odd = 0.f;  // becomes NaN when an element is not finite
+      T* rows[4];       // the four rows of this thread's group (null: behind the sequence)
 #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tr = (row & ~3) + i, to = it.t0 + t * tile_tokens + (tr >> p.gshift);
+        const int ho = (it.unit << p.gshift) + (tr & ((1 << p.gshift) - 1));
+        rows[i] = to < it.n ? static_cast<T*>(p.out) + (static_cast<int64_t>(it.start + to) * p.H + ho) * D + (lane & 3) * 8
+                            : nullptr;
+      }
+#pragma unroll 1
       for (int cc = 0; cc < D / 32; ++cc) {
         float v[32];
         tc::ld32(tO(t) + lane_base + cc * 32, v);
         tc::wait_ld(v);
+        uint32_t w[4][4];  // piece, word
 #pragma unroll
-        for (int i = 0; i < 32; ++i) odd = fmaf(v[i], 0.f, odd);
-        if (mine) {
+        for (int i = 0; i < 16; ++i) {
+          odd = fmaf(v[2 * i], 0.f, fmaf(v[2 * i + 1], 0.f, odd));
+          w[i / 4][i % 4] = pack2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
+        }
+        // 4 x 4 transpose: piece c of row r goes to thread c, place r.
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
+        for (int step = 1; step < 4; step <<= 1) {
+          const bool up = lane & step;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack2<T>(v[8 * e + 2 * i] * inv, v[8 * e + 2 * i + 1] * inv);
-            *reinterpret_cast<uint4*>(orow + cc * 32 + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int c = 0; c < 4; ++c) {
+            if (c & step) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[c][i] : w[c + step][i], step);
+              if (up) w[c][i] = got;
+              else w[c + step][i] = got;
+            }
           }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (rows[r]) *reinterpret_cast<uint4*>(rows[r] + cc * 32) = make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
         }
       }
       tc::fence_before_sync();
-      uint32_t redo = __ballot_sync(0xffffffffu, ok && mine && !(odd == 0.f && l_run > 0.f && l_run < INFINITY));
+      // A weight of the row's maximum is at least 1 and no weight exceeds 2^8, so
+      // a sum outside [1/2, 2^100) is not one of finite scores.
+      uint32_t redo = __ballot_sync(0xffffffffu, ok && tok < it.n && !(odd == 0.f && l_run >= 0.5f && l_run < 1.2e30f));
       __syncwarp();
       while (redo) {
         const int from = __ffs(redo) - 1;
@@ -405,91 +506,97 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kMmaWarp) {
-      // ============================== MMA warp ==============================
-      // Warp-uniform code; elect.sync issues each instruction once.
-      const uint64_t dq0 = tc::sdesc_sw128(sbase, 16, 1024);
+    if (warp < kLoadWarp) {
+      // ============================= MMA warps =============================
+      // One warp per tile, so that a wait of one leaves the tensor pipe to the
+      // other.  Warp-uniform code; elect.sync issues each instruction once.
+      // Both follow every K/V block of the item, used or not: a block is free
+      // when both have let it go.
+      const int t = warp - kMmaWarp;
+      const uint64_t dq = tc::sdesc_sw128(sbase + t * C::TILE, 16, 1024);
       const uint64_t dk0 = tc::sdesc_sw128(sbase + C::KV_OFF, 16, 1024);
       const uint64_t dv0 = tc::sdesc_sw128(sbase + C::KV_OFF, C::HALF, 1024);
-      auto wait_all = [&](const uint64_t& b, uint32_t parity) {
-        return __all_sync(0xffffffffu, wait_bar(at(b), parity & 1));
-      };
-      uint32_t loads = 0;                // K/V blocks consumed before this item
-      uint32_t blocks[2] = {0, 0};       // P blocks of each tile so far
+      Slot<C::STAGES> ring;        // of the next block to use
+      uint32_t blocks = 0;         // P blocks of the tile so far
       bool ok = true;
+      auto wait_for = [&](const uint64_t& b, uint32_t parity) { ok &= wait_bar(at(b), parity & 1); };
+      auto in_step = [&] {  // the waits' outcome, the same in every lane
+        ok = __all_sync(0xffffffffu, ok);
+        tc::fence_after_sync();
+        return ok;
+      };
       Item it;
       for (int k = 0; ok && next_item(k, it); ++k) {
-        const Range r[2] = {tile_range(p, it, 0), tile_range(p, it, 1)};
-        const int LO = r[0].lo, HI = max(r[0].hi, r[1].hi);  // tile 0 exists and starts first
-        auto stage_of = [&](int j, int v) { return static_cast<int>((loads + 2u * (j - LO) + v) % C::STAGES); };
-        auto phase_of = [&](int j, int v) { return (loads + 2u * (j - LO) + v) / C::STAGES; };
-        auto in = [&](int t, int j) { return j >= r[t].lo && j < r[t].hi; };
-        auto issue_s = [&](int t, int j) {
-          const uint64_t dk = dk0 + static_cast<uint64_t>((stage_of(j, 0) * C::TILE) >> 4);
-          const uint64_t dq = dq0 + static_cast<uint64_t>((t * C::TILE) >> 4);
+        const Range r0 = tile_range(p, it, 0), r1 = tile_range(p, it, 1);
+        const int LO = r0.lo, HI = max(r0.hi, r1.hi);  // tile 0 exists and starts first
+        const int lo = t ? r1.lo : r0.lo, hi = t ? r1.hi : r0.hi, last = t ? r1.last : r0.last;
+        auto scores = [&](int j) {  // S(j) if the tile has the block; lets K(j) and, at the end, Q go
+          if (j >= lo && j < hi) {
+            // The softmax reads 64 columns where no key behind them is seen.
+            const uint32_t idesc = last - j * kBN > 64 ? kIdescS : kIdescS64;
+            const uint64_t dk = dk0 + static_cast<uint64_t>((ring.stage * C::TILE) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = static_cast<uint64_t>(((kk / 4) * C::HALF + (kk % 4) * 32) >> 4);
-            tc::mma_f16_elect(tS(t), dq + off, dk + off, kIdescS, kk > 0);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint64_t off = static_cast<uint64_t>(((kk / 4) * C::HALF + (kk % 4) * 32) >> 4);
+              tc::mma_f16_elect(tS(t), dq + off, dk + off, idesc, kk > 0);
+            }
+            tc::commit_elect(at(bars.s_full[t]));
           }
-          tc::commit_elect(at(bars.s_full[t]));
-        };
-        // K(j) is there, S(j) of both tiles; then the block and, after the last one, Q are free.
-        auto after_s = [&](int j) {
-          tc::commit_elect(at(bars.kv_free[stage_of(j, 0)]));
+          tc::commit_elect(at(bars.kv_free[ring.stage]));
           if (j == HI - 1) tc::commit_elect(at(bars.q_free));
+          ring.next();
         };
-        ok = wait_all(bars.q_full, k) && wait_all(bars.kv_full[stage_of(LO, 0)], phase_of(LO, 0));
-        if (!ok) break;
-        tc::fence_after_sync();
-        for (int t = 0; t < 2; ++t)
-          if (in(t, LO)) issue_s(t, LO);
-        after_s(LO);
-        const bool tail = HI * kBN > it.n && (it.n & 15);  // the last block runs past the sequence's end
-        for (int j = LO; j < HI && ok; ++j) {
-          ok = wait_all(bars.kv_full[stage_of(j, 1)], phase_of(j, 1));
-          if (ok && tail && j == HI - 1) {
-            // Rows behind the sequence's end, up to the 16 keys of an instruction, become zero.
+        wait_for(bars.q_full, k);
+        wait_for(bars.kv_full[ring.stage], ring.phase);
+        if (!in_step()) break;
+        scores(LO);
+        for (int j = LO; j < HI; ++j) {
+          const Slot<C::STAGES> v = ring;
+          wait_for(bars.kv_full[v.stage], v.phase);
+          if (j == HI - 1 && HI * kBN > it.n && (it.n & 15)) {
+            // The block runs past the sequence's end: its rows there, up to the
+            // 16 keys of an instruction, become zero.
             const int first = it.n - j * kBN, rows = 16 - (first & 15);
-            uint8_t* v0 = base + C::KV_OFF + stage_of(j, 1) * C::TILE + first * 128;
+            uint8_t* v0 = base + C::KV_OFF + v.stage * C::TILE + first * 128;
             for (int i = lane; i < rows * C::HALVES * 8; i += 32)
               *reinterpret_cast<uint4*>(v0 + (i % C::HALVES) * C::HALF + (i / C::HALVES) * 16) = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
-            __syncwarp();
           }
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (in(t, j)) {
-              const uint64_t dv = dv0 + static_cast<uint64_t>((stage_of(j, 1) * C::TILE) >> 4);
-              const int steps = min(kBN, r[t].last - j * kBN + 15) / 16;  // of 16 keys, up to the last one seen
-              for (int half = 0; half < 2 && ok; ++half) {
-                ok = wait_all(bars.p_half[t][half], blocks[t]);
-                if (!ok) break;
-                tc::fence_after_sync();
+          ring.next();
+          if (j + 1 < HI) wait_for(bars.kv_full[ring.stage], ring.phase);
+          if (j >= lo && j < hi) {
+            const uint64_t dv = dv0 + static_cast<uint64_t>((v.stage * C::TILE) >> 4);
+            const int steps = min(kBN, last - j * kBN + 15) / 16;  // of 16 keys, up to the last one seen
+            wait_for(bars.p_half[t][0], blocks);
+            if (!in_step()) break;
 #pragma unroll
-                for (int kk = 4 * half; kk < 4 * half + 4; ++kk) {
-                  if (kk < steps)
-                    tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4),
-                                             kIdescPV, (j > r[t].lo || kk > 0) ? 1u : 0u);
-                }
-              }
-              if (!ok) break;
-              tc::commit_elect(at(bars.pv_done[t]));
-              ++blocks[t];
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk < steps)
+                tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4), kIdescPV,
+                                         (j > lo || kk > 0) ? 1u : 0u);
             }
-            if (j + 1 < HI) {
-              if (t == 0) ok = wait_all(bars.kv_full[stage_of(j + 1, 0)], phase_of(j + 1, 0));
-              if (!ok) break;
-              if (in(t, j + 1)) issue_s(t, j + 1);
+            wait_for(bars.p_half[t][1], blocks);
+            if (!in_step()) break;
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk) {
+              if (kk < steps)
+                tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4), kIdescPV,
+                                         1u);
             }
+            tc::commit_elect(at(bars.pv_done[t]));
+            ++blocks;
+          } else if (!in_step()) {
+            break;
           }
-          if (!ok) break;
-          tc::commit_elect(at(bars.kv_free[stage_of(j, 1)]));
-          if (j + 1 < HI) after_s(j + 1);
+          tc::commit_elect(at(bars.kv_free[v.stage]));
+          if (j + 1 < HI) scores(j + 1);
         }
-        loads += 2u * (HI - LO);
       }
       // The last commit's arrival lands before the CTA ends.
-      if (ok && loads > 0) wait_all(bars.kv_free[(loads - 1) % C::STAGES], (loads - 1) / C::STAGES);
+      if (ok) {
+        tc::commit_elect(at(bars.end[t]));
+        wait_bar(at(bars.end[t]), 0);
+      }
     } else if (warp == kLoadWarp) {
       // ============================== loads ==============================
       if (lane == 0) {
@@ -526,6 +633,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
                             it.start + j * kBN, at(bars.kv_full[st]));
             }
           }
+          if (ok) mbar_arrive(at(bars.loaded));
           if (!ok) {  // nothing may be in flight when the CTA ends
             for (uint32_t u = loads > C::STAGES ? loads - C::STAGES : 0; u < loads; ++u)
               wait_bar(at(bars.kv_full[u % C::STAGES]), (u / C::STAGES) & 1);
@@ -534,10 +642,11 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         ok = __shfl_sync(0xffffffffu, ok, 0);
         loads = __shfl_sync(0xffffffffu, loads, 0);
       }
-    } else if (warp == kSchedWarp) {
+    } else {
       // ============================ scheduler ============================
-      // Items in descending order of token block index L, within one index the
-      // sequences that have it in order, within a sequence the head units.
+      // Head units in chunks (their keys and values stay in L2 while the chunk's
+      // items run); within a chunk items in descending order of token block index
+      // L, within one index the sequences that have it, within a sequence the units.
       const int tokens = tile_tokens * p.tiles;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
         lo = min(max(__ldg(p.cu + s), 0), p.T);
@@ -563,16 +672,48 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         for (int s = lane; s < p.S; s += 32) n += nblocks(s) > L;
         return __reduce_add_sync(0xffffffffu, n);
       };
-      const int64_t total = all * p.units;
-      int L = most - 1, here = total > 0 ? count_above(L) : 0;
+      const int64_t total = all * p.units, per_chunk = all * p.chunk;
+      int L = 0, here = 0, unit0 = -p.chunk;
       int64_t above = 0;  // token blocks of a larger index
-      bool ok = true;
+      bool ok = true, more = true;  // more: there may be CTAs that have not begun
+      int64_t i = blockIdx.x;
+      uint32_t asked = 0;
+      // Takes the index of a CTA that has not begun (the launch has one per item at
+      // most); false when there is none left.
+      auto take_next = [&]() -> bool {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(at(bars.next), 16);
+          tc::try_cancel(smem_u32(&next_cta), at(bars.next));
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, wait_bar(at(bars.next), asked++ & 1));
+        uint32_t cta = 0;
+        const bool got = ok && tc::query_cancel(smem_u32(&next_cta), cta);
+        fence_proxy_async_smem();  // read before the next answer is written
+        __syncwarp();
+        i = cta;
+        return got;
+      };
       for (int k = 0; ok; ++k) {
-        // every other round in reverse: the sums of work differ less between CTAs
-        const int64_t i = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (k >= 2) ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_free[k & 1]), ((k >> 1) - 1) & 1));
+        if (!ok) break;
+        // Not before the loads of the item at hand have been issued: what is taken
+        // early is missing where another CTA runs dry.
+        if (k > 0) {
+          ok = __all_sync(0xffffffffu, wait_bar(at(bars.loaded), (k - 1) & 1));
+          if (!ok) break;
+          more = take_next();
+        }
         Item it{0, -1, 0, 0};
-        if (i < total) {
-          const int64_t b = i / p.units;
+        if (more && i < total) {
+          const int first = static_cast<int>(i / per_chunk) * p.chunk, units = min(p.chunk, p.units - first);
+          const int64_t in_chunk = i - static_cast<int64_t>(first) * all, b = in_chunk / units;
+          if (first != unit0 || b < above) {
+            unit0 = first;
+            above = 0;
+            L = most - 1;
+            here = count_above(L);
+          }
           while (b >= above + here) {
             above += here;
             here = count_above(--L);
@@ -585,14 +726,12 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
               const int s = s0 + static_cast<int>(__fns(has, 0, skip + 1));
               int lo, hi;
               bounds(s, lo, hi);
-              it = Item{lo, hi - lo, L * tokens, static_cast<int>(i - b * p.units)};
+              it = Item{lo, hi - lo, L * tokens, first + static_cast<int>(in_chunk - b * units)};
               break;
             }
             skip -= n;
           }
         }
-        if (k >= 2) ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_free[k & 1]), ((k >> 1) - 1) & 1));
-        if (!ok) break;
         if (lane == 0) {
           items[k & 1] = it;
           mbar_arrive(at(bars.item_full[k & 1]));
@@ -600,6 +739,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         __syncwarp();
         if (it.n < 0) break;
       }
+      // The CTAs past the last item never begin.
+      while (ok && more) more = take_next();
     }
   }
   tc::fence_before_sync();
@@ -643,7 +784,7 @@ int map_rows(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_
 }
 
 template <typename T, int D>
-int launch(const Params& p, int KVH, int grid, cudaStream_t s) {
+int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   alignas(64) CUtensorMap qm, km, vm;
   const int Gp = 1 << p.gshift;
@@ -654,7 +795,7 @@ int launch(const Params& p, int KVH, int grid, cudaStream_t s) {
   auto kern = packed_attention_kernel<T, D>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed_attention)");
-  kern<<<grid, kThreads, Cfg<D>::SMEM, s>>>(p, qm, km, vm);
+  kern<<<static_cast<unsigned>(grid), kThreads, Cfg<D>::SMEM, s>>>(p, qm, km, vm);
   MEMOPT_LAUNCH_CHECK("packed_attention_kernel launch");
   return MEMOPT_OK;
 }
@@ -700,8 +841,14 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   const int64_t tokens = 128 >> p.gshift;
   auto most_items = [&](int tiles) { return (total_tokens / (tokens * tiles) + num_seqs) * p.units; };
   p.tiles = most_items(2) < sm_count() ? 1 : 2;
+  // Head units per chunk: the chunk's keys and values fill about a quarter of L2.
+  // Units that share a KV head stay together.
+  const int per_kv = p.group >> p.gshift;
+  const int64_t kv_bytes = total_tokens * head_dim * 4;
+  p.chunk = static_cast<int>(std::min<int64_t>(p.units, per_kv * std::max<int64_t>(1, (int64_t(32) << 20) / kv_bytes)));
   (void)max_seqlen;
-  const int grid = static_cast<int>(std::min<int64_t>(most_items(p.tiles), sm_count()));
+  const int64_t grid = most_items(p.tiles);
+  if (grid > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many work items");
   cudaStream_t s = as_stream(stream);
   if (dtype == MEMOPT_DTYPE_F16)
     return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, grid, s)

@@ -100,6 +100,31 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t lbo, ui
   return d;
 }
 
+// ---- cluster launch control: take over a CTA of the grid that has not begun --
+// The 16-byte answer lands in shared memory and completes 16 bytes on the
+// mbarrier.  No further request may follow an answer that says "none".
+__device__ __forceinline__ void try_cancel(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   answer),
+               "r"(bar)
+               : "memory");
+}
+// Whether the answer names a CTA; its blockIdx.x.
+__device__ __forceinline__ bool query_cancel(uint32_t answer, uint32_t& cta) {
+  uint32_t got;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=&r"(got), "=&r"(cta)
+      : "r"(answer)
+      : "memory");
+  return got != 0;
+}
+
 // ---- TMEM <-> registers (warp-collective; a warp reaches lanes 32*(warp%4)..) --
 __device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -116,6 +141,17 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 16 columns; the wait is part of it (short transfers off the hot path).
+__device__ __forceinline__ void ld16_wait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void st32(uint32_t taddr, const float (&v)[32]) {
   asm volatile(
