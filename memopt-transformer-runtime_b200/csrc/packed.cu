@@ -11,8 +11,7 @@
 // K and V tile and a short prompt still fills rows.  An item has two tiles of
 // consecutive tokens over the same key blocks of 128.
 //
-// The launch has a CTA per item at most, long items first (token blocks by
-// descending index: under a causal mask the work grows with it).  A CTA that has
+// The launch has a CTA per item at most, long items first.  A CTA that has
 // done its item takes over one that has not begun (cluster launch control), so
 // about one CTA per SM runs and the SMs stay balanced.  12 warps:
 //   * warps 0-3 / 4-7: softmax of tile 0 / 1, one thread per row (= TMEM lane);
@@ -48,6 +47,8 @@ namespace memopt {
 namespace packed {
 
 constexpr int kBN = 128;       // keys per block
+constexpr int kFirst = 6;       // of the 8 steps of 16 keys, those that P.V starts with
+constexpr int kAhead = 3;       // blocks before an item's last loads at which the next item is taken
 constexpr int kMaxGp = 16;     // query heads packed into a tile
 constexpr int kMmaWarp = 8, kLoadWarp = 10;  // MMA warps 8 and 9, scheduler warp 11
 constexpr int kThreads = 384;
@@ -76,6 +77,9 @@ struct Cfg {
   static constexpr int STAGES = D == 128 ? 5 : 8;
   static constexpr int KV_OFF = 2 * TILE;
   static constexpr int SMEM = KV_OFF + STAGES * TILE + 1024;  // + alignment slack
+  // With D = 64 tensor memory has room for P beside the scores: the next scores
+  // are computed while the weights are, and a block takes its softmax alone.
+  static constexpr bool OWN_P = 2 * (kBN + D + kBN / 2) <= 512;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(2 * (kBN + D) <= 512, "tensor memory columns");
 };
@@ -222,12 +226,12 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
 
 // Barriers: items (2 slots: filled by the scheduler, read by the 11 warps
 // that work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
-// ready (commit), first and second half of P ready (4 warps), P.V done
+// ready (commit), first and second part of P ready (4 warps), P.V done
 // (commit).
 template <int D>
 struct Bars {
   uint64_t item_full[2], item_free[2], q_full, q_free, kv_full[Cfg<D>::STAGES], kv_free[Cfg<D>::STAGES];
-  uint64_t s_full[2], p_half[2][2], pv_done[2], end[2], next, loaded;
+  uint64_t s_full[2], p_part[2][2], pv_done[2], s_read[2], end[2], next, near_end;
 };
 
 template <typename T, int D>
@@ -257,13 +261,14 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       mbar_init(at(bars.item_full[i]), 1);
       mbar_init(at(bars.item_free[i]), 11);
       mbar_init(at(bars.s_full[i]), 1);
-      mbar_init(at(bars.p_half[i][0]), 4);
-      mbar_init(at(bars.p_half[i][1]), 4);
+      mbar_init(at(bars.p_part[i][0]), 4);
+      mbar_init(at(bars.p_part[i][1]), 4);
       mbar_init(at(bars.pv_done[i]), 1);
+      mbar_init(at(bars.s_read[i]), 4);
       mbar_init(at(bars.end[i]), 1);
     }
     mbar_init(at(bars.next), 1);
-    mbar_init(at(bars.loaded), 1);
+    mbar_init(at(bars.near_end), 1);
     mbar_init(at(bars.q_full), 1);
     mbar_init(at(bars.q_free), 2);
     for (int i = 0; i < C::STAGES; ++i) {
@@ -280,9 +285,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  // Tile t: scores (and P) at columns 128 t, O at 256 + D t.
+  // Tile t: scores at columns 128 t, O at 256 + D t, P over the scores or behind O.
   auto tS = [&](int t) { return tmem + 128u * t; };
   auto tO = [&](int t) { return tmem + 256u + static_cast<uint32_t>(D) * t; };
+  auto tP = [&](int t) { return C::OWN_P ? tmem + 256u + 2u * D + 64u * t : tS(t); };
 
   // The k-th item of this CTA (read by every warp but the scheduler).
   auto next_item = [&](int k, Item& it) -> bool {
@@ -347,11 +353,23 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         return true;
       };
+      // The scores are in registers: the next ones may overwrite them (OWN_P).
+      auto s_read = [&] {
+        if (!C::OWN_P) return;
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(at(bars.s_read[t]));
+      };
+      // P of the last block is no longer needed (OWN_P; else its scores say so).
+      auto p_free = [&](int j) -> bool {
+        if (!C::OWN_P || j == r.lo) return true;
+        return __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
+      };
       auto p_ready = [&](int half) {
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(at(bars.p_half[t][half]));
+        if (lane == 0) mbar_arrive(at(bars.p_part[t][half]));
       };
       for (int j = r.lo; j < r.hi && ok; ++j, ++blocks) {
         ok = __all_sync(0xffffffffu, wait_bar(at(bars.s_full[t]), blocks & 1));
@@ -362,43 +380,54 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
           // An edge of the mask: 32 columns at a time up to the last one that the
           // tile sees, the maximum first, then the weights from the scores read
-          // again (P of a chunk lies below the scores of the next one).
+          // again (where P lies over the scores, P of a chunk is below the scores of
+          // the next one).
           const int chunks = (min(kBN, r.last - j * kBN) + 31) / 32;
+          auto chunk = [&](int cc, float (&v)[32]) {
+            tc::ld32(tS(t) + lane_base + cc * 32, v);
+            tc::wait_ld(v);
+            const int l = lo - cc * 32, u = hi - cc * 32;
+            if (__any_sync(0xffffffffu, l > 0 || u < 32)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = (i >= l && i < u) ? v[i] : -INFINITY;
+            }
+          };
           float mx = -INFINITY;
 #pragma unroll 1
           for (int cc = 0; cc < chunks; ++cc) {
             float v[32];
-            tc::ld32(tS(t) + lane_base + cc * 32, v);
-            tc::wait_ld(v);
-            const int l = lo - cc * 32, u = hi - cc * 32;
+            chunk(cc, v);
+            float m0 = v[0], m1 = v[1];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (i >= l && i < u) ? v[i] : -INFINITY);
+            for (int i = 2; i < 32; i += 2) {
+              m0 = fmaxf(m0, v[i]);
+              m1 = fmaxf(m1, v[i + 1]);
+            }
+            mx = fmaxf(mx, fmaxf(m0, m1));
           }
-          ok = take_max(mx, j);
+          ok = take_max(mx, j) && p_free(j);
           if (!ok) break;
           const float msub = m_run == -INFINITY ? 0.f : m_run;  // nothing visible yet: every weight is 2^-inf = 0
           const uint64_t nm2 = f32x2_pack(-msub, -msub);
 #pragma unroll 1
           for (int cc = 0; cc < chunks; ++cc) {
             float v[32];
-            tc::ld32(tS(t) + lane_base + cc * 32, v);
-            tc::wait_ld(v);
-            const int l = lo - cc * 32, u = hi - cc * 32;
+            chunk(cc, v);
+            if (cc == chunks - 1) s_read();
             uint32_t ph[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+            for (int i = 0; i < 16; ++i) {
               float x0, x1;
-              f32x2_unpack(f32x2_fma(f32x2_pack((i >= l && i < u) ? v[i] : -INFINITY,
-                                                (i + 1 >= l && i + 1 < u) ? v[i + 1] : -INFINITY), qs2, nm2), x0, x1);
+              f32x2_unpack(f32x2_fma(f32x2_pack(v[2 * i], v[2 * i + 1]), qs2, nm2), x0, x1);
               x0 = tc::ex2(x0);
               x1 = tc::ex2(x1);
-              sum2[(i / 2) & 3] = f32x2_add(sum2[(i / 2) & 3], f32x2_pack(x0, x1));
-              ph[i / 2] = pack2<T>(x0, x1);
+              sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
+              ph[i] = pack2<T>(x0, x1);
             }
-            tc::st16(tS(t) + lane_base + cc * 16, ph);
-            if (cc == 1) p_ready(0);
+            tc::st16(tP(t) + lane_base + cc * 16, ph);
+            if (2 * (cc + 1) == kFirst) p_ready(0);
           }
-          if (chunks < 2) p_ready(0);
+          if (2 * chunks < kFirst) p_ready(0);
           p_ready(1);
         } else {
           float s[kBN];
@@ -413,6 +442,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
               for (int i = 0; i < 32; ++i) s[cc * 32 + i] = v[cc][i];
             }
           }
+          s_read();
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
           for (int i = 4; i < kBN; i += 8) {
@@ -423,22 +453,26 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           if (!ok) break;
           const float msub = m_run == -INFINITY ? 0.f : m_run;
           const uint64_t nm2 = f32x2_pack(-msub, -msub);
+          ok = p_free(j);
+          if (!ok) break;
+          // 32 keys at a time; P.V starts on the first kFirst steps of 16 keys.
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t ph[32];
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t ph[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int e = half * 64 + 2 * i;
+            for (int i = 0; i < 16; ++i) {
+              const int e = cc * 32 + 2 * i;
               float x0, x1;
               f32x2_unpack(f32x2_fma(f32x2_pack(s[e], s[e + 1]), qs2, nm2), x0, x1);
               x0 = ex2_mufu(x0);
               x1 = ex2_mufu(x1);
-              sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
+              sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));  // the row sum adds them unrounded
               ph[i] = pack2<T>(x0, x1);
             }
-            tc::st32u(tS(t) + lane_base + half * 32, ph);
-            p_ready(half);
+            tc::st16(tP(t) + lane_base + cc * 16, ph);
+            if (2 * (cc + 1) == kFirst) p_ready(0);
           }
+          p_ready(1);
         }
         float a0, a1, b0, b1;
         f32x2_unpack(f32x2_add(sum2[0], sum2[1]), a0, a1);
@@ -564,32 +598,33 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           }
           ring.next();
           if (j + 1 < HI) wait_for(bars.kv_full[ring.stage], ring.phase);
+          if (C::OWN_P && j + 1 < HI) {
+            if (j >= lo && j < hi) wait_for(bars.s_read[t], blocks);
+            if (!in_step()) break;
+            scores(j + 1);
+          }
           if (j >= lo && j < hi) {
             const uint64_t dv = dv0 + static_cast<uint64_t>((v.stage * C::TILE) >> 4);
             const int steps = min(kBN, last - j * kBN + 15) / 16;  // of 16 keys, up to the last one seen
-            wait_for(bars.p_half[t][0], blocks);
-            if (!in_step()) break;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk < steps)
-                tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4), kIdescPV,
-                                         (j > lo || kk > 0) ? 1u : 0u);
-            }
-            wait_for(bars.p_half[t][1], blocks);
-            if (!in_step()) break;
+            for (int part = 0; part < 2; ++part) {
+              wait_for(bars.p_part[t][part], blocks);
+              if (!in_step()) break;
 #pragma unroll
-            for (int kk = 4; kk < 8; ++kk) {
-              if (kk < steps)
-                tc::mma_f16_tmem_a_elect(tO(t), tS(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4), kIdescPV,
-                                         1u);
+              for (int kk = part ? kFirst : 0; kk < (part ? 8 : kFirst); ++kk) {
+                if (kk < steps)
+                  tc::mma_f16_tmem_a_elect(tO(t), tP(t) + 8u * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4),
+                                           kIdescPV, (j > lo || kk > 0) ? 1u : 0u);
+              }
             }
+            if (!ok) break;
             tc::commit_elect(at(bars.pv_done[t]));
             ++blocks;
           } else if (!in_step()) {
             break;
           }
           tc::commit_elect(at(bars.kv_free[v.stage]));
-          if (j + 1 < HI) scores(j + 1);
+          if (!C::OWN_P && j + 1 < HI) scores(j + 1);
         }
       }
       // The last commit's arrival lands before the CTA ends.
@@ -622,6 +657,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
                             it.start + it.t0 + t * tile_tokens, at(bars.q_full));
           }
           for (int j = LO; j < HI && ok; ++j) {
+            if (j == max(HI - kAhead, LO)) mbar_arrive(at(bars.near_end));
             for (int v = 0; v < 2 && ok; ++v, ++loads) {
               const int st = loads % C::STAGES;
               const uint32_t use = loads / C::STAGES;
@@ -633,7 +669,6 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
                             it.start + j * kBN, at(bars.kv_full[st]));
             }
           }
-          if (ok) mbar_arrive(at(bars.loaded));
           if (!ok) {  // nothing may be in flight when the CTA ends
             for (uint32_t u = loads > C::STAGES ? loads - C::STAGES : 0; u < loads; ++u)
               wait_bar(at(bars.kv_full[u % C::STAGES]), (u / C::STAGES) & 1);
@@ -645,8 +680,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     } else {
       // ============================ scheduler ============================
       // Head units in chunks (their keys and values stay in L2 while the chunk's
-      // items run); within a chunk items in descending order of token block index
-      // L, within one index the sequences that have it, within a sequence the units.
+      // items run); within a chunk the items in descending order of work, within a
+      // token block the units.
       const int tokens = tile_tokens * p.tiles;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
         lo = min(max(__ldg(p.cu + s), 0), p.T);
@@ -667,14 +702,32 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
       for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-      auto count_above = [&](int L) {  // sequences with a token block of index L
+      // Token blocks are walked level by level.  Causal: level = index of the
+      // block in its sequence, descending; a sequence has one block on it if it
+      // is long enough.  Not causal: level = blocks of the sequence, descending;
+      // a sequence of that many has all of them on it.
+      auto on_level = [&](int s, int L) {
+        const int nb = nblocks(s);
+        return p.causal ? nb > L : nb == L;
+      };
+      auto count_on = [&](int L) {  // token blocks on a level
         int n = 0;
-        for (int s = lane; s < p.S; s += 32) n += nblocks(s) > L;
-        return __reduce_add_sync(0xffffffffu, n);
+        for (int s = lane; s < p.S; s += 32) n += on_level(s, L);
+        n = __reduce_add_sync(0xffffffffu, n);
+        return p.causal ? static_cast<int64_t>(n) : static_cast<int64_t>(n) * L;
+      };
+      auto next_level = [&](int L) {
+        if (p.causal) return L - 1;
+        int below = 0;
+        for (int s = lane; s < p.S; s += 32) {
+          const int nb = nblocks(s);
+          if (nb < L) below = max(below, nb);
+        }
+        return static_cast<int>(__reduce_max_sync(0xffffffffu, below));
       };
       const int64_t total = all * p.units, per_chunk = all * p.chunk;
-      int L = 0, here = 0, unit0 = -p.chunk;
-      int64_t above = 0;  // token blocks of a larger index
+      int L = 0, unit0 = -p.chunk;
+      int64_t above = 0, here = 0;  // token blocks on the levels above, on this one
       bool ok = true, more = true;  // more: there may be CTAs that have not begun
       int64_t i = blockIdx.x;
       uint32_t asked = 0;
@@ -697,10 +750,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       for (int k = 0; ok; ++k) {
         if (k >= 2) ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_free[k & 1]), ((k >> 1) - 1) & 1));
         if (!ok) break;
-        // Not before the loads of the item at hand have been issued: what is taken
-        // early is missing where another CTA runs dry.
+        // Not before the item at hand nears its end: what is taken early is missing
+        // where another CTA runs dry.  The answer takes up to 10 us.
         if (k > 0) {
-          ok = __all_sync(0xffffffffu, wait_bar(at(bars.loaded), (k - 1) & 1));
+          ok = __all_sync(0xffffffffu, wait_bar(at(bars.near_end), (k - 1) & 1));
           if (!ok) break;
           more = take_next();
         }
@@ -711,22 +764,24 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           if (first != unit0 || b < above) {
             unit0 = first;
             above = 0;
-            L = most - 1;
-            here = count_above(L);
+            L = p.causal ? most - 1 : most;
+            here = count_on(L);
           }
           while (b >= above + here) {
             above += here;
-            here = count_above(--L);
+            L = next_level(L);
+            here = count_on(L);
           }
-          int skip = static_cast<int>(b - above);
+          const int per_seq = p.causal ? 1 : L, at_level = static_cast<int>(b - above);
+          int skip = at_level / per_seq;  // sequences on the level before the one
           for (int s0 = 0; s0 < p.S; s0 += 32) {
-            const uint32_t has = __ballot_sync(0xffffffffu, nblocks(s0 + lane) > L);
+            const uint32_t has = __ballot_sync(0xffffffffu, on_level(s0 + lane, L));
             const int n = __popc(has);
             if (skip < n) {
               const int s = s0 + static_cast<int>(__fns(has, 0, skip + 1));
               int lo, hi;
               bounds(s, lo, hi);
-              it = Item{lo, hi - lo, L * tokens, first + static_cast<int>(in_chunk - b * units)};
+              it = Item{lo, hi - lo, (p.causal ? L : at_level % L) * tokens, first + static_cast<int>(in_chunk - b * units)};
               break;
             }
             skip -= n;
