@@ -16,9 +16,14 @@
 // Everything is held in fp32 and rounded once per output.  Bound by HBM: q and
 // k read and written once, v read once, the K and V rows written to the pool.
 // A lane owns 16 dims of a head (two 16-byte vectors holding 8 whole pairs),
-// D/16 lanes a head, a warp 512 / D heads at a time; a token's 8 cos/sin pairs
-// per lane are computed once, shared out over the lanes that need the same
-// ones, and used for every head of the token.
+// D/16 lanes a head, a warp 512 / D heads at a time (a step).  A CTA takes a few
+// tokens: its warps put their first loads in flight, the threads compute the
+// (cos, sin) of the tokens' pairs once into shared memory, and every step reads
+// them there.  Small CTAs of two warps, each with one batch of loads: on 32768
+// tokens x 64 heads of 128 with the cache (1.88 GB) 297 us = 6.33 TB/s, against
+// 306 to 349 us with four or eight warps, 2 to 4 steps in flight or up to four
+// batches a warp; holding (cos, sin) in registers for all heads of a token and a
+// grid of resident warps took 316 us (28.6 against 25.6 us on 4099 tokens).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -28,8 +33,9 @@
 namespace memopt {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 2;
 constexpr int kMaxAxes = 4;
+constexpr int kBatch = 4;  // steps whose loads a lane has in flight
 
 struct RotaryArgs {
   const void *q, *k, *v;
@@ -40,7 +46,8 @@ struct RotaryArgs {
   __half *kc, *vc;
   int64_t T, q_stride, k_stride, v_stride;  // strides in elements
   int64_t num_slots;
-  int H, KVH, P, axes, split;
+  int H, KVH, P, axes;
+  int steps, tokens;  // warp steps over a token's heads; tokens of a CTA
   int ends[kMaxAxes];  // axis a owns the pairs below ends[a] and from ends[a - 1] on
 };
 
@@ -81,110 +88,103 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
                     Pair<T>::put(f[6], f[7]));
 }
 
-// Both vectors of a lane's unit, rotated (in fp32).
+// Both vectors of a lane's unit, rotated (in fp32); cs holds the (cos, sin) of
+// its 8 pairs, two to a float4.
 template <bool kInterleaved>
-__device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
-  if (kInterleaved) {  // a holds pairs 0..3 of the unit, b pairs 4..7
+__device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], const float4* cs) {
+  auto one = [](float& x, float& y, float c, float s) {
+    const float z = x;
+    x = z * c - y * s;
+    y = z * s + y * c;
+  };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-      a[2 * i] = x * c[i] - y * s[i];
-      a[2 * i + 1] = x * s[i] + y * c[i];
-      b[2 * i] = z * c[4 + i] - w * s[4 + i];
-      b[2 * i + 1] = z * s[4 + i] + w * c[4 + i];
-    }
-  } else {  // a holds the first dims of the 8 pairs, b the second ones
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = x * c[i] - y * s[i];
-      b[i] = x * s[i] + y * c[i];
+  for (int i = 0; i < 4; ++i) {
+    const float4 v = cs[i];
+    if (kInterleaved) {  // a holds pairs 0..3 of the unit, b pairs 4..7
+      float(&x)[8] = i < 2 ? a : b;
+      const int e = 4 * (i & 1);
+      one(x[e], x[e + 1], v.x, v.y);
+      one(x[e + 2], x[e + 3], v.z, v.w);
+    } else {  // a holds the first dims of the 8 pairs, b the second ones
+      one(a[2 * i], b[2 * i], v.x, v.y);
+      one(a[2 * i + 1], b[2 * i + 1], v.z, v.w);
     }
   }
 }
 
 template <typename T, int D, bool kInterleaved>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryArgs p) {
-  constexpr int U = D / 16;         // units (lanes) per head
-  constexpr int HPW = 32 / U;       // heads per warp step
-  constexpr int OWN = 8 / HPW;      // cos/sin pairs a lane computes itself
-  const int lane = threadIdx.x & 31, u = lane % U, sub = lane / U;
+  constexpr int U = D / 16;    // units (lanes) per head
+  constexpr int HPW = 32 / U;  // heads per warp step
+  extern __shared__ float2 turns[];  // (cos, sin) of pair i of the CTA's k-th token at [k][i]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = lane % U, sub = lane / U;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+  const int tokens = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.T - t0));
   const bool rotary = u < p.P / 8;
   // Dims of the unit's two vectors; units past the rotary ones cover the rest of the head.
   const int d0 = (!rotary || kInterleaved) ? 16 * u : 8 * u;
   const int d1 = (!rotary || kInterleaved) ? 16 * u + 8 : p.P + 8 * u;
+  // Heads of a token: those of q, of k and, with a cache, of v (which only move).
+  const int heads = p.H + p.KVH + (p.slots ? p.KVH : 0);
+  const int all = tokens * p.steps;  // warp steps of the CTA
 
-  // This lane's own pairs: frequency in turns (64-bit fraction) and axis.
-  uint64_t turns[OWN];
-  int axis[OWN];
+  uint4 ua[kBatch], ub[kBatch];
+  auto load = [&](int st0) {  // a batch of this warp's steps: st0, st0 + kWarps, ...
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    turns[i] = 0;
-    axis[i] = 0;
-    if (rotary) {
-      const int pair = 8 * u + sub * OWN + i;
-      const double f = __ldg(p.freq + pair) * 0.15915494309189535;  // 1 / (2 pi)
-      turns[i] = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
-      for (int a = 0; a + 1 < p.axes; ++a) axis[i] += pair >= p.ends[a];
+    for (int i = 0; i < kBatch; ++i) {
+      const int st = st0 + i * kWarps, k = st / p.steps, h = (st - k * p.steps) * HPW + sub;
+      if (st < all && h < heads) {
+        const int64_t t = t0 + k;
+        const T* src = h < p.H ? static_cast<const T*>(p.q) + t * p.q_stride + h * D
+                       : h < p.H + p.KVH
+                           ? static_cast<const T*>(p.k) + t * p.k_stride + (h - p.H) * D
+                           : static_cast<const T*>(p.v) + t * p.v_stride + (h - p.H - p.KVH) * D;
+        ua[i] = ld_stream_v4(src + d0);
+        ub[i] = ld_stream_v4(src + d1);
+      }
     }
+  };
+  load(warp);
+  // The angles of the CTA's tokens while the first loads are in flight.
+  for (int i = tid; i < tokens * p.P; i += kWarps * 32) {
+    const int k = i / p.P, pair = i - k * p.P;
+    int axis = 0;
+    for (int a = 0; a + 1 < p.axes; ++a) axis += pair >= p.ends[a];
+    const double f = __ldg(p.freq + pair) * 0.15915494309189535;  // 1 / (2 pi)
+    const uint64_t turn64 = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+    const int64_t pos = __ldg(p.pos + axis * p.T + t0 + k);
+    const uint64_t w = static_cast<uint64_t>(pos) * turn64;
+    float cs, sn;
+    // the top 32 bits as a signed fraction of a turn, in half turns
+    sincospif(static_cast<float>(static_cast<int32_t>(w >> 32)) * 4.656612873077393e-10f, &sn, &cs);
+    turns[i] = make_float2(cs, sn);
   }
-
-  const int heads = p.H + p.KVH;
-  const int steps = (heads + HPW - 1) / HPW;
-  const int64_t items = p.T * p.split;
-  const int64_t nwarps = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); it < items; it += nwarps) {
-    const int64_t t = it / p.split;
-    const int part = static_cast<int>(it - t * p.split);
-    float c[8], s[8];
-    {
-      float oc[OWN], os[OWN];
+  __syncthreads();
+  for (int st0 = warp; st0 < all; st0 += kBatch * kWarps) {
+    if (st0 > warp) load(st0);
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int64_t pos = __ldg(p.pos + axis[i] * p.T + t);
-        const uint64_t w = static_cast<uint64_t>(pos) * turns[i];
-        // the top 32 bits as a signed fraction of a turn, in half turns
-        sincospif(static_cast<float>(static_cast<int32_t>(w >> 32)) * 4.656612873077393e-10f, &os[i], &oc[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int from = (i / OWN) * U + u;
-        c[i] = __shfl_sync(0xffffffffu, oc[i % OWN], from);
-        s[i] = __shfl_sync(0xffffffffu, os[i % OWN], from);
-      }
-    }
-    int64_t slot = -1;
-    if (p.slots) {
-      slot = __ldg(p.slots + t);
-      if (slot >= p.num_slots) slot = -1;
-    }
-    const int lo = static_cast<int>(static_cast<int64_t>(steps) * part / p.split);
-    const int hi = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.split);
-#pragma unroll 2
-    for (int st = lo; st < hi; ++st) {
-      const int h = st * HPW + sub;
-      if (h >= heads) continue;
-      const bool is_k = h >= p.H;
-      const int hk = h - p.H;
-      const T* src = is_k ? static_cast<const T*>(p.k) + t * p.k_stride + hk * D
-                          : static_cast<const T*>(p.q) + t * p.q_stride + h * D;
+    for (int i = 0; i < kBatch; ++i) {
+      const int st = st0 + i * kWarps, k = st / p.steps, h = (st - k * p.steps) * HPW + sub;
+      if (st >= all || h >= heads) continue;
+      const int64_t t = t0 + k;
+      const bool is_v = h >= p.H + p.KVH;
       float a[8], b[8];
-      unpack8<T>(ld_stream_v4(src + d0), a);
-      unpack8<T>(ld_stream_v4(src + d1), b);
-      if (rotary) turn<kInterleaved>(a, b, c, s);
-      T* dst = is_k ? static_cast<T*>(p.k_out) + (t * p.KVH + hk) * D : static_cast<T*>(p.q_out) + (t * p.H + h) * D;
-      *reinterpret_cast<uint4*>(dst + d0) = pack8<T>(a);
-      *reinterpret_cast<uint4*>(dst + d1) = pack8<T>(b);
-      if (is_k && slot >= 0) {
-        __half* kd = p.kc + (slot * p.KVH + hk) * D;
-        *reinterpret_cast<uint4*>(kd + d0) = pack8<__half>(a);
-        *reinterpret_cast<uint4*>(kd + d1) = pack8<__half>(b);
-        const T* vs = static_cast<const T*>(p.v) + t * p.v_stride + hk * D;
-        __half* vd = p.vc + (slot * p.KVH + hk) * D;
-        unpack8<T>(ld_stream_v4(vs + d0), a);
-        unpack8<T>(ld_stream_v4(vs + d1), b);
-        *reinterpret_cast<uint4*>(vd + d0) = pack8<__half>(a);
-        *reinterpret_cast<uint4*>(vd + d1) = pack8<__half>(b);
+      unpack8<T>(ua[i], a);
+      unpack8<T>(ub[i], b);
+      if (rotary && !is_v) turn<kInterleaved>(a, b, reinterpret_cast<const float4*>(turns + k * p.P + 8 * u));
+      if (!is_v) {
+        T* dst = h < p.H ? static_cast<T*>(p.q_out) + (t * p.H + h) * D
+                         : static_cast<T*>(p.k_out) + (t * p.KVH + (h - p.H)) * D;
+        *reinterpret_cast<uint4*>(dst + d0) = pack8<T>(a);
+        *reinterpret_cast<uint4*>(dst + d1) = pack8<T>(b);
+      }
+      if (h >= p.H && p.slots) {
+        const int64_t slot = __ldg(p.slots + t);
+        if (slot >= 0 && slot < p.num_slots) {
+          __half* dst = is_v ? p.vc + (slot * p.KVH + (h - p.H - p.KVH)) * D : p.kc + (slot * p.KVH + (h - p.H)) * D;
+          *reinterpret_cast<uint4*>(dst + d0) = pack8<__half>(a);
+          *reinterpret_cast<uint4*>(dst + d1) = pack8<__half>(b);
+        }
       }
     }
   }
@@ -193,9 +193,11 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T, int D>
-int launch_rotary(const RotaryArgs& p, bool interleaved, int grid, cudaStream_t s) {
-  if (interleaved) rotary_kernel<T, D, true><<<grid, kWarps * 32, 0, s>>>(p);
-  else rotary_kernel<T, D, false><<<grid, kWarps * 32, 0, s>>>(p);
+int launch_rotary(const RotaryArgs& p, bool interleaved, int64_t ctas, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(ctas);
+  const size_t smem = sizeof(float2) * p.tokens * p.P;
+  if (interleaved) rotary_kernel<T, D, true><<<grid, kWarps * 32, smem, s>>>(p);
+  else rotary_kernel<T, D, false><<<grid, kWarps * 32, smem, s>>>(p);
   MEMOPT_LAUNCH_CHECK("rotary_kernel launch");
   return MEMOPT_OK;
 }
@@ -246,13 +248,11 @@ extern "C" int memopt_rotary_write_cache(const void* query, int64_t query_stride
   p.kc = static_cast<__half*>(key_pool), p.vc = static_cast<__half*>(value_pool);
   p.T = num_tokens, p.num_slots = cache ? num_blocks * block_size : 0;
   p.H = num_heads, p.KVH = num_kv_heads, p.P = num_pairs, p.axes = num_axes;
-  // Few tokens: a token's heads are split over several warps, so that a decode
-  // step fills the GPU; the cos/sin are then computed once per part.
-  const int hpw = 512 / head_dim, steps = (num_heads + num_kv_heads + hpw - 1) / hpw;
-  const int64_t want = static_cast<int64_t>(sm_count()) * 16;
-  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(steps, want / num_tokens)));
-  const int64_t items = num_tokens * p.split;
-  const int grid = static_cast<int>(std::min<int64_t>((items + kWarps - 1) / kWarps, static_cast<int64_t>(sm_count()) * 8));
+  const int hpw = 512 / head_dim, heads = num_heads + num_kv_heads * (cache ? 2 : 1);
+  p.steps = (heads + hpw - 1) / hpw;
+  p.tokens = std::max(1, kBatch * kWarps / p.steps);
+  const int64_t grid = (num_tokens + p.tokens - 1) / p.tokens;
+  if (grid > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, "rotary: too many tokens");
   cudaStream_t s = as_stream(stream);
   const bool il = interleaved != 0;
   if (dtype == MEMOPT_DTYPE_F16)
