@@ -400,7 +400,8 @@ int memopt_paged_attention_int4(const void* query, const uint8_t* kv_pages,
 /* (page * block_size + offset) and its position in the sequence              */
 /* (slot_mapping and positions int32 [max_tokens], 16-byte aligned, -1 and 0  */
 /* past the last token), and the batch's own rows: batch_tables [batch,       */
-/* max_blocks_per_seq] and batch_lens [batch] with the new tokens.  A refused */
+/* max_blocks_per_seq] (-1 behind a row's pages) and batch_lens [batch] with   */
+/* the new tokens.  A refused */
 /* call writes zero cu_seqlens and slots of -1 (which write_cache skips).     */
 /* batch <= 8192, num_rows <= 262144, num_blocks * block_size < 2^31.         */
 int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_rows, int max_blocks_per_seq,

@@ -96,12 +96,20 @@ std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tens
   rows = rows.contiguous();
   new_lens = new_lens.contiguous();
   const at::cuda::CUDAGuard g(block_tables.device());
-  const auto o = block_tables.options();
-  auto cu = torch::empty({n.B + 1}, o);
-  auto slots = torch::empty({max_tokens}, o);
-  auto positions = torch::empty({max_tokens}, o);
-  auto tables = torch::empty({n.B, n.MB}, o);
-  auto lens = torch::empty({n.B}, o);
+  // One allocation behind the five outputs (an allocation each costs the host
+  // more than the launch), every one 16-byte aligned.
+  auto up4 = [](int64_t v) { return (v + 3) & ~int64_t(3); };
+  const int64_t at_pos = up4(max_tokens), at_tables = at_pos + up4(max_tokens);
+  const int64_t at_cu = at_tables + up4(static_cast<int64_t>(n.B) * n.MB), at_lens = at_cu + up4(n.B + 1);
+  const auto buf = torch::empty({at_lens + n.B}, block_tables.options());
+  auto part = [&](int64_t at, at::IntArrayRef sizes) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  };
+  auto slots = part(0, {max_tokens}), positions = part(at_pos, {max_tokens});
+  auto tables = part(at_tables, {n.B, n.MB}), cu = part(at_cu, {n.B + 1}), lens = part(at_lens, {n.B});
   check(memopt_reserve_slots(block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(), n.R, n.MB,
                              free_pages.data_ptr<int32_t>(), n.NB, pool_state.data_ptr<int32_t>(),
                              rows.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n.B, block_size, max_tokens,

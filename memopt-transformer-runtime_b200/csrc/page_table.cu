@@ -16,13 +16,14 @@
 //             page order.
 //
 // One launch each: every CTA reads the old lengths and the old ring state and
-// repeats the scan over the batch in shared memory (a few loads per thread;
-// no CTA waits for another), then expands its share of the tokens and of the
-// table rows.  The CTA that arrives last at a ticket in the pool state commits
-// the new lengths, head and count, so nothing reads a value that the same call
-// wrote.  Whole numbers only; bound by the launch and the two dependent loads
-// (row, length) except for very large batches, where the 8 bytes written per
-// token count.
+// repeats the scan over the batch in shared memory (no CTA waits for another),
+// then expands its share of the tokens and of the table rows.  The CTA that
+// arrives last at a ticket in the pool state commits the new lengths, head and
+// count, so nothing reads a value that the same call wrote.  Whole numbers only;
+// bound by latency: the launch, the dependent loads row -> length -> page, the
+// fence and the ticket.  Hence a warp per table row with its entries in flight at
+// once, and CTAs of 256 threads, or of 1024 where the batch is larger than 256
+// rows (the scan is then still one round of loads).
 #include <algorithm>
 
 #include "common.cuh"
@@ -30,8 +31,8 @@
 namespace memopt {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kTokensPerThread = 4;
+constexpr int kInFlight = 8;  // table entries that a lane loads before it stores them
 constexpr int kMaxBatch = 8192;
 constexpr int kMaxRows = 1 << 18;
 
@@ -43,6 +44,7 @@ struct PageArgs {
   const int32_t* rows;  // [B]
   const int32_t* amount;  // [B]: new tokens (reserve) or kept tokens (truncate; null: none kept)
   int R, MB, NB, BS, B;
+  int shift;  // log2(BS), or -1 where BS is no power of two
   int64_t max_tokens;
   int32_t* cu;         // [B + 1]
   int32_t* slots;      // [max_tokens]
@@ -74,15 +76,17 @@ size_t batch_smem(int B, int R) {
   return (static_cast<size_t>(4) * B + 2) * 4 + static_cast<size_t>((R + 31) / 32) * 4;
 }
 
-__device__ __forceinline__ int pages_of(int tokens, int BS) { return (tokens + BS - 1) / BS; }
+__device__ __forceinline__ int over_bs(int x, const PageArgs& a) { return a.shift >= 0 ? x >> a.shift : x / a.BS; }
+__device__ __forceinline__ int pages_of(int tokens, const PageArgs& a) { return over_bs(tokens + a.BS - 1, a); }
 
 // Reads the batch, checks it and scans it.  Returns the status bits of the
 // refusal (0: accepted), the same in every thread.  total_tokens and
 // total_pages are the sums (64-bit: refused sums may exceed an int).
-template <bool kReserve>
+template <int kThreads, bool kReserve>
 __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total_tokens, int64_t& total_pages) {
   __shared__ uint32_t s_status;
-  __shared__ int64_t s_sum[2][kThreads / 32];
+  constexpr int kWarps = kThreads / 32;
+  __shared__ int64_t s_sum[2][kWarps], s_all[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_status = 0;
   for (int i = tid; i < (a.R + 31) / 32; i += kThreads) t.seen[i] = 0;
@@ -116,9 +120,9 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
           bits |= MEMOPT_PAGES_ROW_FULL;
           n = 0;
         }
-        p = pages_of(old + n, a.BS) - pages_of(old, a.BS);
+        p = pages_of(old + n, a) - pages_of(old, a);
       } else {
-        p = pages_of(old, a.BS) - pages_of(n, a.BS);
+        p = pages_of(old, a) - pages_of(n, a);
       }
       t.row[b] = row;
       t.old[b] = old;
@@ -138,15 +142,21 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
       s_sum[1][warp] = sp;
     }
     __syncthreads();
-    int64_t bn = carry_n, bp = carry_p;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) {
-        bn += s_sum[0][w];
-        bp += s_sum[1][w];
+    if (warp < 2) {  // warp 0 scans the warps' tokens, warp 1 their pages
+      const int64_t own = lane < kWarps ? s_sum[warp][lane] : 0;
+      int64_t sum = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
       }
-      carry_n += s_sum[0][w];
-      carry_p += s_sum[1][w];
+      if (lane < kWarps) s_sum[warp][lane] = sum - own;
+      if (lane == 31) s_all[warp] = sum;
     }
+    __syncthreads();
+    const int64_t bn = carry_n + s_sum[0][warp], bp = carry_p + s_sum[1][warp];
+    carry_n += s_all[0];
+    carry_p += s_all[1];
     if (b < a.B) {  // sums past an int belong to refused calls (checked below)
       t.cu[b] = static_cast<int32_t>(bn + sn - n);
       t.page[b] = static_cast<int32_t>(bp + sp - p);
@@ -169,6 +179,10 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
 // all other CTAs before their arrival are then visible to it.
 __device__ bool arrive_last(int32_t* ticket) {
   __shared__ int s_last;
+  if (gridDim.x == 1) {
+    __syncthreads();
+    return true;
+  }
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) s_last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x) - 1;
@@ -177,20 +191,22 @@ __device__ bool arrive_last(int32_t* ticket) {
   return s_last != 0;
 }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ uint8_t smem[];
   const Batch t = carve(smem, a.B);
   const int tid = threadIdx.x, lane = tid & 31;
   const int head = a.state[0], count = a.state[1];
   int64_t tokens, pages;
-  uint32_t status = scan_batch<true>(a, t, tokens, pages);
+  uint32_t status = scan_batch<kThreads, true>(a, t, tokens, pages);
   if (head < 0 || head >= a.NB || count < 0 || count > a.NB) status |= MEMOPT_PAGES_CORRUPT;
   if (status == 0 && pages > count) status |= MEMOPT_PAGES_EXHAUSTED;
   const bool taken = status == 0;
   uint32_t bits = 0;
-  auto ring_at = [&](int64_t i) {
-    int64_t at = head + i;  // head < NB and i < count <= NB
-    if (at >= a.NB) at -= a.NB;
+  auto ring_at = [&](int i) {
+    uint32_t at = static_cast<uint32_t>(head) + i;  // head < NB and i < count <= NB < 2^31
+    if (at >= static_cast<uint32_t>(a.NB)) at -= a.NB;
     return a.ring[at];
   };
 
@@ -222,9 +238,9 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
           page_at = -1;
         }
         const int p = t.old[b] + static_cast<int>(tk - t.cu[b]);
-        const int at = p / a.BS;
+        const int at = over_bs(p, a);
         if (at != page_at) {
-          const int had = pages_of(t.old[b], a.BS);
+          const int had = pages_of(t.old[b], a);
           page = at < had ? a.tables[static_cast<int64_t>(t.row[b]) * a.MB + at] : ring_at(t.page[b] + at - had);
           page_at = at;
         }
@@ -246,26 +262,31 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
     }
   }
 
-  // Table rows: a warp per batch row writes the new pages into the row and
-  // the whole row into the batch's own table.
-  const int nwarps = gridDim.x * (kThreads / 32);
-  for (int b = blockIdx.x * (kThreads / 32) + (tid >> 5); b < a.B; b += nwarps) {
-    const int had = pages_of(t.old[b], a.BS), more = taken ? t.page[b + 1] - t.page[b] : 0;
+  // Table rows: a warp per batch row writes the new pages into the row, and all
+  // its pages into the batch's own table (-1 behind them).
+  const int nwarps = gridDim.x * kWarps;
+  const bool bad = status & MEMOPT_PAGES_BAD_ROW;
+  for (int b = blockIdx.x * kWarps + (tid >> 5); b < a.B; b += nwarps) {
+    const int had = bad ? 0 : pages_of(t.old[b], a), more = taken ? t.page[b + 1] - t.page[b] : 0;
     int32_t* row = a.tables + static_cast<int64_t>(t.row[b]) * a.MB;
     int32_t* out = a.out_tables + static_cast<int64_t>(b) * a.MB;
-    const bool bad = status & MEMOPT_PAGES_BAD_ROW;
-    for (int c = lane; c < a.MB; c += 32) {
-      int32_t v = -1;
-      if (!bad) {
-        if (c >= had && c < had + more) {
-          v = ring_at(t.page[b] + c - had);
-          if (v < 0 || v >= a.NB) bits |= MEMOPT_PAGES_CORRUPT;
-          row[c] = v;
-        } else {
-          v = row[c];
-        }
+    for (int c0 = lane; c0 < a.MB; c0 += 32 * kInFlight) {
+      int32_t v[kInFlight];
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i) {
+        const int c = c0 + 32 * i;
+        v[i] = c < had ? row[c] : c < had + more ? ring_at(t.page[b] + c - had) : -1;
       }
-      out[c] = v;
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i) {
+        const int c = c0 + 32 * i;
+        if (c >= a.MB) break;
+        if (c >= had && c < had + more) {
+          if (v[i] < 0 || v[i] >= a.NB) bits |= MEMOPT_PAGES_CORRUPT;
+          row[c] = v[i];
+        }
+        out[c] = v[i];
+      }
     }
     if (lane == 0) a.out_lens[b] = bad ? 0 : t.old[b] + (taken ? t.cu[b + 1] - t.cu[b] : 0);
   }
@@ -287,27 +308,42 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
   }
 }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) truncate_kernel(const PageArgs a) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ uint8_t smem[];
   const Batch t = carve(smem, a.B);
   const int tid = threadIdx.x, lane = tid & 31;
   const int head = a.state[0], count = a.state[1];
   int64_t kept, pages;
-  uint32_t status = scan_batch<false>(a, t, kept, pages);
+  uint32_t status = scan_batch<kThreads, false>(a, t, kept, pages);
   if (head < 0 || head >= a.NB || count < 0 || count > a.NB || (status == 0 && count + pages > a.NB))
     status |= MEMOPT_PAGES_CORRUPT;
   uint32_t bits = 0;
   if (status == 0) {
-    const int nwarps = gridDim.x * (kThreads / 32);
-    for (int b = blockIdx.x * (kThreads / 32) + (tid >> 5); b < a.B; b += nwarps) {
+    const int nwarps = gridDim.x * kWarps;
+    for (int b = blockIdx.x * kWarps + (tid >> 5); b < a.B; b += nwarps) {
       const int gone = t.page[b + 1] - t.page[b];
-      const int first = pages_of(t.old[b], a.BS) - gone;
-      int32_t* row = a.tables + static_cast<int64_t>(t.row[b]) * a.MB;
-      for (int i = lane; i < gone; i += 32) {
-        const int32_t v = row[first + i];
-        if (v < 0 || v >= a.NB) bits |= MEMOPT_PAGES_CORRUPT;
-        a.ring[(static_cast<int64_t>(head) + count + t.page[b] + i) % a.NB] = v;
-        row[first + i] = -1;
+      const int first = pages_of(t.old[b], a) - gone;
+      int32_t* row = a.tables + static_cast<int64_t>(t.row[b]) * a.MB + first;
+      const uint32_t NB = a.NB;  // below 2^31
+      uint32_t tail = static_cast<uint32_t>(head) + count;
+      tail = tail >= NB ? tail - NB : tail;
+      tail += t.page[b];
+      tail = tail >= NB ? tail - NB : tail;
+      for (int i0 = lane; i0 < gone; i0 += 32 * kInFlight) {
+        int32_t v[kInFlight];
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) v[i] = i0 + 32 * i < gone ? row[i0 + 32 * i] : 0;
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+          const int k = i0 + 32 * i;
+          if (k >= gone) break;
+          if (v[i] < 0 || v[i] >= a.NB) bits |= MEMOPT_PAGES_CORRUPT;
+          const uint32_t at = tail + k;  // k < NB
+          a.ring[at >= NB ? at - NB : at] = v[i];
+          row[k] = -1;
+        }
       }
     }
   }
@@ -338,14 +374,27 @@ int check_pages(const char* who, const PageArgs& a) {
   return MEMOPT_OK;
 }
 
+int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v && s < 30) ++s;
+  return (1 << s) == v ? s : -1;
+}
+
+// One pass over the tokens and one over the rows, at most one CTA per SM: each
+// repeats the scan of the batch.
 template <typename K>
-int launch_pages(K kern, const char* what, const PageArgs& a, int grid, cudaStream_t s) {
+int launch_pages(K small, K large, const char* what, const PageArgs& a, cudaStream_t s) {
+  const int threads = a.B > 256 ? 1024 : 256;
+  const K kern = a.B > 256 ? large : small;
   const size_t smem = batch_smem(a.B, a.R);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return cuda_fail(e, what);
   }
-  kern<<<grid, kThreads, smem, s>>>(a);
+  const int64_t per_cta = threads * kTokensPerThread, rows = threads / 32;
+  const int64_t want = std::max((a.max_tokens + per_cta - 1) / per_cta, (a.B + rows - 1) / rows);
+  const int grid = static_cast<int>(std::min<int64_t>(sm_count(), std::max<int64_t>(1, want)));
+  kern<<<grid, threads, smem, s>>>(a);
   MEMOPT_LAUNCH_CHECK(what);
   return MEMOPT_OK;
 }
@@ -361,7 +410,7 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
                                     int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
                                     int32_t* batch_tables, int32_t* batch_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, max_tokens, cu_seqlens, slot_mapping, positions, batch_tables, batch_lens};
+             num_blocks, block_size, batch, 0, max_tokens, cu_seqlens, slot_mapping, positions, batch_tables, batch_lens};
   const int st = check_pages("reserve_slots", a);
   if (st != MEMOPT_OK) return st;
   if (!cu_seqlens || (batch > 0 && (!new_lens || !batch_tables || !batch_lens)) ||
@@ -369,25 +418,18 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
     return fail(MEMOPT_ERR_INVALID_ARG, "reserve_slots: null pointer");
   if ((reinterpret_cast<uintptr_t>(slot_mapping) | reinterpret_cast<uintptr_t>(positions)) & 15u)
     return fail(MEMOPT_ERR_INVALID_ARG, "reserve_slots: slot_mapping and positions must be 16-byte aligned");
-  // Enough CTAs for one pass over the tokens and the rows, at most two per SM:
-  // each CTA repeats the scan of the batch.
-  const int64_t by_tokens = (max_tokens + kThreads * kTokensPerThread - 1) / (kThreads * kTokensPerThread);
-  const int64_t by_rows = (batch + kThreads / 32 - 1) / (kThreads / 32);
-  const int64_t most = static_cast<int64_t>(sm_count()) * 2;
-  const int grid = static_cast<int>(std::min(most, std::max<int64_t>(1, std::max(by_tokens, by_rows))));
-  return launch_pages(reserve_kernel, "reserve_kernel launch", a, grid, as_stream(stream));
+  a.shift = log2_of(block_size);
+  return launch_pages(reserve_kernel<256>, reserve_kernel<1024>, "reserve_kernel launch", a, as_stream(stream));
 }
 
 extern "C" int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens, int num_rows, int max_blocks_per_seq,
                                     int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
                                     const int32_t* keep_lens, int batch, int block_size, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, keep_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, nullptr, nullptr, nullptr, nullptr, nullptr};
+             num_blocks, block_size, batch, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr};
   const int st = check_pages("truncate_rows", a);
   if (st != MEMOPT_OK) return st;
   if (batch == 0) return MEMOPT_OK;
-  const int64_t by_rows = (batch + kThreads / 32 - 1) / (kThreads / 32);
-  const int64_t most = static_cast<int64_t>(sm_count()) * 2;
-  const int grid = static_cast<int>(std::min(most, by_rows));
-  return launch_pages(truncate_kernel, "truncate_kernel launch", a, grid, as_stream(stream));
+  a.shift = log2_of(block_size);
+  return launch_pages(truncate_kernel<256>, truncate_kernel<1024>, "truncate_kernel launch", a, as_stream(stream));
 }
