@@ -9,27 +9,45 @@
 // most 16), and a tile is 128 rows = 128 / Gp tokens x Gp heads: one TMA box of
 // the query tensor lays them out token by token, so grouped heads share every
 // K and V tile and a short prompt still fills rows.  An item has two tiles of
-// consecutive tokens over the same key blocks of 128.
+// consecutive tokens over the same key blocks of 128, one CTA to an SM; or one
+// tile, two CTAs to an SM, for short prompts and few items (measured at the rule
+// in memopt_packed_attention).
 //
-// The launch has a CTA per item at most, long items first.  A CTA that has
-// done its item takes over one that has not begun (cluster launch control), so
-// about one CTA per SM runs and the SMs stay balanced.  12 warps:
-//   * warps 0-3 / 4-7: softmax of tile 0 / 1, one thread per row (= TMEM lane);
-//   * warps 8 / 9 issue the tcgen05.mma of tile 0 / 1: S = Q K^T (128 x 128 x D)
-//     into its 128 score columns, O += P V (128 x D x 128), P from tensor memory;
-//   * warp 10 loads Q and the K/V blocks by TMA (128-byte swizzle) into a ring;
-//   * warp 11 finds the next item from cu_seqlens while the others work.
-// The tiles alternate on the tensor pipe: while one tile's scores become
-// weights, the other's products run.  P (16-bit pairs) overwrites the scores it
-// came from; P.V starts on its first 64 keys while the weights of the other 64
-// are being computed.  O is rescaled only when the running maximum grows by
-// more than 2^8 (weights stay <= 2^8 and the sums fp32), which is rare.
+// The launch has a CTA per item at most, long items first.  A CTA that has done
+// its item takes over one that has not begun (cluster launch control), so the SMs
+// stay balanced: on 2 x 8192 tokens causal, 32 heads, the CTAs end within 2% of
+// each other.  Head units go in chunks whose K and V fit L2: all heads at once
+// read them from DRAM again for every item (148 heads of 8192 tokens: 4 TB/s and
+// 20% slower under the power cap).  Warps of a CTA:
+//   * four per tile for the softmax, one thread per row (= TMEM lane);
+//   * one per tile issues its tcgen05.mma: S = Q K^T (128 x 128 x D) into its 128
+//     score columns, O += P V (128 x D x 128) with P from tensor memory.  One warp
+//     for both tiles made each wait of one tile a hole in the other's products
+//     (period of a pair of blocks 4280 cycles against 2950);
+//   * one loads Q and the K/V blocks by TMA (128-byte swizzle) into a ring;
+//   * one finds the next item from cu_seqlens while the others work.
+// The tiles take turns on the tensor pipe: while one tile's scores become weights,
+// the other's products run.  With D = 128 P (16-bit pairs) overwrites the scores it
+// came from, so a block is the chain scores -> maximum -> weights -> P V -> scores;
+// P V starts on its first 96 keys while the last 32 weights are being computed
+// (starting at 64 or at 128: 15% slower).  With D = 64 tensor memory has room for
+// P beside the scores, and the next scores run during the softmax.  O is rescaled
+// only when the running maximum grows by more than 2^8 (weights stay <= 2^8 and
+// the sums fp32), which is rare.
+//
+// What bounds it: for each tile and block 1024 cycles of the tensor pipe (D = 128)
+// and 1024 of the exponential unit, which the two tiles overlap to 2950 cycles a
+// pair of blocks (70% of the tensor pipe); in long runs the power cap (1000 W,
+// 1.4 GHz).  148 heads x 8192 tokens, not causal: 3.82-3.94 ms = 1290-1330 TFLOP/s,
+// 0.92-0.95 of the measured sustained cuBLAS rate; 2 x 8192 causal, 32 heads:
+// 1.05 ms = 1040.  A quarter of the exponentials on the FMA pipe saves 3% of the
+// cycles and costs as much power: equal or slower by the clock, not kept.
 //
 // Masked scores are replaced, so a hidden key never matters.  A hidden value
 // meets a weight of exactly 0, which only a non-finite value survives: rows
-// behind the sequence's end are zeroed in shared memory, and a row whose result is not finite
-// is computed again over its visible tokens alone (row_by_row), so a NaN or an
-// infinity reaches exactly the rows that see it.
+// behind the sequence's end are zeroed in shared memory, and a row whose result
+// is not finite is computed again over its visible tokens alone (row_by_row), so
+// a NaN or an infinity reaches exactly the rows that see it.
 //
 // Every wait is bounded; a wait that runs out ends the CTA with NaN in the rows
 // of the item at hand.
@@ -50,10 +68,6 @@ constexpr int kBN = 128;       // keys per block
 constexpr int kFirst = 6;       // of the 8 steps of 16 keys, those that P.V starts with
 constexpr int kAhead = 3;       // blocks before an item's last loads at which the next item is taken
 constexpr int kMaxGp = 16;     // query heads packed into a tile
-constexpr int kMmaWarp = 8, kLoadWarp = 10;  // MMA warps 8 and 9, scheduler warp 11
-constexpr int kThreads = 384;
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 72;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "register split within the launch's registers");
 
 struct Params {
   const void *q, *k, *v;
@@ -63,25 +77,34 @@ struct Params {
   int T, S, H, group;
   int gshift;       // log2 of the heads packed into a tile
   int units;        // head units: H >> gshift
-  int tiles;        // tiles per item, 1 or 2
   int chunk;        // head units walked together
   int window, causal;
   float qscale;     // log2(e) / sqrt(D)
 };
 
-template <int D>
+// TILES: 128-row tiles of an item.  Two share the K/V blocks and take turns on the
+// tensor pipe, one CTA per SM; with one, two CTAs share the SM.
+template <int D, int TILES>
 struct Cfg {
+  // Warps: 4 for the softmax of each tile, then a warpgroup of MMA warps (one per
+  // tile), the load warp and the scheduler.
+  static constexpr int MMA_WARP = 4 * TILES, LOAD_WARP = 5 * TILES, SCHED_WARP = LOAD_WARP + 1;
+  static constexpr int THREADS = 128 * TILES + 128;
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 168 : 128;  // a thread, of 65536 / THREADS / CTAs
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 208 : 184, OTHER_REGS = 72;
+  static_assert(128 * TILES * SOFTMAX_REGS + 128 * OTHER_REGS <= THREADS * LAUNCH_REGS, "within the launch's registers");
+  static constexpr int ITEM_READERS = 5 * TILES + 1;  // softmax, MMA and load warps
   static constexpr int HALVES = D / 64;
   static constexpr int HALF = kBN * 128;          // 128 rows x 128 B
   static constexpr int TILE = HALVES * HALF;      // a Q tile, a K block or a V block
-  static constexpr int STAGES = D == 128 ? 5 : 8;
-  static constexpr int KV_OFF = 2 * TILE;
+  static constexpr int STAGES = TILES == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);
+  static constexpr int KV_OFF = TILES * TILE;
   static constexpr int SMEM = KV_OFF + STAGES * TILE + 1024;  // + alignment slack
   // With D = 64 tensor memory has room for P beside the scores: the next scores
   // are computed while the weights are, and a block takes its softmax alone.
-  static constexpr bool OWN_P = 2 * (kBN + D + kBN / 2) <= 512;
-  static_assert(SMEM <= 227 * 1024, "shared memory");
-  static_assert(2 * (kBN + D) <= 512, "tensor memory columns");
+  static constexpr bool OWN_P = kBN + D + kBN / 2 <= 256;
+  static_assert(SMEM <= (TILES == 2 ? 227 : 112) * 1024, "shared memory");
+  static_assert(kBN + D <= 256, "tensor memory columns of a tile");
 };
 
 struct Item {
@@ -103,10 +126,11 @@ struct Range {
   int lo, hi;
   int last;  // keys below this index are the tile's (visible to some row)
 };
+template <int TILES>
 __device__ __forceinline__ Range tile_range(const Params& p, const Item& it, int t) {
   const int tokens = 128 >> p.gshift;
   const int first = it.t0 + t * tokens;
-  if (t >= p.tiles || first >= it.n) return {0, 0, 0};
+  if (t >= TILES || first >= it.n) return {0, 0, 0};
   const int end = min(first + tokens, it.n);
   const int c_last = p.causal ? end : it.n, c_first = p.causal ? first + 1 : it.n;
   const int from = p.window > 0 && c_first > p.window ? c_first - p.window : 0;
@@ -224,27 +248,27 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
   for (int e = 0; e < E; ++e) dst[e] = pack2<T>(acc[2 * e] / l, acc[2 * e + 1] / l);
 }
 
-// Barriers: items (2 slots: filled by the scheduler, read by the 11 warps
-// that work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
+// Barriers: items (2 slots: filled by the scheduler, read by the warps that
+// work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
 // ready (commit), first and second part of P ready (4 warps), P.V done
 // (commit).
-template <int D>
+template <int STAGES>
 struct Bars {
-  uint64_t item_full[2], item_free[2], q_full, q_free, kv_full[Cfg<D>::STAGES], kv_free[Cfg<D>::STAGES];
+  uint64_t item_full[2], item_free[2], q_full, q_free, kv_full[STAGES], kv_free[STAGES];
   uint64_t s_full[2], p_part[2][2], pv_done[2], s_read[2], end[2], next, near_end;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int TILES>
+__global__ void __launch_bounds__(128 * TILES + 128, 3 - TILES)
 packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qmap,
                         const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using C = Cfg<D>;
+  using C = Cfg<D, TILES>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = tc::idesc_f16(128, kBN, false, false, kBf16);
   constexpr uint32_t kIdescS64 = tc::idesc_f16(128, 64, false, false, kBf16);
   constexpr uint32_t kIdescPV = tc::idesc_f16(128, D, false, true, kBf16);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) Bars<D> bars;
+  __shared__ __align__(8) Bars<C::STAGES> bars;
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) uint4 next_cta;
@@ -259,7 +283,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(at(bars.item_full[i]), 1);
-      mbar_init(at(bars.item_free[i]), 11);
+      mbar_init(at(bars.item_free[i]), C::ITEM_READERS);
       mbar_init(at(bars.s_full[i]), 1);
       mbar_init(at(bars.p_part[i][0]), 4);
       mbar_init(at(bars.p_part[i][1]), 4);
@@ -270,25 +294,25 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     mbar_init(at(bars.next), 1);
     mbar_init(at(bars.near_end), 1);
     mbar_init(at(bars.q_full), 1);
-    mbar_init(at(bars.q_free), 2);
+    mbar_init(at(bars.q_free), TILES);
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(at(bars.kv_full[i]), 1);
-      mbar_init(at(bars.kv_free[i]), 2);
+      mbar_init(at(bars.kv_free[i]), TILES);
     }
     fence_mbar_init();
   }
   if (warp == 0) {
-    tc::tmem_alloc(smem_u32(&tmem_slot), 512);
+    tc::tmem_alloc(smem_u32(&tmem_slot), 256 * TILES);
     tc::tmem_relinquish();
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  // Tile t: scores at columns 128 t, O at 256 + D t, P over the scores or behind O.
-  auto tS = [&](int t) { return tmem + 128u * t; };
-  auto tO = [&](int t) { return tmem + 256u + static_cast<uint32_t>(D) * t; };
-  auto tP = [&](int t) { return C::OWN_P ? tmem + 256u + 2u * D + 64u * t : tS(t); };
+  // Tile t: scores at its first 128 columns, O behind them, P over the scores or behind O.
+  auto tS = [&](int t) { return tmem + 256u * t; };
+  auto tO = [&](int t) { return tS(t) + 128u; };
+  auto tP = [&](int t) { return C::OWN_P ? tO(t) + static_cast<uint32_t>(D) : tS(t); };
 
   // The k-th item of this CTA (read by every warp but the scheduler).
   auto next_item = [&](int k, Item& it) -> bool {
@@ -305,8 +329,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     return it.n >= 0;
   };
 
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+  if (warp < C::MMA_WARP) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
     // =========================== softmax warps ===========================
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
@@ -316,7 +340,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     bool ok = true;
     Item it;
     for (int k = 0; ok && next_item(k, it); ++k) {
-      const Range r = tile_range(p, it, t);
+      const Range r = tile_range<TILES>(p, it, t);
       if (r.hi == 0) continue;
       const int tok = it.t0 + t * tile_tokens + (row >> p.gshift);
       const int h = (it.unit << p.gshift) + (row & ((1 << p.gshift) - 1));
@@ -539,14 +563,14 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp < kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+    if (warp < C::LOAD_WARP) {
       // ============================= MMA warps =============================
       // One warp per tile, so that a wait of one leaves the tensor pipe to the
       // other.  Warp-uniform code; elect.sync issues each instruction once.
       // Both follow every K/V block of the item, used or not: a block is free
       // when both have let it go.
-      const int t = warp - kMmaWarp;
+      const int t = warp - C::MMA_WARP;
       const uint64_t dq = tc::sdesc_sw128(sbase + t * C::TILE, 16, 1024);
       const uint64_t dk0 = tc::sdesc_sw128(sbase + C::KV_OFF, 16, 1024);
       const uint64_t dv0 = tc::sdesc_sw128(sbase + C::KV_OFF, C::HALF, 1024);
@@ -561,7 +585,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       };
       Item it;
       for (int k = 0; ok && next_item(k, it); ++k) {
-        const Range r0 = tile_range(p, it, 0), r1 = tile_range(p, it, 1);
+        const Range r0 = tile_range<TILES>(p, it, 0), r1 = tile_range<TILES>(p, it, 1);
         const int LO = r0.lo, HI = max(r0.hi, r1.hi);  // tile 0 exists and starts first
         const int lo = t ? r1.lo : r0.lo, hi = t ? r1.hi : r0.hi, last = t ? r1.last : r0.last;
         auto scores = [&](int j) {  // S(j) if the tile has the block; lets K(j) and, at the end, Q go
@@ -632,7 +656,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         tc::commit_elect(at(bars.end[t]));
         wait_bar(at(bars.end[t]), 0);
       }
-    } else if (warp == kLoadWarp) {
+    } else if (warp == C::LOAD_WARP) {
       // ============================== loads ==============================
       if (lane == 0) {
         prefetch_tensormap(&qmap);
@@ -643,7 +667,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       bool ok = true;
       Item it;
       for (int k = 0; ok && next_item(k, it); ++k) {
-        const Range r0 = tile_range(p, it, 0), r1 = tile_range(p, it, 1);
+        const Range r0 = tile_range<TILES>(p, it, 0), r1 = tile_range<TILES>(p, it, 1);
         const int LO = r0.lo, HI = max(r0.hi, r1.hi);
         const int h0 = it.unit << p.gshift, hk = h0 / p.group;
         if (lane == 0) {
@@ -677,12 +701,12 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         ok = __shfl_sync(0xffffffffu, ok, 0);
         loads = __shfl_sync(0xffffffffu, loads, 0);
       }
-    } else {
+    } else if (warp == C::SCHED_WARP) {
       // ============================ scheduler ============================
       // Head units in chunks (their keys and values stay in L2 while the chunk's
       // items run); within a chunk the items in descending order of work, within a
       // token block the units.
-      const int tokens = tile_tokens * p.tiles;
+      const int tokens = tile_tokens * TILES;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
         lo = min(max(__ldg(p.cu + s), 0), p.T);
         hi = min(max(__ldg(p.cu + s + 1), lo), p.T);
@@ -800,7 +824,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 0) tc::tmem_dealloc(tmem, 512);
+  if (warp == 0) tc::tmem_dealloc(tmem, 256 * TILES);
 }
 
 namespace {
@@ -838,8 +862,9 @@ int map_rows(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_
   return MEMOPT_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, int TILES>
 int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
+  using C = Cfg<D, TILES>;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   alignas(64) CUtensorMap qm, km, vm;
   const int Gp = 1 << p.gshift;
@@ -847,12 +872,17 @@ int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
   if (st == MEMOPT_OK) st = map_rows(&km, p.k, bf16, p.T, p.k_stride, KVH, D, 1, kBN);
   if (st == MEMOPT_OK) st = map_rows(&vm, p.v, bf16, p.T, p.v_stride, KVH, D, 1, kBN);
   if (st != MEMOPT_OK) return st;
-  auto kern = packed_attention_kernel<T, D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  auto kern = packed_attention_kernel<T, D, TILES>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed_attention)");
-  kern<<<static_cast<unsigned>(grid), kThreads, Cfg<D>::SMEM, s>>>(p, qm, km, vm);
+  kern<<<static_cast<unsigned>(grid), C::THREADS, C::SMEM, s>>>(p, qm, km, vm);
   MEMOPT_LAUNCH_CHECK("packed_attention_kernel launch");
   return MEMOPT_OK;
+}
+
+template <typename T, int D>
+int launch(const Params& p, int KVH, int tiles, int64_t grid, cudaStream_t s) {
+  return tiles == 1 ? launch<T, D, 1>(p, KVH, grid, s) : launch<T, D, 2>(p, KVH, grid, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -890,24 +920,29 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   p.units = num_heads >> p.gshift;
   p.window = window_size > 0 ? window_size : 0, p.causal = causal ? 1 : 0;
   p.qscale = (1.0f / sqrtf(static_cast<float>(head_dim))) * 1.4426950408889634f;
-  // At most this many items (each sequence has one partial token block at most):
-  // with fewer than the SMs, an item takes one tile instead of two, so that twice
-  // as many SMs work.
+  // At most this many items (each sequence has one partial token block at most).
   const int64_t tokens = 128 >> p.gshift;
   auto most_items = [&](int tiles) { return (total_tokens / (tokens * tiles) + num_seqs) * p.units; };
-  p.tiles = most_items(2) < sm_count() ? 1 : 2;
+  // Two tiles an item halve the K/V traffic and pay where the walk over the keys is
+  // long and the items are many: 2 x 8192 tokens, 32 heads 1.05 against 1.11 ms with
+  // one tile, 8 x 2048 with 32/8 heads 265 against 281 us, 4 prompts up to 7696 with
+  // 4/1 heads 155 against 205.  One tile, two CTAs to an SM, hides an item's ends
+  // better and makes twice the items: 32 x 512 118 against 123 us, 64 x 32 tokens
+  // 16.0 against 21.1, one prompt of 1000 24 against 27, 8192 tokens of 4 heads 108
+  // against 117.
+  const int tiles = total_tokens >= 768LL * num_seqs && most_items(2) >= 2 * sm_count() ? 2 : 1;
   // Head units per chunk: the chunk's keys and values fill about a quarter of L2.
   // Units that share a KV head stay together.
   const int per_kv = p.group >> p.gshift;
   const int64_t kv_bytes = total_tokens * head_dim * 4;
   p.chunk = static_cast<int>(std::min<int64_t>(p.units, per_kv * std::max<int64_t>(1, (int64_t(32) << 20) / kv_bytes)));
   (void)max_seqlen;
-  const int64_t grid = most_items(p.tiles);
+  const int64_t grid = most_items(tiles);
   if (grid > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many work items");
   cudaStream_t s = as_stream(stream);
   if (dtype == MEMOPT_DTYPE_F16)
-    return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, grid, s)
-                           : packed::launch<__half, 64>(p, num_kv_heads, grid, s);
-  return head_dim == 128 ? packed::launch<__nv_bfloat16, 128>(p, num_kv_heads, grid, s)
-                         : packed::launch<__nv_bfloat16, 64>(p, num_kv_heads, grid, s);
+    return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, tiles, grid, s)
+                           : packed::launch<__half, 64>(p, num_kv_heads, tiles, grid, s);
+  return head_dim == 128 ? packed::launch<__nv_bfloat16, 128>(p, num_kv_heads, tiles, grid, s)
+                         : packed::launch<__nv_bfloat16, 64>(p, num_kv_heads, tiles, grid, s);
 }
