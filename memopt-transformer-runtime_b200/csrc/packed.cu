@@ -407,6 +407,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           // again (where P lies over the scores, P of a chunk is below the scores of
           // the next one).
           const int chunks = (min(kBN, r.last - j * kBN) + 31) / 32;
+          // Chunks [begin, end) hold a column that a row of this warp sees; the
+          // others get weights of 0 without a look at their scores.
+          const int begin = max(__reduce_min_sync(0xffffffffu, lo), 0) / 32;
+          const int end = min(chunks, (max(__reduce_max_sync(0xffffffffu, hi), 0) + 31) / 32);
           auto chunk = [&](int cc, float (&v)[32]) {
             tc::ld32(tS(t) + lane_base + cc * 32, v);
             tc::wait_ld(v);
@@ -418,7 +422,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           };
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int cc = 0; cc < chunks; ++cc) {
+          for (int cc = begin; cc < end; ++cc) {
             float v[32];
             chunk(cc, v);
             float m0 = v[0], m1 = v[1];
@@ -435,19 +439,21 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           const uint64_t nm2 = f32x2_pack(-msub, -msub);
 #pragma unroll 1
           for (int cc = 0; cc < chunks; ++cc) {
-            float v[32];
-            chunk(cc, v);
-            if (cc == chunks - 1) s_read();
-            uint32_t ph[16];
+            uint32_t ph[16] = {};
+            if (cc >= begin && cc < end) {
+              float v[32];
+              chunk(cc, v);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float x0, x1;
-              f32x2_unpack(f32x2_fma(f32x2_pack(v[2 * i], v[2 * i + 1]), qs2, nm2), x0, x1);
-              x0 = tc::ex2(x0);
-              x1 = tc::ex2(x1);
-              sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
-              ph[i] = pack2<T>(x0, x1);
+              for (int i = 0; i < 16; ++i) {
+                float x0, x1;
+                f32x2_unpack(f32x2_fma(f32x2_pack(v[2 * i], v[2 * i + 1]), qs2, nm2), x0, x1);
+                x0 = tc::ex2(x0);
+                x1 = tc::ex2(x1);
+                sum2[i & 3] = f32x2_add(sum2[i & 3], f32x2_pack(x0, x1));
+                ph[i] = pack2<T>(x0, x1);
+              }
             }
+            if (cc == chunks - 1) s_read();
             tc::st16(tP(t) + lane_base + cc * 16, ph);
             if (2 * (cc + 1) == kFirst) p_ready(0);
           }
