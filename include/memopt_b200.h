@@ -409,7 +409,8 @@ int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_r
                          const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
                          int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
                          int32_t* batch_lens, void* stream);
-/* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none);   */
+/* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none;    */
+/* keep_lens, like new_lens above, must not overlap context_lens);            */
 /* the pages behind them go to the ring's end in row and page order and their */
 /* table entries become -1.  With freed page lists as block_tables, their     */
 /* counts as context_lens and block_size 1 it returns those pages.            */
@@ -442,7 +443,8 @@ int memopt_rotary_write_cache(const void* query, int64_t query_stride, const voi
 /* Attention inside each sequence of a packed batch.  Sequence s is the rows  */
 /* [cu_seqlens[s], cu_seqlens[s+1]) of query / out [total_tokens, num_heads,  */
 /* head_dim] and keys / values [total_tokens, num_kv_heads, head_dim] (fp16   */
-/* or bf16, layout and strides as above; out contiguous); query head h reads  */
+/* or bf16, layout and strides as above; out contiguous, not overlapping the  */
+/* inputs); query head h reads                                                */
 /* KV head h / (num_heads / num_kv_heads).  Row i of a sequence of n tokens   */
 /* sees its tokens [max(0, c - W), c), c = i + 1 (causal) or n; W = n when    */
 /* window_size <= 0 (the meaning of memopt_paged_attention_f16_ex).  Scores   */

@@ -27,6 +27,21 @@ void int32_inplace(const torch::Tensor& t, const char* who, const char* name, in
   TORCH_CHECK(t.is_contiguous(), who, ": ", name, " is updated in place and must be contiguous");
 }
 
+// Whether the bytes that two tensors span meet.
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  auto span = [](const torch::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) == 0) return std::pair<const char*, const char*>{nullptr, nullptr};
+      last += (t.size(d) - 1) * t.stride(d);
+    }
+    const char* p = static_cast<const char*>(t.data_ptr());
+    return std::pair<const char*, const char*>{p, p + (last + 1) * t.element_size()};
+  };
+  const auto x = span(a), y = span(b);
+  return x.first && y.first && x.first < y.second && y.first < x.second;
+}
+
 int to_int(int64_t v, const char* who, const char* name) {
   TORCH_CHECK(v >= 0 && v <= 0x7fffffff, who, ": ", name, " out of range");
   return static_cast<int>(v);
@@ -92,6 +107,7 @@ std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tens
   const PageTensors n = page_checks(who, block_tables, context_lens, free_pages, pool_state, rows, block_size);
   int32_cuda(new_lens, who, "new_lens", 1, block_tables.device());
   TORCH_CHECK(new_lens.size(0) == n.B, who, ": new_lens length != rows length");
+  TORCH_CHECK(!overlap(new_lens, context_lens), who, ": new_lens must not overlap context_lens");
   TORCH_CHECK(max_tokens >= 0 && max_tokens <= 0x7fffffff, who, ": max_tokens out of range");
   rows = rows.contiguous();
   new_lens = new_lens.contiguous();
@@ -128,6 +144,7 @@ void truncate_rows(torch::Tensor block_tables, torch::Tensor context_lens, torch
   if (keep_lens.has_value()) {
     int32_cuda(*keep_lens, who, "keep_lens", 1, block_tables.device());
     TORCH_CHECK(keep_lens->size(0) == n.B, who, ": keep_lens length != rows length");
+    TORCH_CHECK(!overlap(*keep_lens, context_lens), who, ": keep_lens must not overlap context_lens");
     keep = keep_lens->contiguous();
   }
   rows = rows.contiguous();
@@ -246,6 +263,8 @@ torch::Tensor packed_attention(torch::Tensor query, torch::Tensor keys, torch::T
     TORCH_CHECK(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() &&
                     out.device() == query.device() && out.is_contiguous() && (out.numel() == 0 || aligned16(out)),
                 who, ": out must be a contiguous 16-byte aligned tensor of the query's shape, dtype and device");
+    TORCH_CHECK(!overlap(out, query) && !overlap(out, keys) && !overlap(out, values), who,
+                ": out must not overlap the inputs");
   } else {
     out = torch::empty(query.sizes(), query.options());
   }

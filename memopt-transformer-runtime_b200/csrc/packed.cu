@@ -111,14 +111,19 @@ struct Item {
   int start, n, t0, unit;  // first packed row, length, first token, head unit (n < 0: no more items)
 };
 
-// Bounded wait: at most 2^22 polls of at most 1 us each.
+// Bounded wait: ten seconds by the global timer, read every 4096 polls.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
-  uint32_t polls = 0;
-  while (!mbar_try_wait_hint(bar, parity, 1000)) {
-    if (++polls >= (1u << 22)) return false;
+  uint64_t began = 0;
+  for (uint32_t polls = 1;; ++polls) {
+    if (mbar_try_wait_hint(bar, parity, 1000)) return true;
+    if ((polls & 4095u) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+      if (began == 0) began = now;
+      else if (now - began > 10000000000ull) return false;
+    }
   }
-  return true;
 }
 
 // Key blocks [lo, hi) of an item's tile.
@@ -758,6 +763,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       const int64_t total = all * p.units, per_chunk = all * p.chunk;
       int L = 0, unit0 = -p.chunk;
       int64_t above = 0, here = 0;  // token blocks on the levels above, on this one
+      int found_level = -1, found_s0 = 0, found_before = 0;  // sequences on the level before found_s0
       bool ok = true, more = true;  // more: there may be CTAs that have not begun
       int64_t i = blockIdx.x;
       uint32_t asked = 0;
@@ -803,18 +809,27 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
             here = count_on(L);
           }
           const int per_seq = p.causal ? 1 : L, at_level = static_cast<int>(b - above);
-          int skip = at_level / per_seq;  // sequences on the level before the one
-          for (int s0 = 0; s0 < p.S; s0 += 32) {
+          // The sequence is the rank-th on the level.  Ranks grow from item to item:
+          // the search goes on where the last one ended.
+          const int rank = at_level / per_seq;
+          if (L != found_level || rank < found_before) {
+            found_level = L;
+            found_s0 = found_before = 0;
+          }
+          int skip = rank - found_before;
+          for (int s0 = found_s0; s0 < p.S; s0 += 32) {
             const uint32_t has = __ballot_sync(0xffffffffu, on_level(s0 + lane, L));
             const int n = __popc(has);
             if (skip < n) {
               const int s = s0 + static_cast<int>(__fns(has, 0, skip + 1));
               int lo, hi;
               bounds(s, lo, hi);
+              found_s0 = s0;
               it = Item{lo, hi - lo, (p.causal ? L : at_level % L) * tokens, first + static_cast<int>(in_chunk - b * units)};
               break;
             }
             skip -= n;
+            found_before += n;
           }
         }
         if (lane == 0) {

@@ -18,6 +18,9 @@ Same constructor, forward signature and routing as the reference module
   sequence's whole cached context (incremental decode); with
   ``scheduler=MemoryScheduler(...)`` the scheduler's ``retain_ratio`` /
   ``use_int4`` are applied to the cache first (eviction, INT4 conversion);
+* ``forward_packed(x, cache, batch)`` (addition) runs a packed batch, prompts of
+  different lengths or the steps after them, over a
+  :class:`memopt.packed.PackedKVCache`;
 * an exception on the paged path is reported as a RuntimeWarning, counted
   in ``_fallback_count``, disables the paged path for the instance and the
   call is answered by SDPA — unless ``strict=True``, which re-raises.
@@ -139,6 +142,31 @@ class DynamicAttention(nn.Module):
         else:
             attn = self._sdpa_forward(q, k, v, seq_len)
         return self.out_proj(attn)
+
+    def forward_packed(self, x: torch.Tensor, cache, batch, max_seqlen: Optional[int] = None, causal: bool = True,
+                       positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Packed batches over a :class:`memopt.packed.PackedKVCache` (an
+        addition): ``x`` [num_tokens, embed_dim] holds the batch's tokens
+        behind one another.
+
+        With a batch of ``cache.admit`` they are whole prompts of different
+        lengths (``max_seqlen``: the longest) and attend inside each prompt;
+        with a batch of ``cache.extend`` the next tokens of each row, attending
+        over its cached context.  ``positions`` [axes, num_tokens] replaces the
+        tokens' own positions where the cache has rotary positions.  The
+        attention carries no gradient."""
+        T = x.shape[0]
+        shape = (T, self.num_heads, self.head_dim)
+        q, k, v = (p(x).detach().reshape(shape) for p in (self.q_proj, self.k_proj, self.v_proj))
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            q, k, v = (t.to(torch.float16) for t in (q, k, v))
+        if batch.whole:
+            if max_seqlen is None:
+                raise ValueError("forward_packed: max_seqlen is needed for a batch of prompts")
+            out = cache.prompt(q, k, v, batch, max_seqlen, self.window_size, causal, positions)
+        else:
+            out = cache.decode(q, k, v, batch, self.window_size, positions)
+        return self.out_proj(out.reshape(T, self.embed_dim).to(x.dtype))
 
     def _custom_kernel_forward(
         self,

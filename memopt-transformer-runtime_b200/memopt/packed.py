@@ -244,6 +244,8 @@ class PackedKVCache:
         """The next tokens of each row (a batch of :meth:`extend`, the same
         number n of tokens per row): causal paged attention over the cached
         context.  q [B * n, H, D]; the result has q's shape, in fp16."""
+        if batch.whole:
+            raise ValueError("PackedKVCache.decode: the batch must come from extend")
         B = batch.rows.numel()
         if B == 0 or q.shape[0] % B != 0:
             raise ValueError(f"PackedKVCache.decode: {q.shape[0]} tokens for {B} rows")

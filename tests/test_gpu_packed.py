@@ -115,6 +115,56 @@ def test_attention_window(window, causal):
     check_attention([700, 90, 1, 333], 4, 4, 128, torch.float16, causal, window, seed=6)
 
 
+# Long prompts and many heads: the kernel's form with two query tiles an item.
+TWO_TILES = [1500, 777, 1, 1300]
+
+
+@pytest.mark.parametrize("causal,window", [(True, -1), (False, -1), (True, 100), (True, 1000), (False, 300), (True, 1)])
+@pytest.mark.parametrize("H,KVH,D,dtype", [(20, 20, 128, torch.float16), (24, 6, 128, torch.bfloat16),
+                                           (20, 20, 64, torch.bfloat16), (24, 6, 64, torch.float16),
+                                           (40, 8, 128, torch.float16), (64, 4, 64, torch.bfloat16)])
+def test_attention_two_tiles(H, KVH, D, dtype, causal, window):
+    check_attention(TWO_TILES, H, KVH, D, dtype, causal, window, fused=True, seed=H + D)
+
+
+@pytest.mark.parametrize("H,KVH,D", [(20, 20, 64), (24, 6, 128)])
+def test_attention_two_tiles_hidden_tokens(H, KVH, D):
+    """Non-finite values in the two-tile form: rows that do not see them keep
+    their result, also where they lie behind a sequence's end."""
+    q, k, v = make_qkv(TWO_TILES, H, KVH, D, torch.float16, seed=21, tail=33)
+    T = sum(TWO_TILES)
+    at = [700, 1500 + 776, T - 1]  # inside a sequence, last of one, last of all
+    ref, mag = attention_ref(q[:T], k[:T], v[:T], TWO_TILES, -1, True)
+    tol = attention_tol(ref, mag, v, 1500, torch.float16)
+    v[at], v[T:] = float("nan"), float("inf")
+    out = C().packed_attention(q, k, v, cu_of(TWO_TILES), 1500)
+    sees = torch.zeros(T, dtype=torch.bool, device=DEV)
+    sees[700:1500], sees[2276], sees[T - 1] = True, True, True
+    assert torch.isnan(out[:T][sees].float()).all()
+    assert ((out[:T].double() - ref).abs() <= tol)[~sees].all()
+
+
+def test_attention_scores_of_minus_infinity():
+    """A score of -inf weighs nothing; a row with no other score is NaN, as its
+    softmax is."""
+    n, H, D = 150, 2, 64
+    q, k, v = make_qkv([n], H, H, D, torch.float16, seed=22)
+    q[:, :, 0] = 1.0
+    k[:70, 0, 0] = -float("inf")  # head 0: the first 70 keys
+    out = C().packed_attention(q, k, v, cu_of([n]), n)
+    assert torch.isnan(out[:70, 0].float()).all()
+    kk = k.clone()
+    kk[:70, 0, 0] = 0.0
+    ref, mag = attention_ref(q, kk, v, [n], -1, True)
+    assert ((out.double() - ref).abs() <= attention_tol(ref, mag, v, n, torch.float16))[:, 1].all()
+    i = torch.arange(n, device=DEV)
+    s = (q[:, 0].double() @ kk[:, 0].double().T / math.sqrt(D))
+    s = s.masked_fill((i[None] > i[:, None]) | (i[None] < 70), float("-inf"))
+    p = torch.softmax(s, -1)[70:]
+    want, size = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+    assert ((out[70:, 0].double() - want).abs() <= attention_tol(want, size, v, n, torch.float16)).all()
+
+
 def test_attention_long_and_peaked():
     check_attention([5000, 3], 2, 1, 128, torch.float16, seed=7)
     check_attention([3001], 2, 2, 64, torch.bfloat16, seed=8, spread=4.0)  # |s| < 64: q.k/8 of 64 products
@@ -537,6 +587,189 @@ def test_cache_prompt_decode_draft_evict(kv_format):
     cache.table.check()
     assert cache.table.free_count() == 200
     assert sorted(cache.table.free_pages.tolist()) == list(range(200))
+
+
+def test_layer_forward_packed_matches_each_prompt_alone():
+    """A layer over a packed batch gives what it gives to each prompt alone
+    (dense fp64 attention of the fp16 projections), then decodes."""
+    from memopt import DynamicAttention, PackedKVCache
+
+    torch.manual_seed(0)
+    layer = DynamicAttention(256, 4).half().to(DEV)
+    cache = PackedKVCache(64, 4, 64, 16, max_seqs=3, max_seq_len=256)
+    lens = [37, 5, 130]
+    x = torch.randn(sum(lens), 256, device=DEV).half()
+    y = layer.forward_packed(x, cache, cache.admit([2, 0, 1], lens), 130)
+    q, k, v = (p(x).detach().reshape(-1, 4, 64) for p in (layer.q_proj, layer.k_proj, layer.v_proj))
+    ref, mag = attention_ref(q, k, v, lens, -1, True)
+    w = layer.out_proj.weight.detach().double()
+    want = ref.reshape(-1, 256) @ w.T
+    # the attention's own tolerance through |w|, the rounding of the product's
+    # result and of its fp32 sums of 256 terms
+    tol = attention_tol(ref, mag, v, 130, torch.float16).reshape(-1, 256) @ w.abs().T
+    tol = tol + 2.0 ** -11 * want.abs() + 2.0 ** -15 * (ref.reshape(-1, 256).abs() @ w.abs().T) + 2.0 ** -25
+    assert ((y.detach().double() - want).abs() <= tol).all()
+    assert y.requires_grad  # the output projection still trains; the attention does not
+    step = layer.forward_packed(torch.randn(3, 256, device=DEV).half(), cache, cache.extend([2, 0, 1]))
+    assert step.shape == (3, 256) and torch.isfinite(step.float()).all()
+    assert cache.table.context_lens.tolist() == [6, 131, 38]
+    with pytest.raises(ValueError):
+        layer.forward_packed(x, cache, cache.admit([0], [1]))
+    cache.table.check()
+
+
+def test_whole_step_in_a_graph():
+    """Reserve, rotary with the cache write and paged decode captured once and
+    replayed step by step give what the same calls give one by one."""
+    from memopt import DevicePageTable, RotaryPositions
+
+    H, KVH, D, BS, B = 4, 2, 64, 16, 3
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(B, H + 2 * KVH, D, generator=g, device=DEV).half()
+    rot = RotaryPositions(D)
+    rows = torch.tensor([2, 0, 1], dtype=torch.int32, device=DEV)
+    one = torch.ones_like(rows)
+
+    def fresh():
+        table = DevicePageTable(40, BS, B, 160)
+        pools = [torch.zeros(40, BS, KVH, D, dtype=torch.float16, device=DEV) for _ in range(2)]
+        return table, pools
+
+    def step(table, pools):
+        b = table.reserve(rows, one, B)
+        q, _ = rot.write(x[:, :H], x[:, H:H + KVH], x[:, H + KVH:], b.positions, b.slot_mapping, *pools)
+        return C().dynamic_sparse_attention(q[:, None], *pools, b.block_tables, b.context_lens, 160, 160, True)
+
+    table, pools = fresh()
+    plain = [step(table, pools).clone() for _ in range(20)]
+    table2, pools2 = fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*fresh())  # warm-up on the capture stream: its attention workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(table2, pools2)
+        for want in plain:
+            graph.replay()
+            assert torch.equal(out, want)
+    side.synchronize()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(pools, pools2))
+    assert torch.equal(table.block_tables, table2.block_tables)
+    table2.check()
+
+
+def test_two_streams_at_once():
+    """Two batches in flight on two streams do not disturb each other."""
+    sets = [make_qkv([700, 40, 300], 8, 2, 128, torch.float16, seed=s) for s in (1, 2)]
+    cu = cu_of([700, 40, 300])
+    want = [C().packed_attention(*s, cu, 700) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(C().packed_attention(*sets[i], cu, 700))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in (0, 1) for o in got[i])
+
+
+def test_offsets_past_32_bits():
+    """Rows, outputs and slots beyond 2^31 elements."""
+    H, D, T = 64, 128, 270000  # 2.2e9 elements
+    q = torch.zeros(T, H, D, dtype=torch.float16, device=DEV)
+    k = torch.zeros(T, 2, D, dtype=torch.float16, device=DEV)
+    v = torch.zeros_like(k)
+    lens = [300, 1, 129]
+    n = sum(lens)
+    a, b, c = make_qkv(lens, H, 2, D, torch.float16, seed=4)
+    q[-n:], k[-n:], v[-n:] = a, b, c
+    out = torch.zeros_like(q)
+    C().packed_attention(q, k, v, cu_of(lens) + (T - n), 300, -1, True, out)
+    assert torch.equal(out[-n:], C().packed_attention(a, b, c, cu_of(lens), 300))
+    assert not out[:4].any() and not out[T // 2: T // 2 + 4].any()
+    del out
+    freq = 10000.0 ** (-torch.arange(64, device=DEV, dtype=torch.float64) / 64)
+    pos = torch.arange(T, device=DEV, dtype=torch.int32)
+    NB = 540000  # slots: 540000 * 16 * 2 * 128 = 2.2e9 elements
+    kc, vc = (torch.zeros(NB, 16, 2, D, dtype=torch.float16, device=DEV) for _ in range(2))
+    slots = torch.full((T,), -1, dtype=torch.int32, device=DEV)
+    slots[-n:] = torch.arange(NB * 16 - n, NB * 16, device=DEV, dtype=torch.int32)
+    q2, k2 = C().rotary_write_cache(q, k, v, pos, freq, [64], slots, kc, vc)
+    q3, k3 = C().apply_rotary(a, b, pos[-n:], freq, [64])
+    assert torch.equal(q2[-n:], q3) and torch.equal(k2[-n:], k3)
+    assert torch.equal(kc.view(-1, 2, D)[-n:], k3) and torch.equal(vc.view(-1, 2, D)[-n:], c)
+    assert not kc[:100].any() and not kc.view(-1, 2, D)[-n - 16:-n].any()
+
+
+def test_overlapping_arguments_are_refused():
+    q, k, v = make_qkv([8], 2, 2, 64, torch.float16)
+    for out in (q, k, v):
+        with pytest.raises(RuntimeError, match="overlap"):
+            C().packed_attention(q, k, v, cu_of([8]), 8, -1, True, out)
+    from memopt import DevicePageTable
+
+    t = DevicePageTable(8, 16, 2, 64)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="overlap"):
+        t.truncate(rows, t.context_lens)
+    with pytest.raises(RuntimeError, match="overlap"):
+        t.reserve(rows, t.context_lens, 4)
+
+
+@pytest.mark.parametrize("strides", ["sliced", "odd", "expanded", "transposed"])
+def test_layouts_other_than_contiguous(strides):
+    """Rows apart by any multiple of 8 elements are read in place, everything
+    else through a copy: the same result either way."""
+    lens, H, D = [40, 90], 4, 64
+    q, k, v = make_qkv(lens, H, H, D, torch.bfloat16, seed=6)
+    want = C().packed_attention(q, k, v, cu_of(lens), 90)
+
+    def lay(x):
+        T = x.shape[0]
+        if strides == "sliced":
+            return torch.cat([x, x, x], 1)[:, H:2 * H]
+        if strides == "odd":  # tokens 4 elements off a multiple of 8
+            y = torch.zeros(T, H * D + 4, dtype=x.dtype, device=DEV)
+            y[:, :H * D] = x.reshape(T, -1)
+            return y.as_strided((T, H, D), (H * D + 4, D, 1))
+        if strides == "transposed":
+            return x.transpose(0, 1).contiguous().transpose(0, 1)
+        return x[:, :1].expand(-1, H, -1)
+
+    if strides == "expanded":
+        want = C().packed_attention(q, k[:, :1].contiguous(), v[:, :1].contiguous(), cu_of(lens), 90)
+        got = C().packed_attention(q, lay(k), lay(v), cu_of(lens), 90)
+        ref, mag = attention_ref(q, k[:, :1], v[:, :1], lens, -1, True)
+        tol = attention_tol(ref, mag, v, 90, torch.bfloat16)
+        assert ((got.double() - ref).abs() <= tol).all() and ((want.double() - ref).abs() <= tol).all()
+    else:
+        assert torch.equal(C().packed_attention(lay(q), lay(k), lay(v), cu_of(lens), 90), want)
+
+
+def test_many_long_and_short_sequences_find_their_items():
+    """Several thousand sequences: every row belongs to exactly one item."""
+    rng = random.Random(5)
+    lens = [rng.choice([0, 1, 5, 40, 65, 130, 300]) for _ in range(3000)] + [2500]
+    for causal in (True, False):
+        T = sum(lens)
+        q = torch.zeros(T, 2, 64, dtype=torch.float16, device=DEV)
+        k = torch.zeros(T, 1, 64, dtype=torch.float16, device=DEV)
+        v = (torch.arange(T, device=DEV) % 7).half()[:, None, None].expand(T, 1, 64).contiguous()
+        out = torch.full_like(q, float("nan"))
+        C().packed_attention(q, k, v, cu_of(lens), 2500, -1, causal, out)
+        # equal scores: the mean of the visible values
+        x = v[:, 0, 0].double()
+        cum = torch.cat([x.new_zeros(1), x.cumsum(0)])
+        start = torch.repeat_interleave(cu_of(lens)[:-1].long(), torch.tensor(lens, device=DEV))
+        end = torch.repeat_interleave(cu_of(lens)[1:].long(), torch.tensor(lens, device=DEV))
+        at = torch.arange(T, device=DEV) + 1 if causal else end
+        mean = (cum[at] - cum[start]) / (at - start)
+        # weights of 1 are exact; the sum and one rounding of the result remain
+        assert ((out[:, :, 0].double() - mean[:, None]).abs() <= 2.0 ** -11 * mean[:, None] + 1e-5).all()
+        assert torch.equal(out, out[:, :1, :1].expand_as(out))
 
 
 def test_grad_inputs_are_refused():
