@@ -72,6 +72,16 @@ __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   return r;
 }
 
+// The same through the coherent path.
+__device__ __forceinline__ uint4 ld_once_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p)
+               : "memory");
+  return r;
+}
+
 // Packed fp32 pairs (sm_100 f32x2 arithmetic): lane-wise IEEE round-to-nearest.
 __device__ __forceinline__ uint64_t f32x2_pack(float a, float b) {
   uint64_t r;
@@ -166,6 +176,36 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
+
+// ----- programmatic dependent launch ----------------------------------------
+// A kernel launched by launch_after may begin before the stream's previous kernel
+// has ended; it touches no memory before after_previous(), which returns once
+// that kernel has completed and its writes are visible, and reads nothing through
+// the non-coherent path (which wants data constant from the kernel's own start).
+// begin_next() lets the next such launch begin in its turn.  The stream's order is kept; what is saved
+// is the launch latency between small kernels.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void begin_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... Params, typename... Args>
+inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+#define MEMOPT_LAUNCH(call, what)                                \
+  do {                                                           \
+    const cudaError_t _e = (call);                               \
+    if (_e != cudaSuccess) return ::memopt::cuda_fail(_e, what); \
+  } while (0)
 
 // Upper bound on mbarrier polls before a wait is declared failed.  Each
 // try_wait may itself suspend for a hardware-defined interval, so this bound

@@ -195,7 +195,7 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
   auto words = [&](const void* base, int64_t at, uint32_t (&w)[E]) {
     const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(base) + at) + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = __ldg(src + e);
+    for (int e = 0; e < E; ++e) w[e] = src[e];
   };
   float q[2 * E], acc[2 * E], m = -INFINITY, l = 0.f;
   {
@@ -313,6 +313,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  after_previous();
   const uint32_t tmem = tmem_slot;
   // Tile t: scores at its first 128 columns, O behind them, P over the scores or behind O.
   auto tS = [&](int t) { return tmem + 256u * t; };
@@ -719,8 +720,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       // token block the units.
       const int tokens = tile_tokens * TILES;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
-        lo = min(max(__ldg(p.cu + s), 0), p.T);
-        hi = min(max(__ldg(p.cu + s + 1), lo), p.T);
+        lo = min(max(p.cu[s], 0), p.T);
+        hi = min(max(p.cu[s + 1], lo), p.T);
       };
       auto nblocks = [&](int s) {
         int lo = 0, hi = 0;
@@ -896,8 +897,8 @@ int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
   auto kern = packed_attention_kernel<T, D, TILES>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed_attention)");
-  kern<<<static_cast<unsigned>(grid), C::THREADS, C::SMEM, s>>>(p, qm, km, vm);
-  MEMOPT_LAUNCH_CHECK("packed_attention_kernel launch");
+  MEMOPT_LAUNCH(launch_after(kern, static_cast<unsigned>(grid), C::THREADS, C::SMEM, s, p, qm, km, vm),
+                "packed_attention_kernel launch");
   return MEMOPT_OK;
 }
 

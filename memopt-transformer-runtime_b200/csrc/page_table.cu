@@ -98,7 +98,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
     const int b = b0 + tid;
     int n = 0, p = 0;
     if (b < a.B) {
-      int row = __ldg(a.rows + b), old = 0;
+      int row = a.rows[b], old = 0;
       if (row < 0 || row >= a.R) {
         bits |= MEMOPT_PAGES_BAD_ROW;
         row = 0;
@@ -110,7 +110,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
           old = 0;
         }
       }
-      n = a.amount ? __ldg(a.amount + b) : 0;
+      n = a.amount ? a.amount[b] : 0;
       if (n < 0 || (!kReserve && n > old)) {
         bits |= MEMOPT_PAGES_BAD_LENGTH;
         n = 0;
@@ -197,6 +197,8 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
   extern __shared__ uint8_t smem[];
   const Batch t = carve(smem, a.B);
   const int tid = threadIdx.x, lane = tid & 31;
+  begin_next();
+  after_previous();
   const int head = a.state[0], count = a.state[1];
   int64_t tokens, pages;
   uint32_t status = scan_batch<kThreads, true>(a, t, tokens, pages);
@@ -314,6 +316,8 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(const PageArgs a) {
   extern __shared__ uint8_t smem[];
   const Batch t = carve(smem, a.B);
   const int tid = threadIdx.x, lane = tid & 31;
+  begin_next();
+  after_previous();
   const int head = a.state[0], count = a.state[1];
   int64_t kept, pages;
   uint32_t status = scan_batch<kThreads, false>(a, t, kept, pages);
@@ -394,8 +398,7 @@ int launch_pages(K small, K large, const char* what, const PageArgs& a, cudaStre
   const int64_t per_cta = threads * kTokensPerThread, rows = threads / 32;
   const int64_t want = std::max((a.max_tokens + per_cta - 1) / per_cta, (a.B + rows - 1) / rows);
   const int grid = static_cast<int>(std::min<int64_t>(sm_count(), std::max<int64_t>(1, want)));
-  kern<<<grid, threads, smem, s>>>(a);
-  MEMOPT_LAUNCH_CHECK(what);
+  MEMOPT_LAUNCH(launch_after(kern, grid, threads, smem, s, a), what);
   return MEMOPT_OK;
 }
 

@@ -139,20 +139,22 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
                        : h < p.H + p.KVH
                            ? static_cast<const T*>(p.k) + t * p.k_stride + (h - p.H) * D
                            : static_cast<const T*>(p.v) + t * p.v_stride + (h - p.H - p.KVH) * D;
-        ua[i] = ld_stream_v4(src + d0);
-        ub[i] = ld_stream_v4(src + d1);
+        ua[i] = ld_once_v4(src + d0);
+        ub[i] = ld_once_v4(src + d1);
       }
     }
   };
+  begin_next();
+  after_previous();
   load(warp);
   // The angles of the CTA's tokens while the first loads are in flight.
   for (int i = tid; i < tokens * p.P; i += kWarps * 32) {
     const int k = i / p.P, pair = i - k * p.P;
     int axis = 0;
     for (int a = 0; a + 1 < p.axes; ++a) axis += pair >= p.ends[a];
-    const double f = __ldg(p.freq + pair) * 0.15915494309189535;  // 1 / (2 pi)
+    const double f = p.freq[pair] * 0.15915494309189535;  // 1 / (2 pi)
     const uint64_t turn64 = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
-    const int64_t pos = __ldg(p.pos + axis * p.T + t0 + k);
+    const int64_t pos = p.pos[axis * p.T + t0 + k];
     const uint64_t w = static_cast<uint64_t>(pos) * turn64;
     float cs, sn;
     // the top 32 bits as a signed fraction of a turn, in half turns
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
         *reinterpret_cast<uint4*>(dst + d1) = pack8<T>(b);
       }
       if (h >= p.H && p.slots) {
-        const int64_t slot = __ldg(p.slots + t);
+        const int64_t slot = p.slots[t];
         if (slot >= 0 && slot < p.num_slots) {
           __half* dst = is_v ? p.vc + (slot * p.KVH + (h - p.H - p.KVH)) * D : p.kc + (slot * p.KVH + (h - p.H)) * D;
           *reinterpret_cast<uint4*>(dst + d0) = pack8<__half>(a);
@@ -196,9 +198,8 @@ template <typename T, int D>
 int launch_rotary(const RotaryArgs& p, bool interleaved, int64_t ctas, cudaStream_t s) {
   const unsigned grid = static_cast<unsigned>(ctas);
   const size_t smem = sizeof(float2) * p.tokens * p.P;
-  if (interleaved) rotary_kernel<T, D, true><<<grid, kWarps * 32, smem, s>>>(p);
-  else rotary_kernel<T, D, false><<<grid, kWarps * 32, smem, s>>>(p);
-  MEMOPT_LAUNCH_CHECK("rotary_kernel launch");
+  auto kern = interleaved ? rotary_kernel<T, D, true> : rotary_kernel<T, D, false>;
+  MEMOPT_LAUNCH(launch_after(kern, grid, kWarps * 32, smem, s, p), "rotary_kernel launch");
   return MEMOPT_OK;
 }
 

@@ -660,6 +660,50 @@ def test_whole_step_in_a_graph():
     table2.check()
 
 
+def test_calls_back_to_back_wait_for_each_other():
+    """Each kernel may begin before the one ahead of it has ended, but reads its
+    results: chains without a synchronisation give what they give with one."""
+    from memopt import DevicePageTable, RotaryPositions
+
+    lens = [300, 5, 900, 33]
+    q, k, v = make_qkv(lens, 8, 8, 64, torch.bfloat16, seed=9, spread=1.0)
+    cu, rot = cu_of(lens), RotaryPositions(64)
+    pos = torch.arange(sum(lens), dtype=torch.int32, device=DEV)
+
+    def chain(after):
+        a, b, x = q, k, v
+        for _ in range(12):
+            a, b = rot.apply(a, b, pos)
+            after()
+            x = C().packed_attention(a, b, x, cu, 900)
+            after()
+        return a, b, x
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(torch.equal(g, w) for g, w in zip(chain(lambda: None), want))
+
+    rng = random.Random(1)
+    host, table = Host(3000, 16, 40, 90), DevicePageTable(3000, 16, 40, 1440)
+    plan = []
+    for _ in range(150):
+        rows = rng.sample(range(40), 20)
+        new = [rng.randint(0, 60) if host.lens[r] < 1300 else 0 for r in rows]
+        want = host.reserve(rows, new)
+        cut = rng.sample(range(40), 10)
+        keep = [rng.randint(0, host.lens[r]) for r in cut]
+        host.truncate(cut, keep)
+        plan.append(([table.ints(z) for z in (rows, new, cut, keep)], sum(new), want))
+    torch.cuda.synchronize()
+    got = []
+    for (rows, new, cut, keep), n, _ in plan:
+        got.append(table.reserve(rows, new, n))
+        table.truncate(cut, keep)
+    host.same(table)
+    for batch, (_, _, want) in zip(got, plan):
+        assert (batch.slot_mapping.tolist(), batch.positions.tolist()) == want
+
+
 def test_two_streams_at_once():
     """Two batches in flight on two streams do not disturb each other."""
     sets = [make_qkv([700, 40, 300], 8, 2, 128, torch.float16, seed=s) for s in (1, 2)]
