@@ -100,6 +100,9 @@ struct Cfg {
   static constexpr int STAGES = TILES == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);
   static constexpr int KV_OFF = TILES * TILE;
   static constexpr int SMEM = KV_OFF + STAGES * TILE + 1024;  // + alignment slack
+  // cu_seqlens kept in shared memory up to this many values: read from global
+  // memory they cost the scheduler 900 cycles a step beside the loads of K and V.
+  static constexpr int CU = TILES == 2 && D == 128 ? 256 : 3000;
   // With D = 64 tensor memory has room for P beside the scores: the next scores
   // are computed while the weights are, and a block takes its softmax alone.
   static constexpr bool OWN_P = kBN + D + kBN / 2 <= 256;
@@ -276,6 +279,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   __shared__ __align__(8) Bars<C::STAGES> bars;
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ int32_t cu_copy[C::CU];
   __shared__ __align__(16) uint4 next_cta;
 
   const int tid = threadIdx.x, lane = tid & 31;
@@ -314,6 +318,11 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   __syncthreads();
   tc::fence_after_sync();
   after_previous();
+  const bool copied = p.S + 1 <= C::CU;
+  if (copied) {
+    for (int i = tid; i <= p.S; i += C::THREADS) cu_copy[i] = p.cu[i];
+    __syncthreads();
+  }
   const uint32_t tmem = tmem_slot;
   // Tile t: scores at its first 128 columns, O behind them, P over the scores or behind O.
   auto tS = [&](int t) { return tmem + 256u * t; };
@@ -719,9 +728,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       // items run); within a chunk the items in descending order of work, within a
       // token block the units.
       const int tokens = tile_tokens * TILES;
+      const int32_t* cu = copied ? cu_copy : p.cu;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
-        lo = min(max(p.cu[s], 0), p.T);
-        hi = min(max(p.cu[s + 1], lo), p.T);
+        lo = min(max(cu[s], 0), p.T);
+        hi = min(max(cu[s + 1], lo), p.T);
       };
       auto nblocks = [&](int s) {
         int lo = 0, hi = 0;
@@ -730,6 +740,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       };
       int most = 0;
       int64_t all = 0;
+#pragma unroll 4
       for (int s = lane; s < p.S; s += 32) {
         const int nb = nblocks(s);
         most = max(most, nb);
@@ -748,9 +759,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       };
       auto count_on = [&](int L) {  // token blocks on a level
         int n = 0;
+#pragma unroll 4
         for (int s = lane; s < p.S; s += 32) n += on_level(s, L);
         n = __reduce_add_sync(0xffffffffu, n);
-        return p.causal ? static_cast<int64_t>(n) : static_cast<int64_t>(n) * L;
+        return static_cast<uint32_t>(p.causal ? n : n * L);
       };
       auto next_level = [&](int L) {
         if (p.causal) return L - 1;
@@ -761,12 +773,17 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         return static_cast<int>(__reduce_max_sync(0xffffffffu, below));
       };
-      const int64_t total = all * p.units, per_chunk = all * p.chunk;
-      int L = 0, unit0 = -p.chunk;
-      int64_t above = 0, here = 0;  // token blocks on the levels above, on this one
+      // The launch has at least as many CTAs as items, fewer than 2^31: indexes are
+      // 32-bit.  (Overlapping sequences, which the host cannot see, may have more
+      // items; those past the launch are not computed.)
+      const uint32_t blocks_all = static_cast<uint32_t>(min(all, static_cast<int64_t>(0x7fffffff) / p.units));
+      const uint32_t total = blocks_all * p.units, per_chunk = blocks_all * p.chunk;
+      int L = 0;
+      uint32_t chunk_first = 0, chunk_units = 0;  // the present chunk's head units
+      uint32_t above = 0, here = 0, on_first = 0;  // token blocks on the levels above, on this one, on the first
       int found_level = -1, found_s0 = 0, found_before = 0;  // sequences on the level before found_s0
       bool ok = true, more = true;  // more: there may be CTAs that have not begun
-      int64_t i = blockIdx.x;
+      uint32_t i = blockIdx.x;
       uint32_t asked = 0;
       // Takes the index of a CTA that has not begun (the launch has one per item at
       // most); false when there is none left.
@@ -796,23 +813,27 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         Item it{0, -1, 0, 0};
         if (more && i < total) {
-          const int first = static_cast<int>(i / per_chunk) * p.chunk, units = min(p.chunk, p.units - first);
-          const int64_t in_chunk = i - static_cast<int64_t>(first) * all, b = in_chunk / units;
-          if (first != unit0 || b < above) {
-            unit0 = first;
+          if (chunk_units == 0 || i < chunk_first * blocks_all || i >= (chunk_first + chunk_units) * blocks_all) {
+            chunk_first = i / per_chunk * p.chunk;
+            chunk_units = min(static_cast<uint32_t>(p.chunk), p.units - chunk_first);
+            above = here = 0;
+          }
+          const uint32_t in_chunk = i - chunk_first * blocks_all, b = in_chunk / chunk_units;
+          if (here == 0 || b < above) {
             above = 0;
             L = p.causal ? most - 1 : most;
-            here = count_on(L);
+            if (on_first == 0) on_first = count_on(L);
+            here = on_first;
           }
           while (b >= above + here) {
             above += here;
             L = next_level(L);
             here = count_on(L);
           }
-          const int per_seq = p.causal ? 1 : L, at_level = static_cast<int>(b - above);
+          const int at_level = static_cast<int>(b - above);
           // The sequence is the rank-th on the level.  Ranks grow from item to item:
           // the search goes on where the last one ended.
-          const int rank = at_level / per_seq;
+          const int rank = p.causal ? at_level : at_level / L;
           if (L != found_level || rank < found_before) {
             found_level = L;
             found_s0 = found_before = 0;
@@ -822,11 +843,13 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
             const uint32_t has = __ballot_sync(0xffffffffu, on_level(s0 + lane, L));
             const int n = __popc(has);
             if (skip < n) {
-              const int s = s0 + static_cast<int>(__fns(has, 0, skip + 1));
+              const bool found = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == skip;
+              const int s = s0 + __ffs(__ballot_sync(0xffffffffu, found)) - 1;
               int lo, hi;
               bounds(s, lo, hi);
               found_s0 = s0;
-              it = Item{lo, hi - lo, (p.causal ? L : at_level % L) * tokens, first + static_cast<int>(in_chunk - b * units)};
+              it = Item{lo, hi - lo, (p.causal ? L : at_level - rank * L) * tokens,
+                        static_cast<int>(chunk_first + in_chunk - b * chunk_units)};
               break;
             }
             skip -= n;
