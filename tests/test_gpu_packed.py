@@ -487,6 +487,42 @@ def test_page_table_refusals_change_nothing():
     table.check()
 
 
+def test_page_table_with_damaged_state():
+    """Values that no call writes (a foreign page in the ring or a row, a length
+    past the table) are reported and never become a slot."""
+    from memopt import DevicePageTable
+
+    table = DevicePageTable(10, 16, 3, 96)
+    table.free_pages[1] = 4711
+    table.free_pages[2] = -5
+    batch = table.reserve([0], [50])  # pages 0, 4711, -5, 3
+    assert batch.slot_mapping.tolist() == list(range(16)) + [-1] * 32 + [48, 49]
+    with pytest.raises(RuntimeError, match="out of range"):
+        table.check()
+    batch = table.reserve([0], [1])
+    assert batch.slot_mapping.tolist() == [50]
+    table.check()
+    table.truncate([0], [20])  # gives -5 and 3 back, reports the first
+    assert table.free_count() == 8
+    with pytest.raises(RuntimeError, match="out of range"):
+        table.check()
+    for bad in (-1, 97):
+        table.context_lens[1] = bad
+        before = table.pool_state[:2].clone()
+        batch = table.reserve([1], [1])
+        assert batch.slot_mapping.tolist() == [-1] and torch.equal(table.pool_state[:2], before)
+        with pytest.raises(RuntimeError, match="out of range"):
+            table.check()
+    table.context_lens[1] = 0
+    for head, count in ((-1, 3), (10, 3), (0, 11), (0, -1)):
+        table.pool_state[0], table.pool_state[1] = head, count
+        assert table.reserve([1], [1]).slot_mapping.tolist() == [-1]
+        table.truncate([2])
+        assert table.pool_state.tolist() == [head, count, 16, 0]
+        with pytest.raises(RuntimeError):
+            table.check()
+
+
 def test_page_table_step_in_a_graph():
     """A captured decode step: one token per row, replayed; half of the rows are cut back in between."""
     from memopt import DevicePageTable
@@ -541,15 +577,23 @@ def test_cache_prompt_decode_draft_evict(kv_format):
     assert ((out.double() - ref).abs() <= attention_tol(ref, mag, v, 300, torch.float16) +
             2.0 ** -10 * min(size, 64.0) * mag).all()
 
-    def rows_of(row):  # this row's cached keys and values, fp32 [n, KVH, D]
+    if kv_format == "int4":  # the turned keys are what the pool holds, to half a step of their group's scale
+        kcodes, kscale, _, _ = C().get_int4_pool_tensors()
+        for i, row in enumerate([0, 3, 1]):
+            n, first = lens[i], sum(lens[:i])
+            pages = cache.table.block_tables[row, : -(-n // BS)].long()
+            c = kcodes[pages].transpose(1, 2).reshape(-1, KVH, D // 2)[:n].long()
+            codes = torch.stack([c & 15, c >> 4], -1).reshape(n, KVH, D) - 8
+            scale = kscale[pages].transpose(1, 2).reshape(-1, KVH, D // 64)[:n].double().repeat_interleave(64, -1)
+            key = k64[first:first + n]
+            # half a step, the fp16 rounding of the key and that of the scale (7 steps of it)
+            tol = scale * (0.5 + 7 * 2.0 ** -11) + 2.0 ** -11 * key.abs() + 1e-6
+            assert ((codes * scale - key).abs() <= tol).all()
+
+    def rows_of(row):  # this row's cached keys and values [n, KVH, D]
         n = int(cache.table.context_lens[row])
         pages = cache.table.block_tables[row, : -(-n // BS)].long()
-        if kv_format == "fp16":
-            return [c[pages].reshape(-1, KVH, D)[:n].double() for c in C().get_pool_tensors()]
-        import oracle as O
-
-        kv = O.int4_dense(C().get_int4_pages().cpu().numpy(), BS, D) if hasattr(O, "int4_dense") else None
-        return kv
+        return [c[pages].reshape(-1, KVH, D)[:n].double() for c in C().get_pool_tensors()]
 
     def step(n):
         batch = cache.extend([0, 1, 3], n)
@@ -793,15 +837,20 @@ def test_layouts_other_than_contiguous(strides):
         assert torch.equal(C().packed_attention(lay(q), lay(k), lay(v), cu_of(lens), 90), want)
 
 
-def test_many_long_and_short_sequences_find_their_items():
-    """Several thousand sequences: every row belongs to exactly one item."""
-    rng = random.Random(5)
-    lens = [rng.choice([0, 1, 5, 40, 65, 130, 300]) for _ in range(3000)] + [2500]
+@pytest.mark.parametrize("many,D", [(3000, 64), (900, 128), (260, 128)])
+def test_many_long_and_short_sequences_find_their_items(many, D):
+    """Hundreds to thousands of sequences (more than a CTA keeps the bounds of,
+    with one and with two tiles an item): every row belongs to exactly one item."""
+    rng = random.Random(many)
+    if many == 260:  # long ones: two tiles an item
+        lens = [rng.randint(700, 900) for _ in range(many)]
+    else:
+        lens = [rng.choice([0, 1, 5, 40, 65, 130, 300]) for _ in range(many)] + [2500]
     for causal in (True, False):
         T = sum(lens)
-        q = torch.zeros(T, 2, 64, dtype=torch.float16, device=DEV)
-        k = torch.zeros(T, 1, 64, dtype=torch.float16, device=DEV)
-        v = (torch.arange(T, device=DEV) % 7).half()[:, None, None].expand(T, 1, 64).contiguous()
+        q = torch.zeros(T, 2, D, dtype=torch.float16, device=DEV)
+        k = torch.zeros(T, 1, D, dtype=torch.float16, device=DEV)
+        v = (torch.arange(T, device=DEV) % 7).half()[:, None, None].expand(T, 1, D).contiguous()
         out = torch.full_like(q, float("nan"))
         C().packed_attention(q, k, v, cu_of(lens), 2500, -1, causal, out)
         # equal scores: the mean of the visible values
