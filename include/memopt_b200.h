@@ -451,11 +451,17 @@ int memopt_rotary_write_cache(const void* query, int64_t query_stride, const voi
 /* are scaled by 1 / sqrt(head_dim).  Tokens that a row does not see never    */
 /* reach it, whatever they hold.  Rows outside every sequence are not         */
 /* written.  max_seqlen (the longest sequence, or an upper bound) only helps  */
-/* to choose launch shapes.  head_dim 64 or 128.                              */
+/* to choose launch shapes.  head_dim 64 or 128.  Few rows with many keys are */
+/* split along the keys and joined: the workspace (16-byte aligned, no initial */
+/* values; memopt_packed_attention_workspace_size bytes for the same arguments, */
+/* 0 for most calls) holds the partial results.                               */
+size_t memopt_packed_attention_workspace_size(int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads,
+                                              int num_kv_heads, int head_dim, int window_size, int causal);
 int memopt_packed_attention(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
                             const void* values, int64_t value_stride, int dtype, const int32_t* cu_seqlens,
                             int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads, int num_kv_heads,
-                            int head_dim, int window_size, int causal, void* out, void* stream);
+                            int head_dim, int window_size, int causal, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

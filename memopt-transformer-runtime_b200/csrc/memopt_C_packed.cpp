@@ -272,9 +272,14 @@ torch::Tensor packed_attention(torch::Tensor query, torch::Tensor keys, torch::T
   auto q = packed_rows(query), k = packed_rows(keys), v = packed_rows(values);
   cu_seqlens = cu_seqlens.contiguous();
   const int window = window_size <= 0 || window_size > 0x7fffffff ? 0 : static_cast<int>(window_size);
+  const size_t ws_bytes = memopt_packed_attention_workspace_size(S, T, static_cast<int>(max_seqlen), H, KVH, D, window,
+                                                                 causal ? 1 : 0);
+  torch::Tensor ws;
+  if (ws_bytes > 0) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, query.options().dtype(torch::kUInt8));
   check(memopt_packed_attention(q.data_ptr(), row_stride(q), k.data_ptr(), row_stride(k), v.data_ptr(), row_stride(v),
                                 dtype, cu_seqlens.data_ptr<int32_t>(), S, T, static_cast<int>(max_seqlen), H, KVH, D,
-                                window, causal ? 1 : 0, out.data_ptr(), cur_stream()),
+                                window, causal ? 1 : 0, out.data_ptr(), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                cur_stream()),
         who);
   return out;
 }

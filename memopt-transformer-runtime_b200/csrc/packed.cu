@@ -67,6 +67,10 @@ namespace packed {
 constexpr int kBN = 128;       // keys per block
 constexpr int kFirst = 6;       // of the 8 steps of 16 keys, those that P.V starts with
 constexpr int kAhead = 3;       // blocks before an item's last loads at which the next item is taken
+constexpr double kSplitGain = 6;    // key blocks that a split has to save on the longest walk
+constexpr double kItemBlocks = 4;   // what an item costs beside its walk, in key blocks
+constexpr int64_t kMaxWorkspace = int64_t(256) << 20;
+constexpr int kMaxPieces = 16;
 constexpr int kMaxGp = 16;     // query heads packed into a tile
 
 struct Params {
@@ -80,6 +84,11 @@ struct Params {
   int chunk;        // head units walked together
   int window, causal;
   float qscale;     // log2(e) / sqrt(D)
+  // Split items: key blocks of a piece, most pieces of a tile, and for every tile,
+  // head unit and piece the unscaled O [D/4][128 rows] float4 and the rows' (m, l).
+  int split, pieces;
+  float4* part_o;
+  float2* part_ml;
 };
 
 // TILES: 128-row tiles of an item.  Two share the K/V blocks and take turns on the
@@ -112,6 +121,7 @@ struct Cfg {
 
 struct Item {
   int start, n, t0, unit;  // first packed row, length, first token, head unit (n < 0: no more items)
+  int piece, slot;         // split items: which piece, and where its partial result goes
 };
 
 // Bounded wait: ten seconds by the global timer, read every 4096 polls.
@@ -143,6 +153,22 @@ __device__ __forceinline__ Range tile_range(const Params& p, const Item& it, int
   const int c_last = p.causal ? end : it.n, c_first = p.causal ? first + 1 : it.n;
   const int from = p.window > 0 && c_first > p.window ? c_first - p.window : 0;
   return {from / kBN, (c_last + kBN - 1) / kBN, c_last};
+}
+
+// Pieces that a range of key blocks is split into (the last one takes what is left).
+__device__ __forceinline__ int pieces_of(const Params& p, int blocks) {
+  return min(p.pieces, (blocks + p.split - 1) / p.split);
+}
+// What an item does of its tile's range.
+template <int TILES, bool SPLIT>
+__device__ __forceinline__ Range item_range(const Params& p, const Item& it, int t) {
+  Range r = tile_range<TILES>(p, it, t);
+  if (SPLIT && r.hi > 0) {
+    const int lo = r.lo + it.piece * p.split;
+    if (it.piece < p.pieces - 1) r.hi = min(r.hi, lo + p.split);
+    r.lo = lo;
+  }
+  return r;
 }
 
 template <typename T>
@@ -192,7 +218,8 @@ __device__ __forceinline__ float ex2_mufu(float x) {
 // One row from its definition, by one warp: lane l holds dims [l D/32, (l+1) D/32),
 // four keys at a time.  Only rows whose fast result is not finite come here.
 template <typename T, int D>
-__device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int64_t key0, int begin, int end) {
+__device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int64_t key0, int begin, int end,
+                                        int dim0 = 0, int dims = D) {
   constexpr int E = D / 64;  // 32-bit words per lane
   const int lane = threadIdx.x & 31, hk = h / p.group;
   auto words = [&](const void* base, int64_t at, uint32_t (&w)[E]) {
@@ -253,7 +280,10 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
   }
   uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (row * p.H + h) * D) + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = pack2<T>(acc[2 * e] / l, acc[2 * e + 1] / l);
+  for (int e = 0; e < E; ++e) {
+    const int d = 2 * (lane * E + e);
+    if (d >= dim0 && d < dim0 + dims) dst[e] = pack2<T>(acc[2 * e] / l, acc[2 * e + 1] / l);
+  }
 }
 
 // Barriers: items (2 slots: filled by the scheduler, read by the warps that
@@ -266,7 +296,7 @@ struct Bars {
   uint64_t s_full[2], p_part[2][2], pv_done[2], s_read[2], end[2], next, near_end;
 };
 
-template <typename T, int D, int TILES>
+template <typename T, int D, int TILES, bool SPLIT>
 __global__ void __launch_bounds__(128 * TILES + 128, 3 - TILES)
 packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qmap,
                         const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -340,6 +370,10 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     it.n = __shfl_sync(0xffffffffu, src.n, 0);
     it.t0 = __shfl_sync(0xffffffffu, src.t0, 0);
     it.unit = __shfl_sync(0xffffffffu, src.unit, 0);
+    if (SPLIT) {
+      it.piece = __shfl_sync(0xffffffffu, src.piece, 0);
+      it.slot = __shfl_sync(0xffffffffu, src.slot, 0);
+    }
     if (lane == 0) mbar_arrive(at(bars.item_free[k & 1]));
     return it.n >= 0;
   };
@@ -355,7 +389,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
     bool ok = true;
     Item it;
     for (int k = 0; ok && next_item(k, it); ++k) {
-      const Range r = tile_range<TILES>(p, it, t);
+      const Range r = item_range<TILES, SPLIT>(p, it, t);
       if (r.hi == 0) continue;
       const int tok = it.t0 + t * tile_tokens + (row >> p.gshift);
       const int h = (it.unit << p.gshift) + (row & ((1 << p.gshift) - 1));
@@ -526,6 +560,26 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       }
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
       tc::fence_after_sync();
+      if (SPLIT) {
+        const Range whole = tile_range<TILES>(p, it, t);
+        if (pieces_of(p, whole.hi - whole.lo) > 1) {
+          // One of several pieces: O as it is, and the row's maximum and sum.
+          const int64_t at = static_cast<int64_t>(it.slot) * p.pieces + it.piece;
+          float4* po = p.part_o + at * (D / 4) * 128 + row;
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            float v[32];
+            tc::ld32(tO(t) + lane_base + cc * 32, v);
+            tc::wait_ld(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              po[(cc * 8 + e) * 128] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+          p.part_ml[at * 128 + row] = make_float2(m_run, ok ? l_run : __int_as_float(0x7fffffff));
+          tc::fence_before_sync();
+          continue;
+        }
+      }
       // Epilogue: 32 dims of a row are four 16-byte pieces of its thread; the four
       // threads of neighbouring rows exchange pieces, so that a store writes 64
       // contiguous bytes of each of 8 rows instead of 16 bytes of 32 rows.
@@ -606,7 +660,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       };
       Item it;
       for (int k = 0; ok && next_item(k, it); ++k) {
-        const Range r0 = tile_range<TILES>(p, it, 0), r1 = tile_range<TILES>(p, it, 1);
+        const Range r0 = item_range<TILES, SPLIT>(p, it, 0), r1 = item_range<TILES, SPLIT>(p, it, 1);
         const int LO = r0.lo, HI = max(r0.hi, r1.hi);  // tile 0 exists and starts first
         const int lo = t ? r1.lo : r0.lo, hi = t ? r1.hi : r0.hi, last = t ? r1.last : r0.last;
         auto scores = [&](int j) {  // S(j) if the tile has the block; lets K(j) and, at the end, Q go
@@ -688,7 +742,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       bool ok = true;
       Item it;
       for (int k = 0; ok && next_item(k, it); ++k) {
-        const Range r0 = tile_range<TILES>(p, it, 0), r1 = tile_range<TILES>(p, it, 1);
+        const Range r0 = item_range<TILES, SPLIT>(p, it, 0), r1 = item_range<TILES, SPLIT>(p, it, 1);
         const int LO = r0.lo, HI = max(r0.hi, r1.hi);
         const int h0 = it.unit << p.gshift, hk = h0 / p.group;
         if (lane == 0) {
@@ -727,7 +781,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       // Head units in chunks (their keys and values stay in L2 while the chunk's
       // items run); within a chunk the items in descending order of work, within a
       // token block the units.
-      const int tokens = tile_tokens * TILES;
+      const int tshift = 7 - p.gshift + (TILES - 1), tokens = 1 << tshift;
       const int32_t* cu = copied ? cu_copy : p.cu;
       auto bounds = [&](int s, int& lo, int& hi) {  // device data: kept inside the tensors
         lo = min(max(cu[s], 0), p.T);
@@ -736,7 +790,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       auto nblocks = [&](int s) {
         int lo = 0, hi = 0;
         if (s < p.S) bounds(s, lo, hi);
-        return (hi - lo + tokens - 1) / tokens;
+        return (hi - lo + tokens - 1) >> tshift;
       };
       int most = 0;
       int64_t all = 0;
@@ -753,16 +807,30 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       // block in its sequence, descending; a sequence has one block on it if it
       // is long enough.  Not causal: level = blocks of the sequence, descending;
       // a sequence of that many has all of them on it.
-      auto on_level = [&](int s, int L) {
-        const int nb = nblocks(s);
-        return p.causal ? nb > L : nb == L;
+      auto reaches = [&](int nb, int L) { return p.causal ? nb > L : nb == L; };
+      auto on_level = [&](int s, int L) { return reaches(nblocks(s), L); };
+      // Up to 32 sequences, a sequence to a lane, are counted without a loop: few
+      // sequences have many levels, and a CTA's first item may lie far down (one
+      // prompt of 4000 tokens, 16/4 heads 89 -> 66 us).
+      const int own_blocks = nblocks(lane);
+      // Pieces of a token block on a level, at most (a shorter last block may have
+      // fewer; what is too many is skipped).
+      auto pieces_on = [&](int L) {
+        if (!SPLIT) return 1;
+        const int hi = ((p.causal ? L + 1 : L) * tokens + kBN - 1) / kBN;
+        const int first = (p.causal ? L : L - 1) * tokens + 1;
+        return pieces_of(p, hi - (p.window > 0 && first > p.window ? (first - p.window) / kBN : 0));
       };
-      auto count_on = [&](int L) {  // token blocks on a level
+      auto count_on = [&](int L) {  // token blocks (split: their pieces) on a level
         int n = 0;
+        if (p.S <= 32) {
+          n = __popc(__ballot_sync(0xffffffffu, reaches(own_blocks, L)));
+        } else {
 #pragma unroll 4
-        for (int s = lane; s < p.S; s += 32) n += on_level(s, L);
-        n = __reduce_add_sync(0xffffffffu, n);
-        return static_cast<uint32_t>(p.causal ? n : n * L);
+          for (int s = lane; s < p.S; s += 32) n += on_level(s, L);
+          n = __reduce_add_sync(0xffffffffu, n);
+        }
+        return static_cast<uint32_t>(p.causal ? n : n * L) * pieces_on(L);
       };
       auto next_level = [&](int L) {
         if (p.causal) return L - 1;
@@ -801,61 +869,107 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         i = cta;
         return got;
       };
+      // The item of index i; false when there is none.
+      auto find = [&](Item& it) -> bool {
+        if (!SPLIT && i >= total) return false;
+        if (SPLIT) {
+          chunk_units = p.units;  // few items: all units at once
+        } else if (chunk_units == 0 || i < chunk_first * blocks_all || i >= (chunk_first + chunk_units) * blocks_all) {
+          chunk_first = i / per_chunk * p.chunk;
+          chunk_units = min(static_cast<uint32_t>(p.chunk), p.units - chunk_first);
+          above = here = 0;
+        }
+        const uint32_t in_chunk = SPLIT ? i : i - chunk_first * blocks_all, b = in_chunk / chunk_units;
+        if (here == 0 || b < above) {
+          above = 0;
+          L = p.causal ? most - 1 : most;
+          if (on_first == 0 && most > 0) on_first = count_on(L);
+          here = on_first;
+        }
+        while (b >= above + here) {
+          above += here;
+          L = next_level(L);
+          if (SPLIT && (p.causal ? L < 0 : L <= 0)) {
+            here = 0;
+            return false;
+          }
+          if (!SPLIT || !p.causal) {
+            here = count_on(L);
+            continue;
+          }
+          // Split items are found by a level to a lane, 32 levels at once: each has
+          // its own number of pieces (one prompt of 4000 tokens, 4/1 heads 52 -> 33 us).
+          const int own = max(L - lane, 0);
+          uint32_t n = 0;
+          for (int s = 0; s < p.S; ++s) n += reaches(p.S <= 32 ? __shfl_sync(0xffffffffu, own_blocks, s) : nblocks(s), own);
+          n = L >= lane ? n * pieces_on(own) : 0;
+          uint32_t sum = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += v;
+          }
+          const uint32_t reached = __ballot_sync(0xffffffffu, b < above + sum);
+          const int from = reached ? __ffs(reached) - 1 : 31;
+          above += __shfl_sync(0xffffffffu, reached ? sum - n : sum, from);
+          here = reached ? __shfl_sync(0xffffffffu, n, from) : 0;
+          L -= from;
+        }
+        const int at_level = static_cast<int>(b - above), pieces = pieces_on(L);
+        // The sequence is the rank-th on the level.  Ranks grow from item to item:
+        // the search goes on where the last one ended.
+        const int per_seq = p.causal ? pieces : L * pieces;
+        const int rank = p.causal && !SPLIT ? at_level : at_level / per_seq;
+        if (L != found_level || rank < found_before) {
+          found_level = L;
+          found_s0 = found_before = 0;
+        }
+        int skip = rank - found_before;
+        for (int s0 = found_s0; s0 < p.S; s0 += 32) {
+          const uint32_t has = __ballot_sync(0xffffffffu, on_level(s0 + lane, L));
+          const int n = __popc(has);
+          if (skip < n) {
+            const bool found = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == skip;
+            const int s = s0 + __ffs(__ballot_sync(0xffffffffu, found)) - 1;
+            int lo, hi;
+            bounds(s, lo, hi);
+            found_s0 = s0;
+            const int rest = at_level - rank * per_seq;
+            const int tile = p.causal ? L : SPLIT ? rest / pieces : rest;
+            const int unit = static_cast<int>(chunk_first + in_chunk - b * chunk_units);
+            it = Item{lo, hi - lo, tile * tokens, unit, 0, 0};
+            if (SPLIT) {
+              it.piece = p.causal ? rest : rest % pieces;
+              it.slot = ((lo + it.t0) / tokens + s) * p.units + unit;
+            }
+            return true;
+          }
+          skip -= n;
+          found_before += n;
+        }
+        return false;
+      };
       for (int k = 0; ok; ++k) {
         if (k >= 2) ok = __all_sync(0xffffffffu, wait_bar(at(bars.item_free[k & 1]), ((k >> 1) - 1) & 1));
         if (!ok) break;
         // Not before the item at hand nears its end: what is taken early is missing
-        // where another CTA runs dry.  The answer takes up to 10 us.
+        // where another CTA runs dry.
         if (k > 0) {
           ok = __all_sync(0xffffffffu, wait_bar(at(bars.near_end), (k - 1) & 1));
           if (!ok) break;
           more = take_next();
         }
-        Item it{0, -1, 0, 0};
-        if (more && i < total) {
-          if (chunk_units == 0 || i < chunk_first * blocks_all || i >= (chunk_first + chunk_units) * blocks_all) {
-            chunk_first = i / per_chunk * p.chunk;
-            chunk_units = min(static_cast<uint32_t>(p.chunk), p.units - chunk_first);
-            above = here = 0;
+        Item it{0, -1, 0, 0, 0, 0}, got = it;
+        while (more) {
+          if (!find(got)) break;
+          const Range r = item_range<TILES, SPLIT>(p, got, 0);
+          if (!SPLIT || r.lo < r.hi) {
+            it = got;
+            break;
           }
-          const uint32_t in_chunk = i - chunk_first * blocks_all, b = in_chunk / chunk_units;
-          if (here == 0 || b < above) {
-            above = 0;
-            L = p.causal ? most - 1 : most;
-            if (on_first == 0) on_first = count_on(L);
-            here = on_first;
-          }
-          while (b >= above + here) {
-            above += here;
-            L = next_level(L);
-            here = count_on(L);
-          }
-          const int at_level = static_cast<int>(b - above);
-          // The sequence is the rank-th on the level.  Ranks grow from item to item:
-          // the search goes on where the last one ended.
-          const int rank = p.causal ? at_level : at_level / L;
-          if (L != found_level || rank < found_before) {
-            found_level = L;
-            found_s0 = found_before = 0;
-          }
-          int skip = rank - found_before;
-          for (int s0 = found_s0; s0 < p.S; s0 += 32) {
-            const uint32_t has = __ballot_sync(0xffffffffu, on_level(s0 + lane, L));
-            const int n = __popc(has);
-            if (skip < n) {
-              const bool found = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == skip;
-              const int s = s0 + __ffs(__ballot_sync(0xffffffffu, found)) - 1;
-              int lo, hi;
-              bounds(s, lo, hi);
-              found_s0 = s0;
-              it = Item{lo, hi - lo, (p.causal ? L : at_level - rank * L) * tokens,
-                        static_cast<int>(chunk_first + in_chunk - b * chunk_units)};
-              break;
-            }
-            skip -= n;
-            found_before += n;
-          }
+          more = take_next();  // a piece that this token block does not have
         }
+        if (!ok) break;
         if (lane == 0) {
           items[k & 1] = it;
           mbar_arrive(at(bars.item_full[k & 1]));
@@ -870,6 +984,87 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, 256 * TILES);
+}
+
+// Joins the pieces of a tile: with M the largest of the pieces' maxima,
+// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p.  A CTA for 16 dims of a tile
+// and head unit, a thread for a row: its loads do not wait for one another.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Params p) {
+  const int row = threadIdx.x, tokens = 128 >> p.gshift;
+  const int g = blockIdx.x / p.units, unit = blockIdx.x - g * p.units;
+  after_previous();
+  auto bounds = [&](int s, int& lo, int& hi) {
+    lo = min(max(p.cu[s], 0), p.T);
+    hi = min(max(p.cu[s + 1], lo), p.T);
+  };
+  // The tile's number is (first packed row of it) / tokens + its sequence, which
+  // grows along the batch: the last sequence whose first tile is not behind g.
+  int lo = 0, hi = 0, s = 0;
+  for (int below = 0, above = p.S; below < above;) {
+    const int mid = (below + above) / 2;
+    bounds(mid, lo, hi);
+    if (lo / tokens + mid <= g) {
+      s = mid;
+      below = mid + 1;
+    } else {
+      above = mid;
+    }
+  }
+  bounds(s, lo, hi);
+  const int tile = g - (lo / tokens + s);
+  Item it{lo, hi - lo, tile * tokens, unit, 0, 0};
+  if (tile < 0 || static_cast<int64_t>(tile) * tokens >= it.n) return;
+  const Range r = tile_range<1>(p, it, 0);
+  const int pieces = pieces_of(p, r.hi - r.lo);
+  if (pieces <= 1) return;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * p.pieces;
+  const float2* ml = p.part_ml + at * 128 + row;
+  const float4* po = p.part_o + (at * (D / 4) + blockIdx.y * 4) * 128 + row;
+  float m = -INFINITY, l = 0.f, w[kMaxPieces];
+#pragma unroll
+  for (int i = 0; i < kMaxPieces; ++i) {
+    w[i] = i < pieces ? ml[i * 128].x : -INFINITY;
+    m = fmaxf(m, w[i]);
+  }
+  float acc[16] = {};
+#pragma unroll
+  for (int i = 0; i < kMaxPieces; ++i) {
+    if (i >= pieces) continue;
+    w[i] = w[i] == -INFINITY ? 0.f : exp2f(w[i] - m);  // nothing seen in the piece: its sum is 0
+    l += w[i] * ml[i * 128].y;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 o = po[(i * (D / 4) + c) * 128];
+      acc[4 * c] += w[i] * o.x, acc[4 * c + 1] += w[i] * o.y;
+      acc[4 * c + 2] += w[i] * o.z, acc[4 * c + 3] += w[i] * o.w;
+    }
+  }
+  float odd = 0.f;  // becomes NaN when an element is not finite
+#pragma unroll
+  for (int e = 0; e < 16; ++e) odd = fmaf(acc[e], 0.f, odd);
+  const int tok = it.t0 + (row >> p.gshift), h = (unit << p.gshift) + (row & ((1 << p.gshift) - 1));
+  const int c = p.causal ? min(tok + 1, it.n) : it.n;
+  const int ws = p.window > 0 && c > p.window ? c - p.window : 0;
+  if (tok < it.n) {
+    const float inv = 1.f / l;
+    uint32_t out[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (static_cast<int64_t>(lo + tok) * p.H + h) * D +
+                                          blockIdx.y * 16);
+    dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+    dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  }
+  uint32_t redo = __ballot_sync(0xffffffffu, tok < it.n && !(odd == 0.f && l >= 0.5f && l < 1.2e30f));
+  __syncwarp();
+  while (redo) {
+    const int from = __ffs(redo) - 1;
+    redo &= redo - 1;
+    const int rt = __shfl_sync(0xffffffffu, tok, from), rh = __shfl_sync(0xffffffffu, h, from);
+    const int rb = __shfl_sync(0xffffffffu, ws, from), re = __shfl_sync(0xffffffffu, c, from);
+    row_by_row<T, D>(p, lo + rt, rh, lo, rb, re, blockIdx.y * 16, 16);
+  }
 }
 
 namespace {
@@ -907,8 +1102,72 @@ int map_rows(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_
   return MEMOPT_OK;
 }
 
-template <typename T, int D, int TILES>
-int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
+// How a call is launched.
+struct Plan {
+  int gshift, units, tiles;
+  int split, pieces;       // 0: no item is split
+  int64_t tile_slots;      // tiles x head units that may exist
+  int64_t grid, workspace;
+};
+Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window, bool causal) {
+  Plan pl{};
+  const int group = H / KVH, slots = 2 * sm_count();
+  while ((2 << pl.gshift) <= kMaxGp && group % (2 << pl.gshift) == 0) ++pl.gshift;
+  pl.units = H >> pl.gshift;
+  // At most this many items (each sequence has one partial token block at most).
+  const int64_t tokens = 128 >> pl.gshift;
+  auto most_items = [&](int tiles) { return (T / (tokens * tiles) + S) * pl.units; };
+  // Two tiles an item halve the K/V traffic and pay where the walk over the keys is
+  // long and the items are many: 2 x 8192 tokens, 32 heads 1.05 against 1.11 ms with
+  // one tile, 8 x 2048 with 32/8 heads 265 against 281 us, 4 prompts up to 7696 with
+  // 4/1 heads 155 against 205.  One tile, two CTAs to an SM, hides an item's ends
+  // better and makes twice the items: 32 x 512 118 against 123 us, 64 x 32 tokens
+  // 16.0 against 21.1, one prompt of 1000 24 against 27, 8192 tokens of 4 heads 108
+  // against 117.
+  pl.tiles = T >= 768LL * S && most_items(2) >= 2 * sm_count() ? 2 : 1;
+  // Few rows with long walks: the longest item would go on alone, so items are split
+  // into pieces of `split` key blocks.  With the longest sequence as hinted and the
+  // others of equal length: causal walks grow along a sequence and make about
+  // (all their blocks) / split + half an item per tile; other walks are alike and
+  // make ceil(walk / split) each.  The split that fills `rounds` items for every CTA
+  // slot is taken where `rounds` times it and an item's own time (kItemBlocks) is least.
+  const int64_t longest = std::min<int64_t>(T, std::max<int64_t>(max_seqlen, (T + S - 1) / S));
+  const int64_t others = S > 1 ? (T - longest) / (S - 1) : 0;
+  auto walk_of = [&](int64_t n) {  // key blocks of a row's walk over a sequence of n tokens, at most
+    return ((window > 0 ? std::min<int64_t>(n, int64_t(window) + 128) : n) + kBN - 1) / kBN;
+  };
+  auto tiles_of = [&](int64_t n) { return (n + tokens - 1) / tokens; };
+  const int64_t walk = walk_of(longest);
+  const double tiles = static_cast<double>(tiles_of(longest) + (S - 1) * tiles_of(others)) * pl.units;
+  const double blocks = 0.5 * (tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) * pl.units;
+  pl.tile_slots = most_items(1);
+  double best = walk - kSplitGain;
+  for (int rounds = 1; rounds <= 3; ++rounds) {
+    double split;
+    if (causal && window <= 0) {
+      if (rounds * slots <= 0.5 * tiles) continue;
+      split = std::ceil(blocks / (rounds * slots - 0.5 * tiles));
+    } else {
+      if (rounds * slots < tiles) continue;
+      split = std::ceil(walk / std::floor(rounds * slots / tiles));
+    }
+    split = std::max(3.0, split);
+    const double time = rounds * (split + kItemBlocks) - kItemBlocks;
+    const int64_t pieces = std::min<int64_t>(kMaxPieces, static_cast<int64_t>((walk + split - 1) / split));
+    const int64_t bytes = pl.tile_slots * pieces * 128 * (D * 4 + 8);
+    if (time >= best || pieces < 2 || bytes > kMaxWorkspace) continue;
+    best = time;
+    pl.split = static_cast<int>(split);
+    pl.pieces = static_cast<int>(pieces);
+    pl.workspace = bytes;
+  }
+  if (pl.split) pl.tiles = 1;
+  pl.grid = most_items(pl.tiles) * std::max(1, pl.pieces);
+  return pl;
+}
+
+template <typename T, int D, int TILES, bool SPLIT>
+int launch(const Params& p, int KVH, const Plan& pl, cudaStream_t s) {
   using C = Cfg<D, TILES>;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   alignas(64) CUtensorMap qm, km, vm;
@@ -917,17 +1176,21 @@ int launch(const Params& p, int KVH, int64_t grid, cudaStream_t s) {
   if (st == MEMOPT_OK) st = map_rows(&km, p.k, bf16, p.T, p.k_stride, KVH, D, 1, kBN);
   if (st == MEMOPT_OK) st = map_rows(&vm, p.v, bf16, p.T, p.v_stride, KVH, D, 1, kBN);
   if (st != MEMOPT_OK) return st;
-  auto kern = packed_attention_kernel<T, D, TILES>;
+  auto kern = packed_attention_kernel<T, D, TILES, SPLIT>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed_attention)");
-  MEMOPT_LAUNCH(launch_after(kern, static_cast<unsigned>(grid), C::THREADS, C::SMEM, s, p, qm, km, vm),
+  MEMOPT_LAUNCH(launch_after(kern, static_cast<unsigned>(pl.grid), C::THREADS, C::SMEM, s, p, qm, km, vm),
                 "packed_attention_kernel launch");
+  if (SPLIT)
+    MEMOPT_LAUNCH(launch_after(join_pieces_kernel<T, D>, dim3(static_cast<unsigned>(pl.tile_slots), D / 16), 128, 0, s, p),
+                  "join_pieces_kernel launch");
   return MEMOPT_OK;
 }
 
 template <typename T, int D>
-int launch(const Params& p, int KVH, int tiles, int64_t grid, cudaStream_t s) {
-  return tiles == 1 ? launch<T, D, 1>(p, KVH, grid, s) : launch<T, D, 2>(p, KVH, grid, s);
+int launch(const Params& p, int KVH, const Plan& pl, cudaStream_t s) {
+  if (pl.split) return launch<T, D, 1, true>(p, KVH, pl, s);
+  return pl.tiles == 1 ? launch<T, D, 1, false>(p, KVH, pl, s) : launch<T, D, 2, false>(p, KVH, pl, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -938,11 +1201,22 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 using namespace memopt;
 
+extern "C" size_t memopt_packed_attention_workspace_size(int num_seqs, int64_t total_tokens, int max_seqlen,
+                                                         int num_heads, int num_kv_heads, int head_dim,
+                                                         int window_size, int causal) {
+  if (num_seqs <= 0 || total_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return static_cast<size_t>(packed::plan_of(num_seqs, total_tokens, max_seqlen, num_heads, num_kv_heads, head_dim,
+                                             window_size, causal != 0)
+                                 .workspace);
+}
+
 extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
                                        const void* values, int64_t value_stride, int dtype, const int32_t* cu_seqlens,
                                        int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads,
                                        int num_kv_heads, int head_dim, int window_size, int causal, void* out,
-                                       void* stream) {
+                                       void* workspace, size_t workspace_bytes, void* stream) {
   if (num_seqs < 0 || total_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
     return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: invalid geometry");
   if (dtype != MEMOPT_DTYPE_F16 && dtype != MEMOPT_DTYPE_BF16)
@@ -961,33 +1235,28 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   p.q = query, p.k = keys, p.v = values, p.out = out, p.cu = cu_seqlens;
   p.q_stride = query_stride, p.k_stride = key_stride, p.v_stride = value_stride;
   p.T = static_cast<int>(total_tokens), p.S = num_seqs, p.H = num_heads, p.group = num_heads / num_kv_heads;
-  while ((2 << p.gshift) <= packed::kMaxGp && p.group % (2 << p.gshift) == 0) ++p.gshift;
-  p.units = num_heads >> p.gshift;
+  packed::Plan pl = packed::plan_of(num_seqs, total_tokens, max_seqlen, num_heads, num_kv_heads, head_dim, window_size,
+                                    causal != 0);
+  if (pl.split && (workspace == nullptr || workspace_bytes < static_cast<size_t>(pl.workspace)))
+    return fail(MEMOPT_ERR_WORKSPACE, "packed_attention: workspace too small (need " + std::to_string(pl.workspace) +
+                                          " bytes)");
+  if (pl.split && !packed::aligned16(workspace))
+    return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: workspace must be 16-byte aligned");
+  p.gshift = pl.gshift, p.units = pl.units, p.split = pl.split, p.pieces = pl.pieces;
+  p.part_o = static_cast<float4*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + pl.tile_slots * pl.pieces * (head_dim / 4) * 128);
   p.window = window_size > 0 ? window_size : 0, p.causal = causal ? 1 : 0;
   p.qscale = (1.0f / sqrtf(static_cast<float>(head_dim))) * 1.4426950408889634f;
-  // At most this many items (each sequence has one partial token block at most).
-  const int64_t tokens = 128 >> p.gshift;
-  auto most_items = [&](int tiles) { return (total_tokens / (tokens * tiles) + num_seqs) * p.units; };
-  // Two tiles an item halve the K/V traffic and pay where the walk over the keys is
-  // long and the items are many: 2 x 8192 tokens, 32 heads 1.05 against 1.11 ms with
-  // one tile, 8 x 2048 with 32/8 heads 265 against 281 us, 4 prompts up to 7696 with
-  // 4/1 heads 155 against 205.  One tile, two CTAs to an SM, hides an item's ends
-  // better and makes twice the items: 32 x 512 118 against 123 us, 64 x 32 tokens
-  // 16.0 against 21.1, one prompt of 1000 24 against 27, 8192 tokens of 4 heads 108
-  // against 117.
-  const int tiles = total_tokens >= 768LL * num_seqs && most_items(2) >= 2 * sm_count() ? 2 : 1;
   // Head units per chunk: the chunk's keys and values fill about a quarter of L2.
   // Units that share a KV head stay together.
   const int per_kv = p.group >> p.gshift;
   const int64_t kv_bytes = total_tokens * head_dim * 4;
   p.chunk = static_cast<int>(std::min<int64_t>(p.units, per_kv * std::max<int64_t>(1, (int64_t(32) << 20) / kv_bytes)));
-  (void)max_seqlen;
-  const int64_t grid = most_items(tiles);
-  if (grid > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many work items");
+  if (pl.grid > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many work items");
   cudaStream_t s = as_stream(stream);
   if (dtype == MEMOPT_DTYPE_F16)
-    return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, tiles, grid, s)
-                           : packed::launch<__half, 64>(p, num_kv_heads, tiles, grid, s);
-  return head_dim == 128 ? packed::launch<__nv_bfloat16, 128>(p, num_kv_heads, tiles, grid, s)
-                         : packed::launch<__nv_bfloat16, 64>(p, num_kv_heads, tiles, grid, s);
+    return head_dim == 128 ? packed::launch<__half, 128>(p, num_kv_heads, pl, s)
+                           : packed::launch<__half, 64>(p, num_kv_heads, pl, s);
+  return head_dim == 128 ? packed::launch<__nv_bfloat16, 128>(p, num_kv_heads, pl, s)
+                         : packed::launch<__nv_bfloat16, 64>(p, num_kv_heads, pl, s);
 }

@@ -244,6 +244,130 @@ def test_attention_lengths_out_of_range_stay_inside():
     assert torch.equal(out[:60], ref[:60])
 
 
+# Few rows with many keys: items are split along the keys and joined.
+def splits(lens, H, KVH, D, window=-1, causal=True, hint=None):
+    import capi
+
+    f = capi.lib().memopt_packed_attention_workspace_size
+    f.restype = capi.SZ
+    return f(capi.I(len(lens)), capi.I64(sum(lens)), capi.I(max(lens) if hint is None else hint), capi.I(H), capi.I(KVH),
+             capi.I(D), capi.I(max(0, window)), capi.I(int(causal)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,H,KVH,D", [
+    ([4000], 4, 1, 128), ([2049], 1, 1, 64), ([2411, 800, 95], 4, 4, 64), ([3, 0, 2300, 1, 129, 0, 640], 2, 2, 128),
+    ([1900] + [1] * 40, 4, 2, 64), ([3177, 176], 5, 1, 64), ([5000, 3], 2, 1, 128), ([3301], 8, 1, 64)], ids=str)
+def test_attention_split(lens, H, KVH, D, dtype):
+    assert splits(lens, H, KVH, D) > 0
+    check_attention(lens, H, KVH, D, dtype, fused=True, seed=31, tail=9)
+
+
+@pytest.mark.parametrize("lens,H,KVH,D,causal,window", [
+    ([1200], 4, 4, 128, False, -1), ([2500, 1, 300], 4, 1, 64, False, -1), ([1500], 2, 2, 128, False, 1300),
+    ([3000], 2, 1, 64, True, 2000), ([2600, 0, 77], 1, 1, 128, True, 1801), ([4100, 64], 2, 1, 128, True, 1665)], ids=str)
+def test_attention_split_windows_and_all_keys(lens, H, KVH, D, causal, window):
+    assert splits(lens, H, KVH, D, window, causal) > 0
+    check_attention(lens, H, KVH, D, torch.float16, causal, window, seed=32)
+
+
+@pytest.mark.parametrize("hint", [900, 2600, 6000, 2 ** 31 - 1])
+def test_attention_split_with_another_length_hint(hint):
+    """The hint and the true lengths give different pieces: more, fewer or empty ones."""
+    for lens in ([2600], [1300, 1300], [2, 2500, 98], [40] * 65):
+        check_attention(lens, 2, 1, 128, torch.float16, max_seqlen=hint, seed=33)
+
+
+def test_attention_split_non_finite():
+    lens, H, KVH, D = [2500, 300], 2, 2, 64
+    assert splits(lens, H, KVH, D) > 0
+    q, k, v = make_qkv(lens, H, KVH, D, torch.float16, seed=34, tail=33)
+    T = sum(lens)
+    ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, -1, True)
+    tol = attention_tol(ref, mag, v, 2500, torch.float16)
+    for value in (float("nan"), float("inf"), -float("inf")):
+        for which in (0, 1):
+            kk, vv = k.clone(), v.clone()
+            (kk, vv)[which][[1700, T - 1]], (kk, vv)[which][T:] = value, value
+            out = C().packed_attention(q, kk, vv, cu_of(lens), 2500)
+            sees = torch.zeros(T, dtype=torch.bool, device=DEV)
+            sees[1700:2500], sees[T - 1] = True, True
+            assert ((out[:T].double() - ref).abs() <= tol)[~sees].all()
+            if which == 1:
+                assert not torch.isfinite(out[:T][sees].float()).any()
+    # One dim of one value: the others keep their result.
+    vv = v.clone()
+    vv[1700, 0, 5] = float("nan")
+    out = C().packed_attention(q, k, vv, cu_of(lens), 2500)[:T]
+    hit = torch.zeros(T, H, D, dtype=torch.bool, device=DEV)
+    hit[1700:2500, 0, 5] = True
+    assert torch.isnan(out[hit].float()).all()
+    assert ((out.double() - ref).abs() <= tol)[~hit].all()
+
+
+def test_attention_split_rising_and_hidden_scores():
+    """Pieces whose maxima lie far apart, and rows that see nothing in a piece's masked part."""
+    n, D = 2500, 128
+    q = torch.zeros(n, 1, D, device=DEV, dtype=torch.float16)
+    k = torch.zeros_like(q)
+    q[:, 0, 0] = 8.0
+    k[:, 0, 0] = torch.linspace(-40.0, 40.0, n, device=DEV).half()
+    v = torch.randn(n, 1, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).half()
+    for order in (torch.arange(n, device=DEV), torch.arange(n - 1, -1, -1, device=DEV)):
+        for window in (-1, 1500):
+            assert splits([n], 1, 1, D, window) > 0
+            kk, vv = k[order].contiguous(), v[order].contiguous()
+            out = C().packed_attention(q, kk, vv, cu_of([n]), n, window)
+            ref, mag = attention_ref(q, kk, vv, [n], window, True)
+            assert ((out.double() - ref).abs() <= attention_tol(ref, mag, v, n, torch.float16)).all()
+
+
+def test_attention_split_same_bits_and_leaves_the_rest():
+    lens = [2222, 0, 5]
+    q, k, v = make_qkv(lens, 4, 2, 128, torch.bfloat16, fused=True, tail=60)
+    cu, out = cu_of(lens), torch.full((2287, 4, 128), 3.0, dtype=torch.bfloat16, device=DEV)
+    C().packed_attention(q, k, v, cu, 2222, -1, True, out)
+    assert (out[2227:] == 3.0).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    both = []
+    for _ in range(4):  # two streams at once, each with its own workspace
+        both.append(C().packed_attention(q, k, v, cu, 2222))
+        with torch.cuda.stream(side):
+            both.append(C().packed_attention(q, k, v, cu, 2222))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o[:2227], out[:2227]) for o in both)
+
+
+def test_attention_split_in_graphs_with_new_lengths():
+    q, k, v = make_qkv([2600], 2, 1, 128, torch.float16)
+    cu = cu_of([2600, 0, 0])
+    outs, graphs = [torch.zeros_like(q) for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    C().packed_attention(q, k, v, cu, 2600)  # warm-up
+    for out, graph in zip(outs, graphs):
+        with torch.cuda.graph(graph):
+            C().packed_attention(q, k, v, cu, 2600, -1, True, out)
+    for lens in ([2600, 0, 0], [0, 2599, 1], [700, 1000, 900], [1, 1, 1], [0, 0, 0]):
+        cu.copy_(cu_of(lens))
+        T = sum(lens)
+        ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, -1, True)
+        for out, graph in zip(outs, graphs):
+            out.zero_()
+            graph.replay()
+        for out in outs:
+            if T:
+                assert ((out[:T].double() - ref).abs() <= attention_tol(ref, mag, v, max(lens), torch.float16)).all()
+            assert (out[T:] == 0).all()
+
+
+def test_attention_split_lengths_out_of_range_stay_inside():
+    q, k, v = make_qkv([2600], 2, 2, 64, torch.float16)
+    for cu in ([0, 2000, 600, 5000], [-5, 2600, 0, 2600], [2600, 2600, 3, 2600], [0, 2 ** 31 - 1, -2 ** 31, 7]):
+        C().packed_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=DEV), 2600)
+    torch.cuda.synchronize()
+    check_attention([2600], 2, 2, 64, torch.float16)
+
+
 def test_attention_many_sequences():
     rng = random.Random(0)
     lens = [rng.choice([0, 1, 2, 3, 7, 20, 33]) for _ in range(1500)]

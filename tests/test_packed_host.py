@@ -20,9 +20,17 @@ def sections(*values):
     return (C.c_int32 * max(1, len(values)))(*values)
 
 
-def attention(q=SOME, k=SOME, v=SOME, cu=SOME, out=SOME, qs=512, dtype=0, seqs=1, tokens=8, H=4, KVH=2, D=128):
+def attention(q=SOME, k=SOME, v=SOME, cu=SOME, out=SOME, qs=512, dtype=0, seqs=1, tokens=8, H=4, KVH=2, D=128,
+              longest=8, ws=0, ws_bytes=0):
     return capi.lib().memopt_packed_attention(P(q), I64(qs), P(k), I64(256), P(v), I64(256), I(dtype), P(cu), I(seqs),
-                                              I64(tokens), I(8), I(H), I(KVH), I(D), I(0), I(1), P(out), P(0))
+                                              I64(tokens), I(longest), I(H), I(KVH), I(D), I(0), I(1), P(out), P(ws),
+                                              C.c_size_t(ws_bytes), P(0))
+
+
+def workspace_size(seqs=1, tokens=8, longest=8, H=4, KVH=2, D=128, window=0, causal=1):
+    f = capi.lib().memopt_packed_attention_workspace_size
+    f.restype = C.c_size_t
+    return f(I(seqs), I64(tokens), I(longest), I(H), I(KVH), I(D), I(window), I(causal))
 
 
 @pytest.mark.parametrize("change,status", [
@@ -34,6 +42,33 @@ def attention(q=SOME, k=SOME, v=SOME, cu=SOME, out=SOME, qs=512, dtype=0, seqs=1
 def test_packed_attention_refuses(change, status):
     assert attention(**change) == status
     assert capi.lib().memopt_last_error().decode().startswith("packed_attention:")
+
+
+def test_packed_attention_workspace():
+    """One long prompt of few heads is split along its keys: the workspace is asked for and checked."""
+    need = workspace_size(tokens=4000, longest=4000, H=4, KVH=1)
+    assert 0 < need <= 256 << 20
+    assert workspace_size(tokens=4000, longest=4000, H=64, KVH=64) == 0  # items enough
+    assert workspace_size(tokens=100, longest=100) == 0                  # too short
+    for bad in (dict(seqs=0), dict(tokens=0), dict(seqs=-1), dict(tokens=-5), dict(H=0), dict(KVH=0), dict(H=5),
+                dict(D=96)):
+        assert workspace_size(**{**dict(tokens=4000, longest=4000), **bad}) == 0
+    long = dict(tokens=4000, longest=4000, H=4, KVH=1)
+    assert attention(**long) == -6
+    assert attention(**long, ws=SOME, ws_bytes=need - 1) == -6
+    assert attention(**long, ws=0, ws_bytes=need) == -6
+    assert attention(**long, ws=SOME + 8, ws_bytes=need) == INVALID
+
+
+@pytest.mark.parametrize("H,KVH", [(1, 1), (4, 1), (32, 8), (5, 5), (128, 1)])
+def test_packed_attention_workspace_is_bounded(H, KVH):
+    for tokens in (1, 700, 5000, 131072, 2 ** 31 - 1):
+        for seqs in (1, 2, 33, 2 ** 20, 2 ** 31 - 1):
+            for longest in (0, 1, 5000, 2 ** 31 - 1):
+                for window in (0, 1, 4096, 2 ** 31 - 1):
+                    for causal in (0, 1):
+                        for D in (64, 128):
+                            assert workspace_size(seqs, tokens, longest, H, KVH, D, window, causal) <= 256 << 20
 
 
 def test_packed_attention_of_nothing():
