@@ -11,7 +11,9 @@
 // K and V tile and a short prompt still fills rows.  An item has two tiles of
 // consecutive tokens over the same key blocks of 128, one CTA to an SM; or one
 // tile, two CTAs to an SM, for short prompts and few items (measured at the rule
-// in memopt_packed_attention).
+// in plan_of).  Few rows with many keys make fewer or longer items than the SMs
+// need: items are then split along the keys, each piece writes its unscaled sum with
+// its rows' maxima and sums, and a second kernel joins them (join_pieces_kernel).
 //
 // The launch has a CTA per item at most, long items first.  A CTA that has done
 // its item takes over one that has not begun (cluster launch control), so the SMs
@@ -67,11 +69,16 @@ namespace packed {
 constexpr int kBN = 128;       // keys per block
 constexpr int kFirst = 6;       // of the 8 steps of 16 keys, those that P.V starts with
 constexpr int kAhead = 3;       // blocks before an item's last loads at which the next item is taken
-constexpr double kSplitGain = 6;    // key blocks that a split has to save on the longest walk
-constexpr double kItemBlocks = 4;   // what an item costs beside its walk, in key blocks
-constexpr int64_t kMaxWorkspace = int64_t(256) << 20;
+constexpr int kMaxGp = 16;      // query heads packed into a tile
+// Splitting along the keys.  Writing, launching and joining the pieces takes 6-14 us,
+// about 6 blocks' time, which the longest walk has to save: one prompt of 4000 tokens,
+// 4/1 heads 57 -> 33 us, 8192 of 4 heads 114 -> 87, 16384 of 2 heads 220 -> 150, 1200
+// of 4 heads not causal 25 -> 20; below that a split loses (2000 tokens of 16/4 heads,
+// 4 blocks: 35.2 -> 35.7, 1000 of 32/8 heads, 1 block: 22 -> 27).
+constexpr double kSplitGain = 6;
+constexpr double kItemBlocks = 4;  // what an item takes beside its walk, in key blocks
 constexpr int kMaxPieces = 16;
-constexpr int kMaxGp = 16;     // query heads packed into a tile
+constexpr int64_t kMaxWorkspace = int64_t(256) << 20;
 
 struct Params {
   const void *q, *k, *v;
@@ -811,7 +818,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       auto on_level = [&](int s, int L) { return reaches(nblocks(s), L); };
       // Up to 32 sequences, a sequence to a lane, are counted without a loop: few
       // sequences have many levels, and a CTA's first item may lie far down (one
-      // prompt of 4000 tokens, 16/4 heads 89 -> 66 us).
+      // prompt of 4000 tokens, 16/4 heads 89 -> 71 us).
       const int own_blocks = nblocks(lane);
       // Pieces of a token block on a level, at most (a shorter last block may have
       // fewer; what is too many is skipped).
@@ -1118,12 +1125,12 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   const int64_t tokens = 128 >> pl.gshift;
   auto most_items = [&](int tiles) { return (T / (tokens * tiles) + S) * pl.units; };
   // Two tiles an item halve the K/V traffic and pay where the walk over the keys is
-  // long and the items are many: 2 x 8192 tokens, 32 heads 1.05 against 1.11 ms with
-  // one tile, 8 x 2048 with 32/8 heads 265 against 281 us, 4 prompts up to 7696 with
-  // 4/1 heads 155 against 205.  One tile, two CTAs to an SM, hides an item's ends
-  // better and makes twice the items: 32 x 512 118 against 123 us, 64 x 32 tokens
-  // 16.0 against 21.1, one prompt of 1000 24 against 27, 8192 tokens of 4 heads 108
-  // against 117.
+  // long and the items are many: 2 x 8192 tokens, 32 heads 0.91 ms against 0.98 with
+  // one tile, 4 prompts up to 7696 with 4/1 heads 140 us against 162, 12 x 800 with
+  // 32/8 heads of 64 dims 82 against 92.  One tile, two CTAs to an SM, hides an item's
+  // ends better and makes twice the items: 32 x 512 tokens 128 against 132, 64 x 32
+  // 14.5 against 20.0, 12 x 800 with heads of 128 dims 98 against 106, one prompt of
+  // 1000 24 against 29.
   pl.tiles = T >= 768LL * S && most_items(2) >= 2 * sm_count() ? 2 : 1;
   // Few rows with long walks: the longest item would go on alone, so items are split
   // into pieces of `split` key blocks.  With the longest sequence as hinted and the
