@@ -27,19 +27,29 @@ void int32_inplace(const torch::Tensor& t, const char* who, const char* name, in
   TORCH_CHECK(t.is_contiguous(), who, ": ", name, " is updated in place and must be contiguous");
 }
 
-// Whether the bytes that two tensors span meet.
-bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
-  auto span = [](const torch::Tensor& t) {
+// The bytes that a tensor spans, and whether two such spans meet.
+struct Span {
+  const char *begin = nullptr, *end = nullptr;
+  explicit Span(const torch::Tensor& t) {
+    const auto sizes = t.sizes(), strides = t.strides();
     int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) {
-      if (t.size(d) == 0) return std::pair<const char*, const char*>{nullptr, nullptr};
-      last += (t.size(d) - 1) * t.stride(d);
+    for (size_t d = 0; d < sizes.size(); ++d) {
+      if (sizes[d] == 0) return;
+      last += (sizes[d] - 1) * strides[d];
     }
-    const char* p = static_cast<const char*>(t.data_ptr());
-    return std::pair<const char*, const char*>{p, p + (last + 1) * t.element_size()};
-  };
-  const auto x = span(a), y = span(b);
-  return x.first && y.first && x.first < y.second && y.first < x.second;
+    begin = static_cast<const char*>(t.data_ptr());
+    end = begin + (last + 1) * t.element_size();
+  }
+  bool meets(const Span& o) const { return begin && o.begin && begin < o.end && o.begin < end; }
+};
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) { return Span(a).meets(Span(b)); }
+
+// A contiguous tensor inside a buffer: several outputs behind one allocation.
+torch::Tensor part_of(const torch::Tensor& buf, int64_t at, at::IntArrayRef sizes) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
 }
 
 int to_int(int64_t v, const char* who, const char* name) {
@@ -94,6 +104,8 @@ PageTensors page_checks(const char* who, const torch::Tensor& block_tables, cons
   TORCH_CHECK(context_lens.size(0) == block_tables.size(0), who, ": context_lens length != block_tables rows");
   TORCH_CHECK(pool_state.size(0) == 4, who, ": pool_state must hold 4 values (head, count, status, ticket)");
   TORCH_CHECK(block_size > 0, who, ": block_size must be > 0");
+  TORCH_CHECK(!overlap(rows, block_tables) && !overlap(rows, context_lens), who,
+              ": rows must not overlap what the call updates");
   return {to_int(block_tables.size(0), who, "table rows"), to_int(block_tables.size(1), who, "table width"),
           to_int(free_pages.size(0), who, "number of pages"), to_int(rows.size(0), who, "batch")};
 }
@@ -118,14 +130,9 @@ std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tens
   const int64_t at_pos = up4(max_tokens), at_tables = at_pos + up4(max_tokens);
   const int64_t at_cu = at_tables + up4(static_cast<int64_t>(n.B) * n.MB), at_lens = at_cu + up4(n.B + 1);
   const auto buf = torch::empty({at_lens + n.B}, block_tables.options());
-  auto part = [&](int64_t at, at::IntArrayRef sizes) {
-    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
-    t.unsafeGetTensorImpl()->set_storage_offset(at);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    return t;
-  };
-  auto slots = part(0, {max_tokens}), positions = part(at_pos, {max_tokens});
-  auto tables = part(at_tables, {n.B, n.MB}), cu = part(at_cu, {n.B + 1}), lens = part(at_lens, {n.B});
+  auto slots = part_of(buf, 0, {max_tokens}), positions = part_of(buf, at_pos, {max_tokens});
+  auto tables = part_of(buf, at_tables, {n.B, n.MB}), cu = part_of(buf, at_cu, {n.B + 1});
+  auto lens = part_of(buf, at_lens, {n.B});
   check(memopt_reserve_slots(block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(), n.R, n.MB,
                              free_pages.data_ptr<int32_t>(), n.NB, pool_state.data_ptr<int32_t>(),
                              rows.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n.B, block_size, max_tokens,
@@ -199,14 +206,28 @@ std::vector<torch::Tensor> rotary(const char* who, torch::Tensor query, torch::T
       TORCH_CHECK(c->size(2) == KVH && c->size(3) == D, who, ": cache heads or head_dim do not match the keys");
     }
     TORCH_CHECK(key_cache->sizes() == value_cache->sizes(), who, ": key_cache and value_cache shapes differ");
+    const Span kc(*key_cache), vc(*value_cache), in[] = {Span(query), Span(keys), Span(*values)};
+    TORCH_CHECK(!kc.meets(vc), who, ": key_cache and value_cache overlap");
+    for (const Span& x : in)
+      TORCH_CHECK(!x.meets(kc) && !x.meets(vc), who, ": the caches must not overlap the inputs");
     NB = key_cache->size(0);
     BS = to_int(key_cache->size(1), who, "block_size");
     slots = slot_mapping->contiguous();
     v = packed_rows(*values);
   }
   const at::cuda::CUDAGuard g(query.device());
-  auto q_out = torch::empty(query.sizes(), query.options());
-  auto k_out = torch::empty(keys.sizes(), keys.options());
+  // Decode steps wait for the host: one allocation behind both outputs (32 tokens of
+  // 32/8 heads: 6.9 -> 6.2 us a call).  Larger ones stay apart, so that either can be
+  // freed without the other.
+  torch::Tensor q_out, k_out;
+  if (query.numel() + keys.numel() <= (1 << 19) && query.numel() % 8 == 0) {
+    const auto buf = torch::empty({query.numel() + keys.numel()}, query.options());
+    q_out = part_of(buf, 0, query.sizes());
+    k_out = part_of(buf, query.numel(), keys.sizes());
+  } else {
+    q_out = torch::empty(query.sizes(), query.options());
+    k_out = torch::empty(keys.sizes(), keys.options());
+  }
   if (T == 0 || H + KVH == 0) return {q_out, k_out};
   auto q = packed_rows(query), k = packed_rows(keys);
   positions = positions.contiguous();

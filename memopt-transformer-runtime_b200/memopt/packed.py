@@ -110,8 +110,11 @@ class DevicePageTable:
         """Gives back the first ``counts[i]`` pages of each row of ``pages``
         (the ``freed_pages`` and ``freed_count`` of an exact eviction; both
         are cleared)."""
-        n = torch.arange(pages.shape[0], dtype=torch.int32, device=self.device)
-        self._C.truncate_rows(pages, counts, self.free_pages, self.pool_state, n, None, 1)
+        n = torch.arange(min(pages.shape[0], 8192), dtype=torch.int32, device=self.device)
+        for at in range(0, pages.shape[0], 8192):  # the most rows of a call
+            some = slice(at, at + 8192)
+            part = counts[some]
+            self._C.truncate_rows(pages[some], part, self.free_pages, self.pool_state, n[:part.shape[0]], None, 1)
 
     def free_count(self) -> int:
         """Number of free pages (synchronises)."""

@@ -931,6 +931,45 @@ def test_overlapping_arguments_are_refused():
         t.reserve(rows, t.context_lens, 4)
 
 
+def test_caches_and_rows_that_overlap_are_refused():
+    q, k, v = make_qkv([16], 2, 2, 64, torch.float16)
+    kc, vc = torch.zeros(1, 16, 2, 64, device=DEV, dtype=torch.float16), torch.zeros(1, 16, 2, 64, device=DEV,
+                                                                                     dtype=torch.float16)
+    pos = torch.arange(16, device=DEV, dtype=torch.int32)
+    freq = torch.ones(32, device=DEV, dtype=torch.float64)
+    for caches, kk in (((kc, kc), k), ((kc, vc), kc.reshape(16, 2, 64)), ((kc, vc), vc.reshape(16, 2, 64))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            C().rotary_write_cache(q, kk, v, pos, freq, [32], pos, *caches)
+    tables = torch.full((4, 4), -1, device=DEV, dtype=torch.int32)
+    lens, ring = torch.zeros(4, device=DEV, dtype=torch.int32), torch.arange(8, device=DEV, dtype=torch.int32)
+    state = torch.tensor([0, 8, 0, 0], device=DEV, dtype=torch.int32)
+    for rows in (lens[:2], tables[1, :2]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            C().reserve_slots(tables, lens, ring, state, rows, torch.ones(2, device=DEV, dtype=torch.int32), 16, 2)
+        with pytest.raises(RuntimeError, match="overlap"):
+            C().truncate_rows(tables, lens, ring, state, rows, None, 16)
+
+
+def test_pages_of_more_rows_than_a_call_takes_come_back():
+    """An eviction frees pages for every row of the table, also of more than 8192 rows."""
+    from memopt import DevicePageTable
+
+    rows = 9000
+    t = DevicePageTable(rows * 2, 1, rows, 4)
+    for at in range(0, rows, 6000):
+        n = min(6000, rows - at)
+        t.reserve(range(at, at + n), [2] * n)
+    assert t.free_count() == 0
+    pages, counts = t.block_tables.clone(), torch.full((rows,), 2, device=DEV, dtype=torch.int32)
+    counts[5::7] = 1
+    given = int(counts.sum())
+    t.release_pages(pages, counts)
+    assert t.free_count() == given and int(counts.sum()) == 0
+    t.check()
+    want = torch.cat([t.block_tables[i, :2 - (i % 7 == 5)].cpu() for i in range(rows)])
+    assert torch.equal(t.free_pages[:given].cpu(), want)
+
+
 @pytest.mark.parametrize("strides", ["sliced", "odd", "expanded", "transposed"])
 def test_layouts_other_than_contiguous(strides):
     """Rows apart by any multiple of 8 elements are read in place, everything
