@@ -93,7 +93,8 @@ struct Params {
   float qscale;     // log2(e) / sqrt(D)
   // Split items: key blocks of a piece, most pieces of a tile, and for every tile,
   // head unit and piece the unscaled O [D/4][128 rows] float4 and the rows' (m, l).
-  int split, pieces;
+  // The first `whole` tiles of a sequence stay whole.
+  int split, pieces, whole;
   float4* part_o;
   float2* part_ml;
 };
@@ -162,15 +163,16 @@ __device__ __forceinline__ Range tile_range(const Params& p, const Item& it, int
   return {from / kBN, (c_last + kBN - 1) / kBN, c_last};
 }
 
-// Pieces that a range of key blocks is split into (the last one takes what is left).
-__device__ __forceinline__ int pieces_of(const Params& p, int blocks) {
-  return min(p.pieces, (blocks + p.split - 1) / p.split);
+// Pieces of a tile (its number in the sequence) that walks over some key blocks; the
+// last piece takes what is left.
+__device__ __forceinline__ int pieces_of(const Params& p, int tile, int blocks) {
+  return tile < p.whole ? 1 : min(p.pieces, (blocks + p.split - 1) / p.split);
 }
 // What an item does of its tile's range.
 template <int TILES, bool SPLIT>
 __device__ __forceinline__ Range item_range(const Params& p, const Item& it, int t) {
   Range r = tile_range<TILES>(p, it, t);
-  if (SPLIT && r.hi > 0) {
+  if (SPLIT && r.hi > 0 && it.t0 >= p.whole << (7 - p.gshift)) {
     const int lo = r.lo + it.piece * p.split;
     if (it.piece < p.pieces - 1) r.hi = min(r.hi, lo + p.split);
     r.lo = lo;
@@ -597,8 +599,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       if (ok) ok = __all_sync(0xffffffffu, wait_bar(at(bars.pv_done[t]), (blocks - 1) & 1));
       tc::fence_after_sync();
       if (SPLIT) {
-        const Range whole = tile_range<TILES>(p, it, t);
-        if (pieces_of(p, whole.hi - whole.lo) > 1) {
+        const Range all = tile_range<TILES>(p, it, t);
+        if (pieces_of(p, it.t0 >> (7 - p.gshift), all.hi - all.lo) > 1) {
           // One of several pieces: O as it is, and the row's maximum and sum.
           const int64_t at = static_cast<int64_t>(it.slot) * p.pieces + it.piece;
           float4* po = p.part_o + at * (D / 4) * 128 + row;
@@ -858,7 +860,13 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         if (!SPLIT) return 1;
         const int hi = ((p.causal ? L + 1 : L) * tokens + kBN - 1) / kBN;
         const int first = (p.causal ? L : L - 1) * tokens + 1;
-        return pieces_of(p, hi - (p.window > 0 && first > p.window ? (first - p.window) / kBN : 0));
+        return pieces_of(p, p.whole, hi - (p.window > 0 && first > p.window ? (first - p.window) / kBN : 0));
+      };
+      // Items of a sequence on a level: one tile's pieces, or (not causal) all L tiles,
+      // the first of them whole.
+      auto items_on = [&](int L) {
+        if (p.causal) return pieces_on(L);
+        return SPLIT ? min(L, p.whole) + max(L - p.whole, 0) * pieces_on(L) : L;
       };
       auto count_on = [&](int L) {  // token blocks (split: their pieces) on a level
         int n = 0;
@@ -869,7 +877,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           for (int s = lane; s < p.S; s += 32) n += on_level(s, L);
           n = __reduce_add_sync(0xffffffffu, n);
         }
-        return static_cast<uint32_t>(p.causal ? n : n * L) * pieces_on(L);
+        return static_cast<uint32_t>(n) * items_on(L);
       };
       auto next_level = [&](int L) {
         if (p.causal) return L - 1;
@@ -957,7 +965,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         const int at_level = static_cast<int>(b - above), pieces = pieces_on(L);
         // The sequence is the rank-th on the level.  Ranks grow from item to item:
         // the search goes on where the last one ended.
-        const int per_seq = p.causal ? pieces : L * pieces;
+        const int per_seq = items_on(L);
         const int rank = p.causal && !SPLIT ? at_level : at_level / per_seq;
         if (L != found_level || rank < found_before) {
           found_level = L;
@@ -974,12 +982,17 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
             bounds(s, lo, hi);
             found_s0 = s0;
             const int rest = at_level - rank * per_seq;
-            const int tile = p.causal ? L : SPLIT ? rest / pieces : rest;
+            int tile = p.causal ? L : rest, piece = p.causal ? rest : 0;
+            if (SPLIT && !p.causal && rest >= p.whole) {
+              const int of = (rest - p.whole) / pieces;
+              tile = p.whole + of;
+              piece = rest - p.whole - of * pieces;
+            }
             const int unit = static_cast<int>(chunk_first + in_chunk - b * chunk_units);
             it = Item{lo, hi - lo, tile * tokens, unit, 0, 0};
             if (SPLIT) {
-              it.piece = p.causal ? rest : rest % pieces;
-              it.slot = ((lo + it.t0) / tokens + s) * p.units + unit;
+              it.piece = piece;
+              it.slot = ((lo + it.t0) / tokens + s - p.whole) * p.units + unit;  // (a whole tile has none)
             }
             return true;
           }
@@ -1031,7 +1044,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Params p) {
   const int row = threadIdx.x, tokens = 128 >> p.gshift;
-  const int g = blockIdx.x / p.units, unit = blockIdx.x - g * p.units;
+  const int slot = blockIdx.x / p.units, unit = blockIdx.x - slot * p.units, g = slot + p.whole;
   after_previous();
   auto bounds = [&](int s, int& lo, int& hi) {
     lo = min(max(p.cu[s], 0), p.T);
@@ -1055,7 +1068,7 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant_
   Item it{lo, hi - lo, tile * tokens, unit, 0, 0};
   if (tile < 0 || static_cast<int64_t>(tile) * tokens >= it.n) return;
   const Range r = tile_range<1>(p, it, 0);
-  const int pieces = pieces_of(p, r.hi - r.lo);
+  const int pieces = pieces_of(p, tile, r.hi - r.lo);
   if (pieces <= 1) return;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * p.pieces;
   const float2* ml = p.part_ml + at * 128 + row;
@@ -1145,7 +1158,8 @@ int map_rows(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_
 struct Plan {
   int gshift, units, tiles;
   int split, pieces;       // 0: no item is split
-  int64_t tile_slots;      // tiles x head units that may exist
+  int whole;               // tiles of a sequence that stay whole (not causal)
+  int64_t tile_slots;      // tiles x head units that may be split
   int64_t grid, workspace;
 };
 Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window, bool causal) {
@@ -1179,29 +1193,44 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   const int64_t walk = walk_of(longest);
   const double tiles = static_cast<double>(tiles_of(longest) + (S - 1) * tiles_of(others)) * pl.units;
   const double blocks = 0.5 * (tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) * pl.units;
-  pl.tile_slots = most_items(1);
-  double best = walk - kSplitGain;
+  // Not causal, a little more than one item for every slot: the first `whole` tiles of
+  // a sequence fill the slots once, and the rest are split into another round; left
+  // whole they would take as long again (0.65 of it where they have the SM to
+  // themselves): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
+  // 290 -> 182.  Tiles of shorter sequences count by their walks.
+  const double even = static_cast<double>(tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) *
+                      pl.units / walk;
+  const bool spill = !causal && pl.tiles == 1 && even > slots;
+  const double rest = spill ? even - slots : tiles;  // tiles that may be split
+  const double first = spill ? walk + kItemBlocks : 0;
+  const double alone = spill ? (walk + kItemBlocks) * (rest <= slots / 2 ? 0.65 : 1.0) : walk;
+  double best = first + alone - kSplitGain;
   for (int rounds = 1; rounds <= 3; ++rounds) {
     double split;
     if (causal && window <= 0) {
       if (rounds * slots <= 0.5 * tiles) continue;
       split = std::ceil(blocks / (rounds * slots - 0.5 * tiles));
     } else {
-      if (rounds * slots < tiles) continue;
-      split = std::ceil(walk / std::floor(rounds * slots / tiles));
+      if (rounds * slots < rest) continue;
+      split = std::ceil(walk / std::floor(rounds * slots / rest));
     }
     split = std::max(3.0, split);
-    const double time = rounds * (split + kItemBlocks) - kItemBlocks;
+    const double time = first + rounds * (split + kItemBlocks) - (spill ? 0 : kItemBlocks);
     const int64_t pieces = std::min<int64_t>(kMaxPieces, static_cast<int64_t>((walk + split - 1) / split));
-    const int64_t bytes = pl.tile_slots * pieces * 128 * (D * 4 + 8);
+    const int whole = spill ? static_cast<int>(tiles_of(longest) * slots / even) : 0;
+    const int64_t tile_slots = (T / tokens + S - whole) * pl.units, bytes = tile_slots * pieces * 128 * (D * 4 + 8);
     if (time >= best || pieces < 2 || bytes > kMaxWorkspace) continue;
     best = time;
     pl.split = static_cast<int>(split);
     pl.pieces = static_cast<int>(pieces);
+    pl.whole = whole;
+    pl.tile_slots = tile_slots;
     pl.workspace = bytes;
   }
   if (pl.split) pl.tiles = 1;
-  pl.grid = most_items(pl.tiles) * std::max(1, pl.pieces);
+  // Every tile, and the further pieces of those that are split.
+  pl.grid = most_items(pl.tiles);
+  if (pl.split) pl.grid += pl.tile_slots * (pl.pieces - 1);
   return pl;
 }
 
@@ -1281,7 +1310,7 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
                                           " bytes)");
   if (pl.split && !packed::aligned16(workspace))
     return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: workspace must be 16-byte aligned");
-  p.gshift = pl.gshift, p.units = pl.units, p.split = pl.split, p.pieces = pl.pieces;
+  p.gshift = pl.gshift, p.units = pl.units, p.split = pl.split, p.pieces = pl.pieces, p.whole = pl.whole;
   p.part_o = static_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + pl.tile_slots * pl.pieces * (head_dim / 4) * 128);
   p.window = window_size > 0 ? window_size : 0, p.causal = causal ? 1 : 0;
