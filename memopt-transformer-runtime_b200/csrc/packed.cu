@@ -1193,31 +1193,36 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   const int64_t walk = walk_of(longest);
   const double tiles = static_cast<double>(tiles_of(longest) + (S - 1) * tiles_of(others)) * pl.units;
   const double blocks = 0.5 * (tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) * pl.units;
-  // Not causal, a little more than one item for every slot: the first `whole` tiles of
-  // a sequence fill the slots once, and the rest are split into another round; left
-  // whole they would take as long again (0.65 of it where they have the SM to
-  // themselves): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
-  // 290 -> 182.  Tiles of shorter sequences count by their walks.
+  // Not causal, a little more than a whole number of items for every slot: the first
+  // `whole` tiles of a sequence fill the slots, and the rest are split into another
+  // round; left whole they would take as long again (0.65 of it where they have the SM
+  // to themselves): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
+  // 290 -> 182, 8192 of 10 heads 384 -> 314.  Items of two tiles take 0.85 of the time of two items.  Tiles of
+  // shorter sequences count by their walks.
   const double even = static_cast<double>(tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) *
                       pl.units / walk;
-  const bool spill = !causal && pl.tiles == 1 && even > slots;
-  const double rest = spill ? even - slots : tiles;  // tiles that may be split
-  const double first = spill ? walk + kItemBlocks : 0;
-  const double alone = spill ? (walk + kItemBlocks) * (rest <= slots / 2 ? 0.65 : 1.0) : walk;
-  double best = first + alone - kSplitGain;
+  const double filled = causal ? 0 : std::floor(even / slots);
+  const bool spill = filled > 0;
+  const double rest = spill ? even - filled * slots : tiles;  // tiles that may be split
+  const double first = filled * (walk + kItemBlocks);
+  double best = walk;
+  if (spill && rest > 0)
+    best = pl.tiles == 2 ? std::ceil(even / slots) * (0.85 * walk + kItemBlocks)
+                         : first + (walk + kItemBlocks) * (rest <= slots / 2 ? 0.65 : 1.0);
+  best -= kSplitGain;
   for (int rounds = 1; rounds <= 3; ++rounds) {
     double split;
     if (causal && window <= 0) {
       if (rounds * slots <= 0.5 * tiles) continue;
       split = std::ceil(blocks / (rounds * slots - 0.5 * tiles));
     } else {
-      if (rounds * slots < rest) continue;
+      if (rounds * slots < rest || rest <= 0) continue;
       split = std::ceil(walk / std::floor(rounds * slots / rest));
     }
     split = std::max(3.0, split);
     const double time = first + rounds * (split + kItemBlocks) - (spill ? 0 : kItemBlocks);
     const int64_t pieces = std::min<int64_t>(kMaxPieces, static_cast<int64_t>((walk + split - 1) / split));
-    const int whole = spill ? static_cast<int>(tiles_of(longest) * slots / even) : 0;
+    const int whole = spill ? static_cast<int>(tiles_of(longest) * filled * slots / even) : 0;
     const int64_t tile_slots = (T / tokens + S - whole) * pl.units, bytes = tile_slots * pieces * 128 * (D * 4 + 8);
     if (time >= best || pieces < 2 || bytes > kMaxWorkspace) continue;
     best = time;

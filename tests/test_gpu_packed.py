@@ -274,9 +274,9 @@ def test_attention_split_windows_and_all_keys(lens, H, KVH, D, causal, window):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("lens,H,KVH,D,window", [
     ([2500, 5, 7, 0, 20, 1], 16, 4, 128, -1), ([5000], 8, 4, 64, -1), ([2700], 16, 4, 128, 2300),
-    ([2600, 2599], 8, 4, 64, -1)], ids=str)
+    ([2600, 2599], 8, 4, 64, -1), ([2500], 32, 8, 64, -1)], ids=str)
 def test_attention_tiles_past_a_round_are_split(lens, H, KVH, D, window, dtype):
-    """Not causal, a little more than one item for every slot: the last tiles are split, the others whole."""
+    """Not causal, a little more than one or two items for every slot: the last tiles are split, the others whole."""
     assert splits(lens, H, KVH, D, window, False) > 0
     check_attention(lens, H, KVH, D, dtype, False, window, seed=35, tail=7)
     shorter = [max(0, n - 700) for n in lens] + [700 * sum(n > 700 for n in lens)]
