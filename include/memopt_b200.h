@@ -454,7 +454,8 @@ int memopt_rotary_write_cache(const void* query, int64_t query_stride, const voi
 /* to choose launch shapes.  head_dim 64 or 128.  Few rows with many keys are */
 /* split along the keys and joined: the workspace (16-byte aligned, no initial */
 /* values; memopt_packed_attention_workspace_size bytes for the same arguments, */
-/* 0 for most calls) holds the partial results.                               */
+/* 0 for most calls) holds the partial results; calls that may run at once    */
+/* need one each.                                                             */
 size_t memopt_packed_attention_workspace_size(int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads,
                                               int num_kv_heads, int head_dim, int window_size, int causal);
 int memopt_packed_attention(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
