@@ -76,7 +76,9 @@ constexpr int kMaxGp = 16;      // query heads packed into a tile
 // of 4 heads not causal 25 -> 20; below that a split loses (2000 tokens of 16/4 heads,
 // 4 blocks: 35.2 -> 35.7, 1000 of 32/8 heads, 1 block: 22 -> 27).
 constexpr double kSplitGain = 6;
-constexpr double kItemBlocks = 4;  // what an item takes beside its walk, in key blocks
+// What an item takes beside its walk, in key blocks: its ends 1.3 (one tile; 2 with
+// two tiles), the rest a CTA's start and the wait for its first loads.
+constexpr double kItemBlocks = 4;
 constexpr int kMaxPieces = 16;
 constexpr int64_t kMaxWorkspace = int64_t(256) << 20;
 
@@ -1199,8 +1201,9 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   // Not causal, a little more than a whole number of items for every slot: the first
   // `whole` tiles of a sequence fill the slots, and the rest are split into another
   // round; left whole they would take as long again (0.65 of it where they have the SM
-  // to themselves): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
-  // 290 -> 182, 8192 of 10 heads 384 -> 314.  Items of two tiles take 0.85 of the time of two items.  Tiles of
+  // to themselves: 1.5 against 2.3 us a block of 128 dims): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
+  // 290 -> 182, 8192 of 10 heads 384 -> 314.  Items of two tiles take 0.85 of the time of two items
+  // (1.95 against 2.29 us a block).  Tiles of
   // shorter sequences count by their walks.
   const double even = static_cast<double>(tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) *
                       pl.units / walk;
