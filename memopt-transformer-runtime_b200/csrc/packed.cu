@@ -1201,10 +1201,10 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   // Not causal, a little more than a whole number of items for every slot: the first
   // `whole` tiles of a sequence fill the slots, and the rest are split into another
   // round; left whole they would take as long again (0.65 of it where they have the SM
-  // to themselves: 1.5 against 2.3 us a block of 128 dims): one prompt of 2500 tokens, 16/4 heads 79 -> 59 us, 10000 of 4 heads
-  // 290 -> 182, 8192 of 10 heads 384 -> 314.  Items of two tiles take 0.85 of the time of two items
-  // (1.95 against 2.29 us a block).  Tiles of
-  // shorter sequences count by their walks.
+  // to themselves: 1.5 against 2.3 us a block of 128 dims).  One prompt of 2500 tokens,
+  // 16/4 heads 79 -> 59 us, 10000 of 4 heads 290 -> 182, 8192 of 10 heads 384 -> 314.
+  // Items of two tiles take 0.85 of the time of two items (1.95 against 2.29 us a
+  // block).  Tiles of shorter sequences count by their walks.
   const double even = static_cast<double>(tiles_of(longest) * walk + (S - 1) * tiles_of(others) * walk_of(others)) *
                       pl.units / walk;
   const double filled = causal ? 0 : std::floor(even / slots);
