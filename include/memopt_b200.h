@@ -66,6 +66,9 @@ int memopt_pool_init(int num_blocks, int block_size, int num_heads, int head_dim
 /* Drop the pool: afterwards every pool call reports NOT_INITIALIZED. */
 void memopt_pool_reset(void);
 int memopt_pool_is_initialized(void);
+/* A number that changes whenever the free-list begins anew or is dropped:
+ * pages popped under another generation belong to a pool that is gone. */
+int64_t memopt_pool_generation(void);
 /* Writes the live geometry; NOT_INITIALIZED when there is no pool. */
 int memopt_pool_config(int* num_blocks, int* block_size, int* num_heads, int* head_dim);
 /* Pops the oldest free block: >=0 on success, -1 when exhausted,

@@ -19,6 +19,7 @@ struct PoolState {
   std::mutex mu;
   bool initialized = false;
   int num_blocks = 0, block_size = 0, num_heads = 0, head_dim = 0;
+  int64_t generation = 0;  // free-lists begun or dropped so far
   std::deque<int> free_list;
 };
 PoolState& pool() {
@@ -87,6 +88,7 @@ int memopt_pool_init(int num_blocks, int block_size, int num_heads, int head_dim
     return MEMOPT_OK;
   // Any failed re-initialisation leaves the pool uninitialised, so a later
   // write cannot silently land in the previous pool's geometry.
+  ++p.generation;
   p.initialized = false;
   p.free_list.clear();
   if (num_blocks <= 0) return memopt::fail(MEMOPT_ERR_INVALID_ARG, "init_pool: num_blocks must be > 0");
@@ -107,6 +109,7 @@ int memopt_pool_init(int num_blocks, int block_size, int num_heads, int head_dim
 void memopt_pool_reset(void) {
   auto& p = pool();
   std::lock_guard<std::mutex> lk(p.mu);
+  ++p.generation;
   p.initialized = false;
   p.free_list.clear();
   p.num_blocks = p.block_size = p.num_heads = p.head_dim = 0;
@@ -116,6 +119,12 @@ int memopt_pool_is_initialized(void) {
   auto& p = pool();
   std::lock_guard<std::mutex> lk(p.mu);
   return p.initialized ? 1 : 0;
+}
+
+int64_t memopt_pool_generation(void) {
+  auto& p = pool();
+  std::lock_guard<std::mutex> lk(p.mu);
+  return p.generation;
 }
 
 int memopt_pool_config(int* num_blocks, int* block_size, int* num_heads, int* head_dim) {

@@ -91,6 +91,8 @@ void free_block(int block_idx) { check(memopt_pool_free_block(block_idx), "free_
 
 int free_blocks_count() { return memopt_pool_free_blocks_count(); }
 
+int64_t pool_generation() { return memopt_pool_generation(); }
+
 namespace {
 // Strided views of the four regions of every INT4 page in stored order (the
 // layout is documented at memopt_write_cache_int4 in memopt_b200.h).
@@ -599,6 +601,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("get_int4_pages", &get_int4_pages, "Return the int4 page tensor [num_blocks, num_heads, page_bytes]");
   m.def("pool_format", &pool_format, "'fp16' or 'int4'");
   m.def("free_blocks_count", &free_blocks_count, "Return the number of free blocks remaining in the pool");
+  m.def("pool_generation", &pool_generation, "A number that changes whenever the pool is initialised anew or dropped");
   m.def("write_cache", &write_cache, "Scatter key/value tokens into the paged KV cache pool via slot_mapping",
         py::arg("keys"), py::arg("values"), py::arg("block_tables"), py::arg("slot_mapping"));
   m.def("evict_cache", &evict_cache, "Zero evicted token slots in the pool based on attention score ranking",

@@ -14,15 +14,19 @@ and everything that depends on the lengths is built on the GPU:
   refused calls.
 * :class:`RotaryPositions` — rotary positions with 1 to 4 axes (time, height,
   width), applied to q and k and fused with the write into an fp16 pool.
-* :class:`PackedKVCache` — the process-wide pool behind both: ``admit`` /
-  ``prompt`` run a batch of whole prompts (causal attention over the packed
-  tokens), ``extend`` / ``decode`` the steps after them (paged attention).
+* :class:`PackedKVCache` — pages of the process-wide pool behind both:
+  ``admit`` / ``prompt`` run a batch of whole prompts (causal attention over
+  the packed tokens), ``extend`` / ``decode`` the steps after them (paged
+  attention).
 
 These operators serve; they carry no gradient and refuse inputs that ask for
 one.
 """
 from __future__ import annotations
 
+import contextlib
+import gc
+import weakref
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple, Union
 
@@ -55,12 +59,17 @@ class PackedBatch:
 
 
 class DevicePageTable:
-    """Block tables and free pages in device memory, one sequence per row."""
+    """Block tables and free pages in device memory, one sequence per row.
+    ``pages``: those of the pool's ``num_blocks`` pages that the table may
+    hand out, in this order (all of them by default)."""
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_len: int,
-                 device: Optional[torch.device] = None) -> None:
+                 device: Optional[torch.device] = None, pages: Optional[Sequence[int]] = None) -> None:
         if min(num_blocks, block_size, max_seqs, max_seq_len) <= 0:
             raise ValueError("DevicePageTable: num_blocks, block_size, max_seqs and max_seq_len must be > 0")
+        ring = list(range(num_blocks)) if pages is None else list(pages)
+        if len(set(ring)) != len(ring) or any(not 0 <= p < num_blocks for p in ring):
+            raise ValueError("DevicePageTable: pages must be distinct pages of the pool")
         import memopt_C
 
         self._C = memopt_C
@@ -74,8 +83,8 @@ class DevicePageTable:
 
         self.block_tables = int32(-1, max_seqs, width)
         self.context_lens = int32(0, max_seqs)
-        self.free_pages = torch.arange(num_blocks, dtype=torch.int32, device=self.device)
-        self.pool_state = torch.tensor([0, num_blocks, 0, 0], dtype=torch.int32, device=self.device)
+        self.free_pages = torch.tensor(ring + [-1] * (num_blocks - len(ring)), dtype=torch.int32, device=self.device)
+        self.pool_state = torch.tensor([0, len(ring), 0, 0], dtype=torch.int32, device=self.device)
 
     def ints(self, values: Ints) -> torch.Tensor:
         """Whole numbers as an int32 tensor on the table's device."""
@@ -176,8 +185,57 @@ class RotaryPositions:
         return q2, k2
 
 
+_caches: "weakref.WeakSet[PackedKVCache]" = weakref.WeakSet()
+
+
+def _pool_kind(C) -> Optional[tuple]:
+    """(block_size, heads, head_dim, format, device) and the number of pages of
+    the process-wide pool, None where there is none."""
+    try:
+        fmt = C.pool_format()
+    except RuntimeError:
+        return None
+    k = C.get_pool_tensors()[0]
+    if fmt == "int4":  # codes [NB, H, BS, D / 2]
+        return (k.shape[2], k.shape[1], 2 * k.shape[3], fmt, k.device), k.shape[0]
+    return (k.shape[1], k.shape[2], k.shape[3], fmt, k.device), k.shape[0]
+
+
+def _take_pages(C, num_blocks: int, kind: tuple) -> Tuple[List[int], int]:
+    """``num_blocks`` pages off the free-list of a pool of this kind, and the
+    pool's number of pages.  A pool that has them free is used as it is;
+    otherwise the pool is initialised, unless a cache still lives in it."""
+    pool = _pool_kind(C)
+    if pool is None or pool[0] != kind or C.free_blocks_count() < num_blocks:
+        if any(c._owns() for c in _caches):
+            gc.collect()  # one that only a reference cycle keeps does not count
+        if any(c._owns() for c in _caches):
+            raise RuntimeError("PackedKVCache: the process-wide pool belongs to another PackedKVCache and has not "
+                               f"{num_blocks} free pages of this kind; call memopt_C.init_pool with the pages of all "
+                               "caches before the first one is made, or close the other one")
+        C.init_pool(num_blocks, *kind[:3], kv_format=kind[3])
+        if C.free_blocks_count() < num_blocks:
+            raise RuntimeError(f"PackedKVCache: the pool has {C.free_blocks_count()} free pages, {num_blocks} are asked "
+                               "for; the others are held through allocate_block")
+    return [C.allocate_block() for _ in range(num_blocks)], _pool_kind(C)[1]
+
+
+def _give_back(C, generation: int, pages: List[int]) -> None:
+    if C.pool_generation() == generation:
+        for page in pages:
+            C.free_block(page)
+
+
 class PackedKVCache:
-    """Packed-batch KV cache of one attention layer over the process-wide pool."""
+    """Packed-batch KV cache of one attention layer.
+
+    It takes ``num_blocks`` pages from the free-list of the process-wide pool,
+    as :class:`PagedKVCache` does page by page, and gives them back when it is
+    closed or dropped.  A pool of its kind (block size, heads, head_dim,
+    format) that has so many free pages is used as it is, otherwise it is
+    initialised with ``num_blocks`` pages: for several caches, one per layer,
+    call ``memopt_C.init_pool`` with the pages of all of them first.  While a
+    cache lives in the pool another one does not replace it."""
 
     def __init__(self, num_blocks: int, num_heads: int, head_dim: int, block_size: int = 16, max_seqs: int = 256,
                  max_seq_len: int = 32768, kv_format: str = "fp16", rotary: Optional[RotaryPositions] = None,
@@ -188,8 +246,30 @@ class PackedKVCache:
         if rotary is not None and rotary.head_dim != head_dim:
             raise ValueError("PackedKVCache: rotary.head_dim differs from head_dim")
         self.num_heads, self.head_dim, self.block_size, self.rotary = num_heads, head_dim, block_size, rotary
-        memopt_C.init_pool(num_blocks, block_size, num_heads, head_dim, kv_format=kv_format)
-        self.table = DevicePageTable(num_blocks, block_size, max_seqs, max_seq_len, device)
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():
+            pages, total = _take_pages(memopt_C, num_blocks, (block_size, num_heads, head_dim, kv_format, dev))
+        self._generation = memopt_C.pool_generation()
+        self._pages = weakref.finalize(self, _give_back, memopt_C, self._generation, pages)
+        self._pages.atexit = False
+        _caches.add(self)
+        self.table = DevicePageTable(total, block_size, max_seqs, max_seq_len, dev, pages)
+
+    def close(self) -> None:
+        """Gives the cache's pages back to the pool; the cache is then empty
+        and refuses further use."""
+        self._pages()
+
+    def _owns(self) -> bool:
+        return self._pages.alive and self._C.pool_generation() == self._generation
+
+    def _need_pool(self) -> None:
+        if not self._pages.alive:
+            raise RuntimeError("PackedKVCache: the cache was closed")
+        if self._C.pool_generation() != self._generation:
+            raise RuntimeError("PackedKVCache: the process-wide pool was initialised anew, the cache's pages are gone")
 
     @property
     def kv_format(self) -> str:
@@ -199,6 +279,7 @@ class PackedKVCache:
     def admit(self, rows: Ints, prompt_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
         """Starts a sequence in each row (what the row held is given back) and
         reserves its prompt."""
+        self._need_pool()
         r = self.table.ints(rows)
         self.table.truncate(r)
         batch = self.table.reserve(r, prompt_lens, max_tokens)
@@ -207,12 +288,14 @@ class PackedKVCache:
 
     def extend(self, rows: Ints, tokens_per_row: int = 1) -> PackedBatch:
         """Reserves the next ``tokens_per_row`` tokens of each row."""
+        self._need_pool()
         r = self.table.ints(rows)
         n = torch.full_like(r, tokens_per_row)
         return self.table.reserve(r, n, int(r.numel()) * tokens_per_row)
 
     def finish(self, rows: Ints) -> None:
         """Gives the pages of finished rows back."""
+        self._need_pool()
         self.table.truncate(rows)
 
     # ---- data path -------------------------------------------------------------
@@ -239,6 +322,7 @@ class PackedKVCache:
         past the batch's last token come back as they are in memory."""
         if not batch.whole:
             raise ValueError("PackedKVCache.prompt: the batch must come from admit (whole sequences)")
+        self._need_pool()
         q, k = self._store(q, k, v, batch, positions)
         return self._C.packed_attention(q, k, v, batch.cu_seqlens, max_seqlen, window_size, causal)
 
@@ -252,6 +336,7 @@ class PackedKVCache:
         B = batch.rows.numel()
         if B == 0 or q.shape[0] % B != 0:
             raise ValueError(f"PackedKVCache.decode: {q.shape[0]} tokens for {B} rows")
+        self._need_pool()
         q, _ = self._store(q, k, v, batch, positions)
         q4 = q.to(torch.float16).reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])
         reach = batch.block_tables.shape[1] * self.block_size
@@ -270,6 +355,7 @@ class PackedKVCache:
         [max_seqs, heads, L], L at least the longest row): kept tokens move to
         the front, lengths shrink, emptied pages return to the ring.  Returns
         (kept_idx, kept_count)."""
+        self._need_pool()
         t = self.table
         kept, count, freed, freed_count = self._C.evict_topk_compact(scores, t.block_tables, t.context_lens,
                                                                      float(retain_ratio), int(num_sink_tokens))

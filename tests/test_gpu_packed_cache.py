@@ -1,0 +1,141 @@
+"""The packed-batch cache as a program uses it: several caches in a process,
+positions after an eviction, refused batches, arguments of every kind."""
+from __future__ import annotations
+
+import ctypes
+import gc
+import math
+import threading
+
+import pytest
+import torch
+
+import capi
+from test_gpu_packed import DEV, attention_ref, attention_tol, cu_of, half_step, make_qkv, rotary_close, rotary_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def C():
+    import memopt_C
+
+    return memopt_C
+
+
+def tokens(n, H, KVH, D, seed=0, dtype=torch.float16):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(n, H + 2 * KVH, D, generator=g, device=DEV).to(dtype)
+    return tuple(t.contiguous() for t in x.split([H, KVH, KVH], 1))
+
+
+def cached(cache, row):
+    """This row's keys and values in the fp16 pool, [n, KVH, D]."""
+    n = int(cache.table.context_lens[row])
+    pages = cache.table.block_tables[row, : -(-n // cache.block_size)].long()
+    return [c[pages].reshape(-1, cache.num_heads, cache.head_dim)[:n].clone() for c in C().get_pool_tensors()]
+
+
+def paged_close(out, q, kk, vv, first):
+    """Rows of q are the tokens from `first` on of a sequence whose keys and
+    values are kk and vv: causal attention, to the paged kernels' tolerance."""
+    m, (n, H, D) = kk.shape[0], q.shape
+    full = torch.zeros(m, H, D, dtype=torch.float64, device=DEV)
+    full[first:first + n] = q.double()
+    ref, _ = attention_ref(full, kk.double(), vv.double(), [m], -1, True)
+    ref = ref[first:first + n]
+    return bool(((out.double() - ref).abs() <= 2e-3 + 1e-2 * ref.abs()).all())
+
+
+# ---- caches that share the process-wide pool ----------------------------------
+def test_two_caches_in_a_process_keep_apart():
+    """Two layers, each with its own cache over one pool: neither finds the
+    other's keys in its pages."""
+    from memopt import PackedKVCache
+
+    H, KVH, D, BS = 4, 2, 64, 16
+    gc.collect()
+    C().init_pool(60, BS, KVH, D)
+    caches = [PackedKVCache(30, KVH, D, BS, max_seqs=3, max_seq_len=320) for _ in range(2)]
+    lens = [40, 1, 100]
+    kept = [[], []]
+    for i, cache in enumerate(caches):
+        q, k, v = tokens(sum(lens), H, KVH, D, seed=i)
+        cache.prompt(q, k, v, cache.admit([0, 1, 2], lens), max(lens))
+        kept[i] += [list(x) for x in zip(k.split(lens), v.split(lens))]
+    for step in range(20):
+        for i, cache in enumerate(caches):
+            q, k, v = tokens(3, H, KVH, D, seed=100 + 2 * step + i)
+            out = cache.decode(q, k, v, cache.extend([0, 1, 2]))
+            for r in range(3):
+                kept[i][r] = [torch.cat([a, b[r:r + 1]]) for a, b in zip(kept[i][r], (k, v))]
+                kk, vv = kept[i][r]
+                assert paged_close(out[r:r + 1], q[r:r + 1], kk, vv, kk.shape[0] - 1)
+    for i, cache in enumerate(caches):
+        cache.table.check()
+        for r in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(cached(cache, r), kept[i][r]))
+    used = [set(c.table.block_tables[c.table.block_tables >= 0].tolist()) for c in caches]
+    assert not used[0] & used[1]
+
+
+def test_caches_take_their_pages_from_the_pool():
+    """A pool whose pages are taken is neither handed out again nor replaced
+    under the cache; a cache that is dropped or closed gives its pages back."""
+    from memopt import PackedKVCache, PagedKVCache
+
+    H, KVH, D, BS = 2, 2, 64, 16
+    gc.collect()
+    C().init_pool(21, BS, KVH, D)
+    first = PackedKVCache(21, KVH, D, BS, max_seqs=2, max_seq_len=160)
+    assert C().free_blocks_count() == 0
+    q, k, v = tokens(30, H, KVH, D)
+    first.prompt(q, k, v, first.admit([0], [30]), 30)
+    for args in ((21, KVH, D, BS), (1, KVH, D, BS), (40, KVH, D, BS), (21, 4, D, BS), (21, KVH, 128, BS)):
+        with pytest.raises(RuntimeError, match="another PackedKVCache"):
+            PackedKVCache(*args, max_seqs=2, max_seq_len=160)
+    with pytest.raises(RuntimeError, match="another PackedKVCache"):
+        PackedKVCache(21, KVH, D, BS, max_seqs=2, max_seq_len=160, kv_format="int4")
+    paged = PagedKVCache(21, KVH, D, BS)  # the free-list is the same one
+    with pytest.raises(MemoryError):
+        paged.table.reserve(paged.add_sequence(), 1)
+    kk, vv = cached(first, 0)
+    assert torch.equal(kk, k) and torch.equal(vv, v)
+    first.close()
+    assert C().free_blocks_count() == 21
+    with pytest.raises(RuntimeError, match="closed"):
+        first.extend([0])
+    second = PackedKVCache(10, KVH, D, BS, max_seqs=2, max_seq_len=160)  # a part of the pool
+    assert C().free_blocks_count() == 11 and second.table.free_count() == 10
+    del second, first
+    gc.collect()
+    assert C().free_blocks_count() == 21
+    # Pages that somebody holds are not the cache's.
+    held = [C().allocate_block() for _ in range(5)]
+    with pytest.raises(RuntimeError, match="free pages"):
+        PackedKVCache(21, KVH, D, BS, max_seqs=2, max_seq_len=160)
+    third = PackedKVCache(16, KVH, D, BS, max_seqs=2, max_seq_len=160)
+    assert not set(third.table.free_pages[:16].tolist()) & set(held)
+
+
+def test_a_pool_that_was_replaced_is_noticed():
+    from memopt import PackedKVCache
+
+    H, KVH, D, BS = 2, 2, 64, 16
+    gc.collect()
+    C().init_pool(23, BS, KVH, D)
+    cache = PackedKVCache(23, KVH, D, BS, max_seqs=2, max_seq_len=160)
+    q, k, v = tokens(30, H, KVH, D)
+    batch = cache.admit([0], [30])
+    cache.prompt(q, k, v, batch, 30)
+    step = cache.extend([0])
+    C().init_pool(24, BS, KVH, D)  # as another part of the program may
+    assert C().free_blocks_count() == 24
+    for call in (lambda: cache.admit([1], [3]), lambda: cache.extend([0]), lambda: cache.finish([0]),
+                 lambda: cache.prompt(q, k, v, batch, 30), lambda: cache.decode(q[:1], k[:1], v[:1], step),
+                 lambda: cache.evict(torch.rand(2, KVH, 160, device=DEV), 0.5)):
+        with pytest.raises(RuntimeError, match="initialised anew"):
+            call()
+    del cache, call
+    gc.collect()
+    assert C().free_blocks_count() == 24  # nothing is given back to a pool that it did not come from
+    assert not C().get_pool_tensors()[0].any()

@@ -1,0 +1,123 @@
+"""The packed-batch cache's bookkeeping and refusals that need no GPU."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import capi
+
+
+def test_pool_generation_changes_with_the_free_list():
+    lib = capi.lib()
+    lib.memopt_pool_generation.restype = ctypes.c_int64
+    now = lib.memopt_pool_generation
+    lib.memopt_pool_reset()
+    seen = [now()]
+    for init in ((6, 16, 2, 64), (7, 16, 2, 64), (0, 16, 2, 64), (6, 16, 2, 64)):
+        lib.memopt_pool_init(*init)
+        assert now() not in seen
+        seen.append(now())
+    assert lib.memopt_pool_init(6, 16, 2, 64) == 0 and lib.memopt_pool_allocate_block() == 0
+    assert lib.memopt_pool_free_block(0) == 0 and now() == seen[-1]  # the same free-list
+    lib.memopt_pool_reset()
+    assert now() not in seen
+
+
+class FakePool:
+    """memopt_C's pool as far as a cache's constructor uses it, on the CPU."""
+
+    def __init__(self):
+        self.kind, self.free, self.generation, self.inits = None, [], 0, 0
+
+    def init_pool(self, num_blocks, block_size, num_heads, head_dim, kv_format="fp16"):
+        kind = (num_blocks, block_size, num_heads, head_dim, kv_format)
+        if kind != self.kind:
+            self.kind, self.free = kind, list(range(num_blocks))
+            self.generation += 1
+
+    def pool_format(self):
+        if self.kind is None:
+            raise RuntimeError("pool not initialized")
+        return self.kind[4]
+
+    def get_pool_tensors(self):
+        nb, bs, h, d, fmt = self.kind
+        k = torch.empty((nb, h, bs, d // 2) if fmt == "int4" else (nb, bs, h, d))
+        return k, k
+
+    def pool_generation(self):
+        return self.generation
+
+    def free_blocks_count(self):
+        return len(self.free)
+
+    def allocate_block(self):
+        return self.free.pop(0) if self.free else -1
+
+    def free_block(self, page):
+        self.free.append(page)
+
+
+@pytest.fixture
+def pool(monkeypatch):
+    import sys
+
+    import memopt  # noqa: F401  its modules keep the real memopt_C
+
+    fake = FakePool()
+    monkeypatch.setitem(sys.modules, "memopt_C", fake)
+    return fake
+
+
+def cache_of(num_blocks, heads=2, kv_format="fp16"):
+    from memopt import PackedKVCache
+
+    return PackedKVCache(num_blocks, heads, 64, 16, max_seqs=2, max_seq_len=64, kv_format=kv_format, device="cpu")
+
+
+@pytest.mark.parametrize("kv_format", ["fp16", "int4"])
+def test_caches_share_a_pool_without_sharing_pages(pool, kv_format):
+    pool.init_pool(20, 16, 2, 64, kv_format)
+    a, b = cache_of(12, kv_format=kv_format), cache_of(8, kv_format=kv_format)
+    assert pool.generation == 1 and pool.free == []
+    rings = [c.table.free_pages[:c.table.free_count()].tolist() for c in (a, b)]
+    assert rings == [list(range(12)), list(range(12, 20))]
+    assert a.table.free_pages.numel() == 20  # a page is told from another by the pool's number of pages
+    for heads, fmt in ((2, kv_format), (4, kv_format), (2, "fp16" if kv_format == "int4" else "int4")):
+        with pytest.raises(RuntimeError, match="another PackedKVCache"):
+            cache_of(1, heads, fmt)
+    assert pool.generation == 1
+    a.close()
+    a.close()
+    assert pool.free == list(range(12))
+    with pytest.raises(RuntimeError, match="closed"):
+        a.finish([0])
+    del b
+    assert pool.free == list(range(20))
+    c = cache_of(30, kv_format=kv_format)  # nobody lives in the pool: a larger one
+    assert pool.generation == 2 and c.table.free_count() == 30
+
+
+def test_a_cache_notices_that_its_pool_is_gone(pool):
+    a = cache_of(5)
+    pool.init_pool(6, 16, 2, 64)
+    for call in (lambda: a.admit([0], [1]), lambda: a.extend([0]), lambda: a.finish([0]), lambda: a.evict(None, 0.5)):
+        with pytest.raises(RuntimeError, match="initialised anew"):
+            call()
+    a.close()
+    assert pool.free == list(range(6))
+    pool.free = pool.free[2:]  # somebody holds two
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache_of(6)
+
+
+def test_table_pages_are_checked():
+    from memopt import DevicePageTable
+
+    table = DevicePageTable(9, 16, 2, 64, device="cpu", pages=[7, 3, 4])
+    assert table.free_pages.tolist() == [7, 3, 4] + [-1] * 6 and table.free_count() == 3
+    for bad in ([0, 0], [-1], [9]):
+        with pytest.raises(ValueError, match="pages"):
+            DevicePageTable(9, 16, 2, 64, device="cpu", pages=bad)
