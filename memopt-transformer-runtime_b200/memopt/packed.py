@@ -338,7 +338,7 @@ class PackedKVCache:
             raise ValueError(f"PackedKVCache.decode: {q.shape[0]} tokens for {B} rows")
         self._need_pool()
         q, _ = self._store(q, k, v, batch, positions)
-        q4 = q.to(torch.float16).reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])
+        q4 = q.to(torch.float16).contiguous().reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])
         reach = batch.block_tables.shape[1] * self.block_size
         window = reach if window_size <= 0 else window_size
         if self.kv_format == "int4":

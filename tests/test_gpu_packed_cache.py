@@ -139,3 +139,32 @@ def test_a_pool_that_was_replaced_is_noticed():
     gc.collect()
     assert C().free_blocks_count() == 24  # nothing is given back to a pool that it did not come from
     assert not C().get_pool_tensors()[0].any()
+
+
+# ---- arguments as they come out of a fused projection ----------------------------------
+@pytest.mark.parametrize("kv_format,D", [("fp16", 64), ("int4", 128)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_slices_of_a_projection(kv_format, D, dtype):
+    """q, k and v as parts of one tensor, without rotary positions: the same
+    results as from copies."""
+    from memopt import PackedKVCache
+
+    H, KVH = 4, 2
+    results = []
+    for copy in (False, True):
+        gc.collect()
+        cache = PackedKVCache(12, KVH, D, 16, max_seqs=2, max_seq_len=96, kv_format=kv_format)
+        g = torch.Generator(device=DEV).manual_seed(7)
+        outs = []
+        for n in (50, 2, 6):
+            parts = torch.randn(n, H + 2 * KVH, D, generator=g, device=DEV).to(dtype).split([H, KVH, KVH], 1)
+            if copy:
+                parts = [t.contiguous() for t in parts]
+            if n == 50:
+                outs.append(cache.prompt(*parts, cache.admit([0, 1], [30, 20]), 30))
+            else:
+                outs.append(cache.decode(*parts, cache.extend([0, 1], n // 2)))
+        cache.table.check()
+        results.append(outs)
+        cache.close()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
