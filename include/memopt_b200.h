@@ -400,7 +400,7 @@ int memopt_paged_attention_int4(const void* query, const uint8_t* kv_pages,
 /* most once).  New pages are taken from the ring in batch order, as          */
 /* memopt_pool_allocate_block would hand them out.  Writes cu_seqlens         */
 /* [batch + 1] (exclusive scan of new_lens), for each new token its slot      */
-/* (page * block_size + offset) and its position in the sequence              */
+/* (page * block_size + offset) and its position, its index in the row        */
 /* (slot_mapping and positions int32 [max_tokens], 16-byte aligned, -1 and 0  */
 /* past the last token), and the batch's own rows: batch_tables [batch,       */
 /* max_blocks_per_seq] (-1 behind a row's pages) and batch_lens [batch] with   */
@@ -412,6 +412,17 @@ int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_r
                          const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
                          int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
                          int32_t* batch_lens, void* stream);
+/* The same over rows that may have been evicted from: position_offsets int32  */
+/* [num_rows], 0 in a new state, holds how far a row's tokens lie behind their */
+/* positions in the sequence, which is what keys in the cache were turned by.  */
+/* positions are index + offset; an empty row's offset becomes 0.  Whoever     */
+/* takes n tokens out of the middle of a row (evict_topk_compact shrinks       */
+/* context_lens by them) adds n to its offset.                                 */
+int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* position_offsets, int num_rows,
+                        int max_blocks_per_seq, int32_t* free_pages, int num_blocks, int32_t* pool_state,
+                        const int32_t* rows, const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
+                        int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
+                        int32_t* batch_lens, void* stream);
 /* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none;    */
 /* keep_lens, like new_lens above, must not overlap context_lens);            */
 /* the pages behind them go to the ring's end in row and page order and their */

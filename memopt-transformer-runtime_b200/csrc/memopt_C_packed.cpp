@@ -112,15 +112,23 @@ PageTensors page_checks(const char* who, const torch::Tensor& block_tables, cons
 
 }  // namespace
 
-std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tensor context_lens,
-                                         torch::Tensor free_pages, torch::Tensor pool_state, torch::Tensor rows,
-                                         torch::Tensor new_lens, int block_size, int64_t max_tokens) {
-  const char* who = "reserve_slots";
+namespace {
+
+std::vector<torch::Tensor> reserve(const char* who, torch::Tensor block_tables, torch::Tensor context_lens,
+                                   const torch::Tensor* position_offsets, torch::Tensor free_pages,
+                                   torch::Tensor pool_state, torch::Tensor rows, torch::Tensor new_lens, int block_size,
+                                   int64_t max_tokens) {
   const PageTensors n = page_checks(who, block_tables, context_lens, free_pages, pool_state, rows, block_size);
   int32_cuda(new_lens, who, "new_lens", 1, block_tables.device());
   TORCH_CHECK(new_lens.size(0) == n.B, who, ": new_lens length != rows length");
   TORCH_CHECK(!overlap(new_lens, context_lens), who, ": new_lens must not overlap context_lens");
   TORCH_CHECK(max_tokens >= 0 && max_tokens <= 0x7fffffff, who, ": max_tokens out of range");
+  if (position_offsets) {
+    int32_inplace(*position_offsets, who, "position_offsets", 1, block_tables.device());
+    TORCH_CHECK(position_offsets->size(0) == n.R, who, ": position_offsets length != block_tables rows");
+    for (const auto* t : {&block_tables, &context_lens, &free_pages, &pool_state, &rows, &new_lens})
+      TORCH_CHECK(!overlap(*position_offsets, *t), who, ": position_offsets must not overlap the other tensors");
+  }
   rows = rows.contiguous();
   new_lens = new_lens.contiguous();
   const at::cuda::CUDAGuard g(block_tables.device());
@@ -133,13 +141,33 @@ std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tens
   auto slots = part_of(buf, 0, {max_tokens}), positions = part_of(buf, at_pos, {max_tokens});
   auto tables = part_of(buf, at_tables, {n.B, n.MB}), cu = part_of(buf, at_cu, {n.B + 1});
   auto lens = part_of(buf, at_lens, {n.B});
-  check(memopt_reserve_slots(block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(), n.R, n.MB,
-                             free_pages.data_ptr<int32_t>(), n.NB, pool_state.data_ptr<int32_t>(),
-                             rows.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n.B, block_size, max_tokens,
-                             cu.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
-                             tables.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), cur_stream()),
+  auto p = [](const torch::Tensor& t) { return t.data_ptr<int32_t>(); };
+  check(position_offsets
+            ? memopt_reserve_rows(p(block_tables), p(context_lens), p(*position_offsets), n.R, n.MB, p(free_pages),
+                                  n.NB, p(pool_state), p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu),
+                                  p(slots), p(positions), p(tables), p(lens), cur_stream())
+            : memopt_reserve_slots(p(block_tables), p(context_lens), n.R, n.MB, p(free_pages), n.NB, p(pool_state),
+                                   p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu), p(slots), p(positions),
+                                   p(tables), p(lens), cur_stream()),
         who);
   return {cu, slots, positions, tables, lens};
+}
+
+}  // namespace
+
+std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tensor context_lens,
+                                         torch::Tensor free_pages, torch::Tensor pool_state, torch::Tensor rows,
+                                         torch::Tensor new_lens, int block_size, int64_t max_tokens) {
+  return reserve("reserve_slots", block_tables, context_lens, nullptr, free_pages, pool_state, rows, new_lens,
+                 block_size, max_tokens);
+}
+
+std::vector<torch::Tensor> reserve_rows(torch::Tensor block_tables, torch::Tensor context_lens,
+                                        torch::Tensor position_offsets, torch::Tensor free_pages,
+                                        torch::Tensor pool_state, torch::Tensor rows, torch::Tensor new_lens,
+                                        int block_size, int64_t max_tokens) {
+  return reserve("reserve_rows", block_tables, context_lens, &position_offsets, free_pages, pool_state, rows, new_lens,
+                 block_size, max_tokens);
 }
 
 void truncate_rows(torch::Tensor block_tables, torch::Tensor context_lens, torch::Tensor free_pages,
@@ -312,6 +340,10 @@ void bind_packed(pybind11::module_& m) {
         "slot_mapping, positions, block tables and context lengths",
         py::arg("block_tables"), py::arg("context_lens"), py::arg("free_pages"), py::arg("pool_state"),
         py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"));
+  m.def("reserve_rows", &reserve_rows,
+        "reserve_slots over rows that may have been evicted from: positions are index + position_offsets[row]",
+        py::arg("block_tables"), py::arg("context_lens"), py::arg("position_offsets"), py::arg("free_pages"),
+        py::arg("pool_state"), py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"));
   m.def("truncate_rows", &truncate_rows,
         "Cut table row rows[b] to its first keep_lens[b] tokens (None: to nothing) and return the pages to the ring",
         py::arg("block_tables"), py::arg("context_lens"), py::arg("free_pages"), py::arg("pool_state"),

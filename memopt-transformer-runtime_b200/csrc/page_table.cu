@@ -10,8 +10,9 @@
 //             need_b = ceil((o_b + n_b) / BS) - ceil(o_b / BS), g = its
 //             exclusive scan; page i of row b is its table entry for
 //             i < ceil(o_b / BS), else ring[(head + g_b + i - ceil(o_b/BS)) mod NB];
-//             token cu_b + r has position p = o_b + r and slot
-//             page(p / BS) * BS + p mod BS.
+//             token cu_b + r has index p = o_b + r in its row, slot
+//             page(p / BS) * BS + p mod BS and position p + offset_b, the
+//             offset being what an eviction took out of the row before it.
 //   truncate: the pages past ceil(k_b / BS) go to the ring's tail in row and
 //             page order.
 //
@@ -46,6 +47,7 @@ struct PageArgs {
   int R, MB, NB, BS, B;
   int shift;  // log2(BS), or -1 where BS is no power of two
   int64_t max_tokens;
+  int32_t* offsets;    // [R]: a token's position less its index in the row (null: 0)
   int32_t* cu;         // [B + 1]
   int32_t* slots;      // [max_tokens]
   int32_t* positions;  // [max_tokens]
@@ -59,6 +61,7 @@ struct Batch {
   int32_t* old;   // [B] length before the call
   int32_t* cu;    // [B + 1] exclusive scan of the new tokens (truncate: unused)
   int32_t* page;  // [B + 1] exclusive scan of the pages taken (truncate: given back)
+  int32_t* off;   // [B] position offset (truncate: unused); an empty row begins at 0 again
   uint32_t* seen;  // bit per table row
 };
 
@@ -68,12 +71,13 @@ __device__ __forceinline__ Batch carve(uint8_t* smem, int B) {
   t.old = t.row + B;
   t.cu = t.old + B;
   t.page = t.cu + B + 1;
-  t.seen = reinterpret_cast<uint32_t*>(t.page + B + 1);
+  t.off = t.page + B + 1;
+  t.seen = reinterpret_cast<uint32_t*>(t.off + B);
   return t;
 }
 
 size_t batch_smem(int B, int R) {
-  return (static_cast<size_t>(4) * B + 2) * 4 + static_cast<size_t>((R + 31) / 32) * 4;
+  return (static_cast<size_t>(5) * B + 2) * 4 + static_cast<size_t>((R + 31) / 32) * 4;
 }
 
 __device__ __forceinline__ int over_bs(int x, const PageArgs& a) { return a.shift >= 0 ? x >> a.shift : x / a.BS; }
@@ -98,13 +102,14 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
     const int b = b0 + tid;
     int n = 0, p = 0;
     if (b < a.B) {
-      int row = a.rows[b], old = 0;
+      int row = a.rows[b], old = 0, off = 0;
       if (row < 0 || row >= a.R) {
         bits |= MEMOPT_PAGES_BAD_ROW;
         row = 0;
       } else {
         if (atomicOr(&t.seen[row >> 5], 1u << (row & 31)) & (1u << (row & 31))) bits |= MEMOPT_PAGES_BAD_ROW;
         old = a.lens[row];
+        if (kReserve && a.offsets) off = a.offsets[row];
         if (old < 0 || old > cap) {
           bits |= MEMOPT_PAGES_CORRUPT;
           old = 0;
@@ -126,6 +131,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
       }
       t.row[b] = row;
       t.old[b] = old;
+      t.off[b] = old > 0 ? off : 0;
     }
     // Block-wide exclusive scan of (n, p): within the warp, then over the warps.
     int64_t sn = n, sp = p;
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
           page = at < had ? a.tables[static_cast<int64_t>(t.row[b]) * a.MB + at] : ring_at(t.page[b] + at - had);
           page_at = at;
         }
-        pos[k] = p;
+        pos[k] = p + t.off[b];
         if (page >= 0 && page < a.NB) slot[k] = page * a.BS + (p - at * a.BS);
         else bits |= MEMOPT_PAGES_CORRUPT;
       }
@@ -297,7 +303,10 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
 
   if (arrive_last(a.state + 3)) {
     if (taken) {
-      for (int b = tid; b < a.B; b += kThreads) a.lens[t.row[b]] = t.old[b] + (t.cu[b + 1] - t.cu[b]);
+      for (int b = tid; b < a.B; b += kThreads) {
+        a.lens[t.row[b]] = t.old[b] + (t.cu[b + 1] - t.cu[b]);
+        if (a.offsets && t.old[b] == 0) a.offsets[t.row[b]] = 0;
+      }
     }
     if (tid == 0) {
       if (taken) {
@@ -402,6 +411,18 @@ int launch_pages(K small, K large, const char* what, const PageArgs& a, cudaStre
   return MEMOPT_OK;
 }
 
+int reserve(const char* who, PageArgs a, cudaStream_t s) {
+  const int st = check_pages(who, a);
+  if (st != MEMOPT_OK) return st;
+  if (!a.cu || (a.B > 0 && (!a.amount || !a.out_tables || !a.out_lens)) ||
+      (a.max_tokens > 0 && (!a.slots || !a.positions)))
+    return fail(MEMOPT_ERR_INVALID_ARG, std::string(who) + ": null pointer");
+  if ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15u)
+    return fail(MEMOPT_ERR_INVALID_ARG, std::string(who) + ": slot_mapping and positions must be 16-byte aligned");
+  a.shift = log2_of(a.BS);
+  return launch_pages(reserve_kernel<256>, reserve_kernel<1024>, "reserve_kernel launch", a, s);
+}
+
 }  // namespace
 }  // namespace memopt
 
@@ -413,23 +434,28 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
                                     int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
                                     int32_t* batch_tables, int32_t* batch_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, max_tokens, cu_seqlens, slot_mapping, positions, batch_tables, batch_lens};
-  const int st = check_pages("reserve_slots", a);
-  if (st != MEMOPT_OK) return st;
-  if (!cu_seqlens || (batch > 0 && (!new_lens || !batch_tables || !batch_lens)) ||
-      (max_tokens > 0 && (!slot_mapping || !positions)))
-    return fail(MEMOPT_ERR_INVALID_ARG, "reserve_slots: null pointer");
-  if ((reinterpret_cast<uintptr_t>(slot_mapping) | reinterpret_cast<uintptr_t>(positions)) & 15u)
-    return fail(MEMOPT_ERR_INVALID_ARG, "reserve_slots: slot_mapping and positions must be 16-byte aligned");
-  a.shift = log2_of(block_size);
-  return launch_pages(reserve_kernel<256>, reserve_kernel<1024>, "reserve_kernel launch", a, as_stream(stream));
+             num_blocks, block_size, batch, 0, max_tokens, nullptr, cu_seqlens, slot_mapping, positions, batch_tables,
+             batch_lens};
+  return reserve("reserve_slots", a, as_stream(stream));
+}
+
+extern "C" int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* position_offsets,
+                                   int num_rows, int max_blocks_per_seq, int32_t* free_pages, int num_blocks,
+                                   int32_t* pool_state, const int32_t* rows, const int32_t* new_lens, int batch,
+                                   int block_size, int64_t max_tokens, int32_t* cu_seqlens, int32_t* slot_mapping,
+                                   int32_t* positions, int32_t* batch_tables, int32_t* batch_lens, void* stream) {
+  PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
+             num_blocks, block_size, batch, 0, max_tokens, position_offsets, cu_seqlens, slot_mapping, positions,
+             batch_tables, batch_lens};
+  if (!position_offsets) return fail(MEMOPT_ERR_INVALID_ARG, "reserve_rows: null pointer");
+  return reserve("reserve_rows", a, as_stream(stream));
 }
 
 extern "C" int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens, int num_rows, int max_blocks_per_seq,
                                     int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
                                     const int32_t* keep_lens, int batch, int block_size, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, keep_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr};
+             num_blocks, block_size, batch, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   const int st = check_pages("truncate_rows", a);
   if (st != MEMOPT_OK) return st;
   if (batch == 0) return MEMOPT_OK;

@@ -52,7 +52,7 @@ class PackedBatch:
     rows: torch.Tensor          # [B] table rows
     cu_seqlens: torch.Tensor    # [B + 1] first packed token of each sequence
     slot_mapping: torch.Tensor  # [max_tokens] slot of each new token, -1 past the last
-    positions: torch.Tensor     # [max_tokens] position of each new token in its sequence
+    positions: torch.Tensor     # [max_tokens] position of each new token in its sequence, evicted tokens counted
     block_tables: torch.Tensor  # [B, max_blocks_per_seq]
     context_lens: torch.Tensor  # [B] lengths with the new tokens
     whole: bool = False         # the new tokens are the whole sequences
@@ -83,6 +83,7 @@ class DevicePageTable:
 
         self.block_tables = int32(-1, max_seqs, width)
         self.context_lens = int32(0, max_seqs)
+        self.position_offsets = int32(0, max_seqs)  # tokens that evictions took out of a row
         self.free_pages = torch.tensor(ring + [-1] * (num_blocks - len(ring)), dtype=torch.int32, device=self.device)
         self.pool_state = torch.tensor([0, len(ring), 0, 0], dtype=torch.int32, device=self.device)
 
@@ -103,9 +104,9 @@ class DevicePageTable:
                 raise ValueError("reserve: max_tokens is needed when new_lens is a tensor")
             max_tokens = sum(new_lens)
         r = self.ints(rows)
-        cu, slots, pos, tables, lens = self._C.reserve_slots(
-            self.block_tables, self.context_lens, self.free_pages, self.pool_state, r, self.ints(new_lens),
-            self.block_size, max_tokens)
+        cu, slots, pos, tables, lens = self._C.reserve_rows(
+            self.block_tables, self.context_lens, self.position_offsets, self.free_pages, self.pool_state, r,
+            self.ints(new_lens), self.block_size, max_tokens)
         return PackedBatch(r, cu, slots, pos, tables, lens)
 
     def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
@@ -353,11 +354,14 @@ class PackedKVCache:
     def evict(self, scores: torch.Tensor, retain_ratio: float, num_sink_tokens: int = 4):
         """``evict_topk_compact`` over every row of the table (scores fp32
         [max_seqs, heads, L], L at least the longest row): kept tokens move to
-        the front, lengths shrink, emptied pages return to the ring.  Returns
-        (kept_idx, kept_count)."""
+        the front, lengths shrink, emptied pages return to the ring.  Positions
+        go on from the sequence's own length: kept keys stay turned by those
+        that they were written with.  Returns (kept_idx, kept_count)."""
         self._need_pool()
         t = self.table
+        before = t.context_lens.clone()
         kept, count, freed, freed_count = self._C.evict_topk_compact(scores, t.block_tables, t.context_lens,
                                                                      float(retain_ratio), int(num_sink_tokens))
+        t.position_offsets += before - t.context_lens
         t.release_pages(freed, freed_count)
         return kept, count

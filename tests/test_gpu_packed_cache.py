@@ -168,3 +168,115 @@ def test_slices_of_a_projection(kv_format, D, dtype):
         results.append(outs)
         cache.close()
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+# ---- positions after an eviction ----------------------------------------------
+def evicted(cache, rows, scores, ratio):
+    kept, count = cache.evict(scores, ratio)
+    return [kept[r, : int(count[r])].tolist() for r in rows]
+
+
+@pytest.mark.parametrize("sections", [[32], [10, 14, 8]], ids=str)
+def test_rotary_positions_after_an_eviction(sections):
+    """Kept keys stay turned by the positions that they were written with, so
+    the tokens after an eviction go on from the sequence's true length."""
+    from memopt import PackedKVCache, RotaryPositions
+
+    H, KVH, D, BS = 4, 2, 64, 16
+    rot = RotaryPositions(D, sections=sections)
+    cache = PackedKVCache(90, KVH, D, BS, max_seqs=4, max_seq_len=320, rotary=rot)
+    lens = {2: 92, 0: 5, 1: 200}
+    rows, total = list(lens), sum(lens.values())
+    q, k, v = tokens(total, H, KVH, D, seed=1)
+    cache.prompt(q, k, v, cache.admit(rows, list(lens.values())), 200)
+    true = dict(lens)               # logical length of each row
+    at = {r: list(range(n)) for r, n in lens.items()}  # logical positions of the cached tokens
+    raw = dict(zip(rows, zip(k.split(list(lens.values())), v.split(list(lens.values())))))
+
+    def turned(x, pos):
+        p = torch.tensor(pos, device=DEV, dtype=torch.int32)
+        return rotary_ref(x, p.expand(len(sections), -1), rot.inv_freq, rot.sections, False)
+
+    def step(n, seed):
+        batch = cache.extend(rows, n)
+        q, k, v = tokens(n * len(rows), H, KVH, D, seed=seed)
+        out = cache.decode(q, k, v, batch)
+        for i, r in enumerate(rows):
+            some = slice(i * n, (i + 1) * n)
+            pos = list(range(true[r], true[r] + n))
+            assert batch.positions[some].tolist() == pos
+            raw[r] = tuple(torch.cat([a, b[some]]) for a, b in zip(raw[r], (k, v)))
+            at[r], true[r] = at[r] + pos, true[r] + n
+            kk, vv = cached(cache, r)
+            assert rotary_close(kk, *turned(raw[r][0], at[r])) and torch.equal(vv, raw[r][1])
+            assert paged_close(out[some], turned(q[some], pos)[0].half(), kk, vv, kk.shape[0] - n)
+
+    def cut(r, n):  # the last n cached tokens are rejected
+        raw[r] = tuple(x[: x.shape[0] - n] for x in raw[r])
+        at[r], true[r] = at[r][: len(at[r]) - n], true[r] - n
+
+    step(1, 2)
+    for round, ratio in enumerate((0.5, 0.7)):  # twice, so that offsets add up
+        g = torch.Generator(device=DEV).manual_seed(round)
+        for r, kept in zip(rows, evicted(cache, rows, torch.rand(4, KVH, 256, generator=g, device=DEV), ratio)):
+            assert len(kept) < len(at[r]) or len(at[r]) < 7
+            raw[r] = tuple(x[kept] for x in raw[r])
+            at[r] = [at[r][i] for i in kept]
+        for i in range(3):
+            step(1, 10 * round + i + 3)
+        step(5, 40 + round)
+        cache.table.truncate(rows, [len(at[r]) - 4 for r in rows])  # four of five drafts rejected
+        for r in rows:
+            cut(r, 4)
+        step(1, 50 + round)
+    # A row that begins anew begins at 0; the others keep their offsets.
+    cache.finish([2])
+    q, k, v = tokens(30, H, KVH, D, seed=60)
+    batch = cache.admit([2], [30])
+    assert batch.positions.tolist() == list(range(30))
+    cache.prompt(q, k, v, batch, 30)
+    true[2], at[2], raw[2] = 30, list(range(30)), (k, v)
+    step(2, 61)
+    batch = cache.admit([0], [3])  # without finish
+    assert batch.positions.tolist() == [0, 1, 2]
+    cache.table.check()
+
+
+def test_positions_after_an_eviction_in_a_graph():
+    """A captured step goes on from the true positions after evictions between its replays."""
+    from memopt import PackedKVCache
+
+    cache = PackedKVCache(40, 2, 64, 16, max_seqs=3, max_seq_len=160)
+    q, k, v = tokens(100, 2, 2, 64)
+    cache.prompt(q, k, v, cache.admit([0, 2], [60, 40]), 60)
+    rows = torch.tensor([2, 0], dtype=torch.int32, device=DEV)
+    cache.extend(rows)  # warm-up
+    true = [41, 61]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch = cache.extend(rows)
+    for ratio in (1.0, 0.5, 0.25):
+        if ratio < 1:
+            cache.evict(torch.rand(3, 2, 160, device=DEV), ratio)
+        for _ in range(3):
+            graph.replay()
+            assert batch.positions.tolist() == true
+            true = [t + 1 for t in true]
+    cache.table.check()
+
+
+def test_a_refused_batch_keeps_the_positions():
+    from memopt import PackedKVCache
+
+    cache = PackedKVCache(6, 2, 64, 16, max_seqs=2, max_seq_len=96)
+    q, k, v = tokens(64, 2, 2, 64)
+    cache.prompt(q, k, v, cache.admit([0], [64]), 64)
+    cache.evict(torch.rand(2, 2, 96, device=DEV), 0.5)  # 32 cached, the next token is the 65th
+    cache.extend([0], 90)
+    with pytest.raises((MemoryError, RuntimeError)):
+        cache.table.check()
+    cache.extend([0, 0])
+    with pytest.raises(RuntimeError, match="twice"):
+        cache.table.check()
+    assert cache.extend([0, 1], 2).positions.tolist() == [64, 65, 0, 1]
+    cache.table.check()

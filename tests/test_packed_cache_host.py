@@ -121,3 +121,24 @@ def test_table_pages_are_checked():
     for bad in ([0, 0], [-1], [9]):
         with pytest.raises(ValueError, match="pages"):
             DevicePageTable(9, 16, 2, 64, device="cpu", pages=bad)
+
+
+P, I, I64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+SOME = 0x1000  # a 16-byte aligned address that no call may touch
+
+
+def reserve_rows(tables=SOME, lens=SOME, off=SOME, R=4, MB=8, ring=SOME, NB=32, state=SOME, rows=SOME, new=SOME, B=2,
+                 BS=16, most=64, cu=SOME, slots=SOME, pos=SOME, bt=SOME, bl=SOME):
+    return capi.lib().memopt_reserve_rows(P(tables), P(lens), P(off), I(R), I(MB), P(ring), I(NB), P(state), P(rows),
+                                          P(new), I(B), I(BS), I64(most), P(cu), P(slots), P(pos), P(bt), P(bl), P(0))
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(tables=0), -1), (dict(lens=0), -1), (dict(off=0), -1), (dict(ring=0), -1), (dict(state=0), -1),
+    (dict(rows=0), -1), (dict(new=0), -1), (dict(cu=0), -1), (dict(slots=0), -1), (dict(pos=0), -1), (dict(bt=0), -1),
+    (dict(bl=0), -1), (dict(slots=SOME + 4), -1), (dict(pos=SOME + 8), -1), (dict(most=-1), -1), (dict(B=-1), -1),
+    (dict(R=0), -1), (dict(MB=0), -1), (dict(NB=0), -1), (dict(BS=0), -1), (dict(B=8193), -3),
+    (dict(R=2 ** 18 + 1), -3), (dict(NB=2 ** 27), -3), (dict(MB=2 ** 27), -3), (dict(most=2 ** 31), -3)])
+def test_reserve_rows_refuses(change, status):
+    assert reserve_rows(**change) == status
+    assert capi.lib().memopt_last_error().decode().startswith("reserve_rows:")
