@@ -902,8 +902,9 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
       bool ok = true, more = true;  // more: there may be CTAs that have not begun
       uint32_t i = blockIdx.x;
       uint32_t asked = 0;
-      // Takes the index of a CTA that has not begun (the launch has one per item at
-      // most); false when there is none left.
+      // Takes the index of a CTA that has not begun; false when there is none left.
+      // Nothing promises an order of the indexes, so each of them is looked up, also
+      // behind one that had no item.
       auto take_next = [&]() -> bool {
         if (lane == 0) {
           mbar_arrive_expect_tx(at(bars.next), 16);
@@ -918,9 +919,11 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         i = cta;
         return got;
       };
-      // The item of index i; false when there is none.
+      // The item of index i; false when there is none.  The items are those of the
+      // indexes below `end` (split: an upper bound that every miss lowers).
+      uint32_t end = SPLIT ? 0xffffffffu : total;
       auto find = [&](Item& it) -> bool {
-        if (!SPLIT && i >= total) return false;
+        if (i >= end) return false;
         if (SPLIT) {
           chunk_units = p.units;  // few items: all units at once
         } else if (chunk_units == 0 || i < chunk_first * blocks_all || i >= (chunk_first + chunk_units) * blocks_all) {
@@ -940,6 +943,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           L = next_level(L);
           if (SPLIT && (p.causal ? L < 0 : L <= 0)) {
             here = 0;
+            end = i;
             return false;
           }
           if (!SPLIT || !p.causal) {
@@ -1015,13 +1019,16 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         Item it{0, -1, 0, 0, 0, 0}, got = it;
         while (more) {
-          if (!find(got)) break;
-          const Range r = item_range<TILES, SPLIT>(p, got, 0);
-          if (!SPLIT || r.lo < r.hi) {
+          bool has = find(got);
+          if (SPLIT && has) {  // not a piece that this token block does not have
+            const Range r = item_range<TILES, SPLIT>(p, got, 0);
+            has = r.lo < r.hi;
+          }
+          if (has) {
             it = got;
             break;
           }
-          more = take_next();  // a piece that this token block does not have
+          more = take_next();
         }
         if (!ok) break;
         if (lane == 0) {
@@ -1029,10 +1036,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           mbar_arrive(at(bars.item_full[k & 1]));
         }
         __syncwarp();
-        if (it.n < 0) break;
+        if (it.n < 0) break;  // no CTA is left that has not begun
       }
-      // The CTAs past the last item never begin.
-      while (ok && more) more = take_next();
     }
   }
   tc::fence_before_sync();

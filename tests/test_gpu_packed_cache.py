@@ -280,3 +280,25 @@ def test_a_refused_batch_keeps_the_positions():
         cache.table.check()
     assert cache.extend([0, 1], 2).positions.tolist() == [64, 65, 0, 1]
     cache.table.check()
+
+
+# ---- attention: work that other CTAs have not begun -----------------------------
+@pytest.mark.parametrize("H,KVH,split", [(16, 16, False), (2, 1, True)])
+def test_attention_with_far_more_ctas_than_items(H, KVH, split):
+    """Short sequences in tensors that have room for long ones: nearly all
+    CTAs have no item, and every row that has one is computed."""
+    D, room = 64, 6000 if split else 40000
+    q, k, v = make_qkv([room], H, KVH, D, torch.float16, seed=41)
+    need = capi.lib().memopt_packed_attention_workspace_size
+    need.restype = capi.SZ
+    for lens in ([3], [0, 500, 1, 700], [1] * 30, [2600, 0, 5]):
+        cu = cu_of(lens + [0] * (31 - len(lens)))
+        asked = need(capi.I(31), capi.I64(room), capi.I(room), capi.I(H), capi.I(KVH), capi.I(D), capi.I(0), capi.I(1))
+        assert (asked > 0) == split
+        T = sum(lens)
+        for causal in (True, False):
+            out = torch.full_like(q, float("nan"))
+            C().packed_attention(q, k, v, cu, room, -1, causal, out)
+            ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, -1, causal)
+            assert ((out[:T].double() - ref).abs() <= attention_tol(ref, mag, v, max(lens), torch.float16)).all()
+            assert torch.isnan(out[T:].float()).all()
