@@ -35,7 +35,10 @@
 // (starting at 64 or at 128: 15% slower).  With D = 64 tensor memory has room for
 // P beside the scores, and the next scores run during the softmax.  O is rescaled
 // only when the running maximum grows by more than 2^8 (weights stay <= 2^8 and
-// the sums fp32), which is rare.
+// the sums fp32), which is rare.  Weights are rounded to 16 bits for P V, as its A
+// operand has to be of V's type; the row sum adds them in fp32.  Against 64 bits a
+// result is off by 9 to 32% more than with fp32 weights (fp16 2.1e-4 to 2.7e-4 over
+// an output, bf16 2.1e-3; the rounding of the result alone 1.9e-4 and 1.65e-3).
 //
 // What bounds it: for each tile and block 1024 cycles of the tensor pipe (D = 128)
 // and 1024 of the exponential unit, which the two tiles overlap to 2950 cycles a
@@ -207,6 +210,14 @@ __device__ __forceinline__ uint32_t odd2<__nv_bfloat16>(uint32_t u, uint32_t sum
   asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(u), "r"(0u));
   return sum;
 }
+
+// Weights are held as 2^kLift of themselves (O and the row's sum alike, so it cancels).
+// P.V takes them in 16 bits, relative to a running maximum that may lag by 2^8: fp16
+// weights then end at 2^15, and those that would be subnormal or nothing keep 7 bits
+// more. Without it thousands of weights below 2^-25 beside one large key were lost
+// (65536 of them 2^-25.2 each: 0 for 1.6e-3).  bf16 has the range of fp32.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t u);
@@ -520,8 +531,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           }
           ok = take_max(mx, j) && p_free(j);
           if (!ok) break;
-          const float msub = m_run == -INFINITY ? 0.f : m_run;  // nothing visible yet: every weight is 2^-inf = 0
-          const uint64_t nm2 = f32x2_pack(-msub, -msub);
+          const float add = kLift<T> - (m_run == -INFINITY ? 0.f : m_run);  // nothing visible yet: every weight is 2^-inf = 0
+          const uint64_t nm2 = f32x2_pack(add, add);
 #pragma unroll 1
           for (int cc = 0; cc < chunks; ++cc) {
             uint32_t ph[16] = {};
@@ -566,8 +577,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
           }
           ok = take_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), j);
           if (!ok) break;
-          const float msub = m_run == -INFINITY ? 0.f : m_run;
-          const uint64_t nm2 = f32x2_pack(-msub, -msub);
+          const float add = kLift<T> - (m_run == -INFINITY ? 0.f : m_run);
+          const uint64_t nm2 = f32x2_pack(add, add);
           ok = p_free(j);
           if (!ok) break;
           // 32 keys at a time; P.V starts on the first kFirst steps of 16 keys.
@@ -668,8 +679,8 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
       }
       tc::fence_before_sync();
-      // A weight of the row's maximum is at least 1 and no weight exceeds 2^8, so
-      // a sum outside [1/2, 2^100) is not one of finite scores.
+      // A weight of the row's maximum is at least 1 and no weight exceeds 2^15 (both
+      // with the lift), so a sum outside [1/2, 2^100) is not one of finite scores.
       uint32_t redo = __ballot_sync(0xffffffffu, ok && tok < it.n && !((odd & 0x7fff7fffu) == 0 && l_run >= 0.5f && l_run < 1.2e30f));
       __syncwarp();
       while (redo) {

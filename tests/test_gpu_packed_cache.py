@@ -302,3 +302,28 @@ def test_attention_with_far_more_ctas_than_items(H, KVH, split):
             ref, mag = attention_ref(q[:T], k[:T], v[:T], lens, -1, causal)
             assert ((out[:T].double() - ref).abs() <= attention_tol(ref, mag, v, max(lens), torch.float16)).all()
             assert torch.isnan(out[T:].float()).all()
+
+
+# ---- attention: many small weights --------------------------------------------------
+@pytest.mark.parametrize("H,n", [(1, 65536), (64, 12000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_a_sink_and_a_flat_tail(H, n, dtype):
+    """One key far above all others, and thousands of others that count only
+    together: e^-17.5 = 2^-25.2 each.  All are seen in every row's sum, so the
+    result is i w / (1 + i w) for values of 0 (the sink) and 1."""
+    D = 64
+    q = torch.zeros(n, H, D, device=DEV, dtype=dtype)
+    k, v = torch.zeros(n, 1, D, device=DEV, dtype=dtype), torch.ones(n, 1, D, device=DEV, dtype=dtype)
+    q[..., 0] = 8.0
+    k[0, 0, 0], v[0] = 17.5, 0.0
+    out = C().packed_attention(q, k, v, cu_of([n]), n)
+    w = torch.arange(n, device=DEV, dtype=torch.float64) * math.exp(-17.5)
+    want = (w / (1 + w))[:, None, None]
+    # half a step of the result; the weight's own rounding (2 half steps) and the exponential
+    # (2^-14, scores below 32); fp16 weights are held as 2^7 of themselves, so that each is off
+    # by at most 2^-25 / 2^7 where it is subnormal
+    u = half_step(dtype)
+    tol = (3 * u + 2.0 ** -14) * want + 1e-7
+    if dtype == torch.float16:
+        tol = tol + torch.arange(n, device=DEV)[:, None, None] * 2.0 ** -32
+    assert ((out.double() - want).abs() <= tol).all()
