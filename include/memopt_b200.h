@@ -417,12 +417,14 @@ int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_r
 /* positions in the sequence, which is what keys in the cache were turned by.  */
 /* positions are index + offset; an empty row's offset becomes 0.  Whoever     */
 /* takes n tokens out of the middle of a row (evict_topk_compact shrinks       */
-/* context_lens by them) adds n to its offset.                                 */
+/* context_lens by them) adds n to its offset.  replace != 0: the rows begin   */
+/* anew, what they held is given back first (truncate_rows to nothing; those   */
+/* pages count as free); a refused call leaves them as they were.              */
 int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* position_offsets, int num_rows,
                         int max_blocks_per_seq, int32_t* free_pages, int num_blocks, int32_t* pool_state,
                         const int32_t* rows, const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
-                        int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
-                        int32_t* batch_lens, void* stream);
+                        int replace, int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
+                        int32_t* batch_tables, int32_t* batch_lens, void* stream);
 /* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none;    */
 /* keep_lens, like new_lens above, must not overlap context_lens);            */
 /* the pages behind them go to the ring's end in row and page order and their */

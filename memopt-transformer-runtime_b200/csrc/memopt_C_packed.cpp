@@ -117,7 +117,7 @@ namespace {
 std::vector<torch::Tensor> reserve(const char* who, torch::Tensor block_tables, torch::Tensor context_lens,
                                    const torch::Tensor* position_offsets, torch::Tensor free_pages,
                                    torch::Tensor pool_state, torch::Tensor rows, torch::Tensor new_lens, int block_size,
-                                   int64_t max_tokens) {
+                                   int64_t max_tokens, bool replace) {
   const PageTensors n = page_checks(who, block_tables, context_lens, free_pages, pool_state, rows, block_size);
   int32_cuda(new_lens, who, "new_lens", 1, block_tables.device());
   TORCH_CHECK(new_lens.size(0) == n.B, who, ": new_lens length != rows length");
@@ -144,8 +144,9 @@ std::vector<torch::Tensor> reserve(const char* who, torch::Tensor block_tables, 
   auto p = [](const torch::Tensor& t) { return t.data_ptr<int32_t>(); };
   check(position_offsets
             ? memopt_reserve_rows(p(block_tables), p(context_lens), p(*position_offsets), n.R, n.MB, p(free_pages),
-                                  n.NB, p(pool_state), p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu),
-                                  p(slots), p(positions), p(tables), p(lens), cur_stream())
+                                  n.NB, p(pool_state), p(rows), p(new_lens), n.B, block_size, max_tokens,
+                                  replace ? 1 : 0, p(cu), p(slots), p(positions), p(tables), p(lens),
+                                  cur_stream())
             : memopt_reserve_slots(p(block_tables), p(context_lens), n.R, n.MB, p(free_pages), n.NB, p(pool_state),
                                    p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu), p(slots), p(positions),
                                    p(tables), p(lens), cur_stream()),
@@ -159,15 +160,15 @@ std::vector<torch::Tensor> reserve_slots(torch::Tensor block_tables, torch::Tens
                                          torch::Tensor free_pages, torch::Tensor pool_state, torch::Tensor rows,
                                          torch::Tensor new_lens, int block_size, int64_t max_tokens) {
   return reserve("reserve_slots", block_tables, context_lens, nullptr, free_pages, pool_state, rows, new_lens,
-                 block_size, max_tokens);
+                 block_size, max_tokens, false);
 }
 
 std::vector<torch::Tensor> reserve_rows(torch::Tensor block_tables, torch::Tensor context_lens,
                                         torch::Tensor position_offsets, torch::Tensor free_pages,
                                         torch::Tensor pool_state, torch::Tensor rows, torch::Tensor new_lens,
-                                        int block_size, int64_t max_tokens) {
+                                        int block_size, int64_t max_tokens, bool replace) {
   return reserve("reserve_rows", block_tables, context_lens, &position_offsets, free_pages, pool_state, rows, new_lens,
-                 block_size, max_tokens);
+                 block_size, max_tokens, replace);
 }
 
 void truncate_rows(torch::Tensor block_tables, torch::Tensor context_lens, torch::Tensor free_pages,
@@ -341,9 +342,11 @@ void bind_packed(pybind11::module_& m) {
         py::arg("block_tables"), py::arg("context_lens"), py::arg("free_pages"), py::arg("pool_state"),
         py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"));
   m.def("reserve_rows", &reserve_rows,
-        "reserve_slots over rows that may have been evicted from: positions are index + position_offsets[row]",
+        "reserve_slots over rows that may have been evicted from: positions are index + position_offsets[row]; with "
+        "replace the rows begin anew, unless the call is refused",
         py::arg("block_tables"), py::arg("context_lens"), py::arg("position_offsets"), py::arg("free_pages"),
-        py::arg("pool_state"), py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"));
+        py::arg("pool_state"), py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"),
+        py::arg("replace") = false);
   m.def("truncate_rows", &truncate_rows,
         "Cut table row rows[b] to its first keep_lens[b] tokens (None: to nothing) and return the pages to the ring",
         py::arg("block_tables"), py::arg("context_lens"), py::arg("free_pages"), py::arg("pool_state"),

@@ -15,8 +15,11 @@
 //             offset being what an eviction took out of the row before it.
 //   truncate: the pages past ceil(k_b / BS) go to the ring's tail in row and
 //             page order.
+//   replace:  truncate to nothing, then reserve, both or neither: the first
+//             launch checks the second one's batch too and does nothing if that
+//             will not fit, and the second refuses rows that were not cut.
 //
-// One launch each: every CTA reads the old lengths and the old ring state and
+// One launch each (two for replace): every CTA reads the old lengths and the old ring state and
 // repeats the scan over the batch in shared memory (no CTA waits for another),
 // then expands its share of the tokens and of the table rows.  The CTA that
 // arrives last at a ticket in the pool state commits the new lengths, head and
@@ -47,6 +50,8 @@ struct PageArgs {
   int R, MB, NB, BS, B;
   int shift;  // log2(BS), or -1 where BS is no power of two
   int64_t max_tokens;
+  const int32_t* next;  // [B]: truncate's rows begin anew with so many tokens (null: they do not)
+  bool fresh;           // reserve: the rows have to be empty
   int32_t* offsets;    // [R]: a token's position less its index in the row (null: 0)
   int32_t* cu;         // [B + 1]
   int32_t* slots;      // [max_tokens]
@@ -54,6 +59,8 @@ struct PageArgs {
   int32_t* out_tables;  // [B, MB]
   int32_t* out_lens;    // [B]
 };
+
+constexpr uint32_t kNotCut = 1u << 30;  // internal refusal: the call's first launch has set the status
 
 // What a CTA holds of the batch in shared memory.
 struct Batch {
@@ -118,6 +125,10 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
       n = a.amount ? a.amount[b] : 0;
       if (n < 0 || (!kReserve && n > old)) {
         bits |= MEMOPT_PAGES_BAD_LENGTH;
+        n = 0;
+      }
+      if (kReserve && a.fresh && old > 0) {
+        bits |= kNotCut;
         n = 0;
       }
       if (kReserve) {
@@ -313,10 +324,44 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
         a.state[0] = static_cast<int32_t>((head + pages) % a.NB);
         a.state[1] = static_cast<int32_t>(count - pages);
       }
-      if (status) atomicOr(a.state + 2, static_cast<int>(status));
+      if (status & ~kNotCut) atomicOr(a.state + 2, static_cast<int>(status & ~kNotCut));
       a.state[3] = 0;
     }
   }
+}
+
+// Whether the batch of a.next fits once the rows are empty and `free_pages` pages
+// are free: the status bits that reserve would give it.
+template <int kThreads>
+__device__ uint32_t next_batch_fits(const PageArgs& a, int64_t free_pages) {
+  __shared__ unsigned long long s_sum[2];
+  __shared__ uint32_t s_bits;
+  if (threadIdx.x == 0) s_sum[0] = s_sum[1] = s_bits = 0;
+  __syncthreads();
+  const int64_t cap = static_cast<int64_t>(a.MB) * a.BS;
+  uint32_t bits = 0;
+  int64_t tokens = 0, pages = 0;
+  for (int b = threadIdx.x; b < a.B; b += kThreads) {
+    const int n = a.next[b];
+    if (n < 0) bits |= MEMOPT_PAGES_BAD_LENGTH;
+    else if (n > cap) bits |= MEMOPT_PAGES_ROW_FULL;
+    else tokens += n, pages += pages_of(n, a);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    tokens += __shfl_xor_sync(0xffffffffu, tokens, d);
+    pages += __shfl_xor_sync(0xffffffffu, pages, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    atomicAdd(&s_sum[0], static_cast<unsigned long long>(tokens));
+    atomicAdd(&s_sum[1], static_cast<unsigned long long>(pages));
+  }
+  if (bits) atomicOr(&s_bits, bits);
+  __syncthreads();
+  bits = s_bits;
+  if (static_cast<int64_t>(s_sum[0]) > a.max_tokens) bits |= MEMOPT_PAGES_BAD_LENGTH;
+  if (bits == 0 && static_cast<int64_t>(s_sum[1]) > free_pages) bits |= MEMOPT_PAGES_EXHAUSTED;
+  return bits;
 }
 
 template <int kThreads>
@@ -332,6 +377,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(const PageArgs a) {
   uint32_t status = scan_batch<kThreads, false>(a, t, kept, pages);
   if (head < 0 || head >= a.NB || count < 0 || count > a.NB || (status == 0 && count + pages > a.NB))
     status |= MEMOPT_PAGES_CORRUPT;
+  if (a.next) status |= next_batch_fits<kThreads>(a, count + pages);
   uint32_t bits = 0;
   if (status == 0) {
     const int nwarps = gridDim.x * kWarps;
@@ -405,7 +451,8 @@ int launch_pages(K small, K large, const char* what, const PageArgs& a, cudaStre
     if (e != cudaSuccess) return cuda_fail(e, what);
   }
   const int64_t per_cta = threads * kTokensPerThread, rows = threads / 32;
-  const int64_t want = std::max((a.max_tokens + per_cta - 1) / per_cta, (a.B + rows - 1) / rows);
+  const int64_t tokens = a.next ? 0 : a.max_tokens;  // truncate expands none
+  const int64_t want = std::max((tokens + per_cta - 1) / per_cta, (a.B + rows - 1) / rows);
   const int grid = static_cast<int>(std::min<int64_t>(sm_count(), std::max<int64_t>(1, want)));
   MEMOPT_LAUNCH(launch_after(kern, grid, threads, smem, s, a), what);
   return MEMOPT_OK;
@@ -420,6 +467,12 @@ int reserve(const char* who, PageArgs a, cudaStream_t s) {
   if ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15u)
     return fail(MEMOPT_ERR_INVALID_ARG, std::string(who) + ": slot_mapping and positions must be 16-byte aligned");
   a.shift = log2_of(a.BS);
+  if (a.fresh && a.B > 0) {
+    PageArgs cut = a;
+    cut.amount = nullptr, cut.next = a.amount;
+    const int st2 = launch_pages(truncate_kernel<256>, truncate_kernel<1024>, "truncate_kernel launch", cut, s);
+    if (st2 != MEMOPT_OK) return st2;
+  }
   return launch_pages(reserve_kernel<256>, reserve_kernel<1024>, "reserve_kernel launch", a, s);
 }
 
@@ -434,7 +487,7 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
                                     int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
                                     int32_t* batch_tables, int32_t* batch_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, max_tokens, nullptr, cu_seqlens, slot_mapping, positions, batch_tables,
+             num_blocks, block_size, batch, 0, max_tokens, nullptr, false, nullptr, cu_seqlens, slot_mapping, positions, batch_tables,
              batch_lens};
   return reserve("reserve_slots", a, as_stream(stream));
 }
@@ -442,11 +495,12 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
 extern "C" int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* position_offsets,
                                    int num_rows, int max_blocks_per_seq, int32_t* free_pages, int num_blocks,
                                    int32_t* pool_state, const int32_t* rows, const int32_t* new_lens, int batch,
-                                   int block_size, int64_t max_tokens, int32_t* cu_seqlens, int32_t* slot_mapping,
-                                   int32_t* positions, int32_t* batch_tables, int32_t* batch_lens, void* stream) {
+                                   int block_size, int64_t max_tokens, int replace, int32_t* cu_seqlens,
+                                   int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
+                                   int32_t* batch_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, max_tokens, position_offsets, cu_seqlens, slot_mapping, positions,
-             batch_tables, batch_lens};
+             num_blocks, block_size, batch, 0, max_tokens, nullptr, replace != 0, position_offsets, cu_seqlens,
+             slot_mapping, positions, batch_tables, batch_lens};
   if (!position_offsets) return fail(MEMOPT_ERR_INVALID_ARG, "reserve_rows: null pointer");
   return reserve("reserve_rows", a, as_stream(stream));
 }
@@ -455,7 +509,7 @@ extern "C" int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens
                                     int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
                                     const int32_t* keep_lens, int batch, int block_size, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, keep_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+             num_blocks, block_size, batch, 0, 0, nullptr, false, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   const int st = check_pages("truncate_rows", a);
   if (st != MEMOPT_OK) return st;
   if (batch == 0) return MEMOPT_OK;

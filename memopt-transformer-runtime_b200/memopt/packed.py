@@ -99,6 +99,14 @@ class DevicePageTable:
         must then be a Python sequence); the sum may be smaller, a larger one
         is refused.  A refused batch changes nothing (see :meth:`check`): its
         ``cu_seqlens`` are zero and its slots -1."""
+        return self._reserve(rows, new_lens, max_tokens, False)
+
+    def replace(self, rows: Ints, new_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
+        """:meth:`reserve` for sequences that begin: what the rows held is
+        given back first, unless the batch is refused."""
+        return self._reserve(rows, new_lens, max_tokens, True)
+
+    def _reserve(self, rows: Ints, new_lens: Ints, max_tokens: Optional[int], replace: bool) -> PackedBatch:
         if max_tokens is None:
             if isinstance(new_lens, torch.Tensor):
                 raise ValueError("reserve: max_tokens is needed when new_lens is a tensor")
@@ -106,7 +114,7 @@ class DevicePageTable:
         r = self.ints(rows)
         cu, slots, pos, tables, lens = self._C.reserve_rows(
             self.block_tables, self.context_lens, self.position_offsets, self.free_pages, self.pool_state, r,
-            self.ints(new_lens), self.block_size, max_tokens)
+            self.ints(new_lens), self.block_size, max_tokens, replace)
         return PackedBatch(r, cu, slots, pos, tables, lens)
 
     def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
@@ -279,11 +287,9 @@ class PackedKVCache:
     # ---- tables --------------------------------------------------------------
     def admit(self, rows: Ints, prompt_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
         """Starts a sequence in each row (what the row held is given back) and
-        reserves its prompt."""
+        reserves its prompt; a refused batch changes nothing."""
         self._need_pool()
-        r = self.table.ints(rows)
-        self.table.truncate(r)
-        batch = self.table.reserve(r, prompt_lens, max_tokens)
+        batch = self.table.replace(rows, prompt_lens, max_tokens)
         batch.whole = True
         return batch
 

@@ -327,3 +327,58 @@ def test_attention_of_a_sink_and_a_flat_tail(H, n, dtype):
     if dtype == torch.float16:
         tol = tol + torch.arange(n, device=DEV)[:, None, None] * 2.0 ** -32
     assert ((out.double() - want).abs() <= tol).all()
+
+
+# ---- refused batches -------------------------------------------------------------
+def test_a_refused_admission_changes_nothing():
+    """Rows that a refused admit names keep what they held."""
+    from memopt import PackedKVCache
+
+    H, KVH, D, BS = 2, 2, 64, 16
+    cache = PackedKVCache(10, KVH, D, BS, max_seqs=3, max_seq_len=96)  # six pages a row
+    own = sorted(cache.table.free_pages[:10].tolist())
+    q, k, v = tokens(50, H, KVH, D, seed=5)
+    cache.prompt(q, k, v, cache.admit([0, 2], [30, 20]), 30)
+    t = cache.table
+    state = lambda: [x.clone() for x in (t.block_tables, t.context_lens, t.free_pages, t.pool_state[:2])]
+    before = state()
+    calls = [(([0, 1, 2], [96, 60, 1]), MemoryError),            # 6 + 4 + 1 pages of 10
+             (([0], [97]), RuntimeError), (([2, 0], [-1, 5], 9), RuntimeError), (([0, 0], [1, 1]), RuntimeError),
+             (([0, 3], [1, 1]), RuntimeError), (([0, 2], [4, 5], 8), RuntimeError),
+             (([1, 0], [2 ** 31 - 1, 1], 64), RuntimeError)]
+    for args, error in calls:
+        batch = cache.admit(*args)
+        assert (batch.slot_mapping == -1).all() and not batch.cu_seqlens.any()
+        assert all(torch.equal(a, b) for a, b in zip(before, state()))
+        with pytest.raises(error):
+            t.check()
+    kk, vv = cached(cache, 0)
+    assert torch.equal(kk, k[:30]) and torch.equal(vv, v[:30])
+    # What only fits with the rows' own pages is taken: 2 + 2 of them held, 6 free, 10 asked for.
+    batch = cache.admit([0, 2], [96, 60])
+    t.check()
+    assert t.free_count() == 0 and batch.context_lens.tolist() == [96, 60]
+    assert sorted(t.block_tables[t.block_tables >= 0].tolist()) == own
+    assert batch.cu_seqlens.tolist() == [0, 96, 156] and batch.positions.tolist() == [*range(96), *range(60)]
+
+
+@pytest.mark.parametrize("rows,high", [(5, 90), (300, 40), (1100, 40)])
+def test_admission_gives_the_old_pages_back_first(rows, high):
+    """admit is truncate and reserve: the same pages in the same order."""
+    from memopt import DevicePageTable
+
+    g = torch.Generator().manual_seed(rows)
+    tables = [DevicePageTable(rows * 8, 16, rows + 5, 112) for _ in range(2)]
+    for step in range(4):
+        pick = torch.randperm(rows + 5, generator=g)[:rows].to(torch.int32).to(DEV)
+        new = torch.randint(0, high, (rows,), generator=g, dtype=torch.int32)
+        total, new = int(new.sum()) + step, new.to(DEV)
+        a = tables[0].replace(pick, new, total)
+        tables[1].truncate(pick)
+        b = tables[1].reserve(pick, new, total)
+        for x, y in zip((a.cu_seqlens, a.slot_mapping, a.positions, a.block_tables, a.context_lens),
+                        (b.cu_seqlens, b.slot_mapping, b.positions, b.block_tables, b.context_lens)):
+            assert torch.equal(x, y)
+        for name in ("block_tables", "context_lens", "free_pages", "pool_state"):
+            assert torch.equal(getattr(tables[0], name), getattr(tables[1], name))
+        tables[0].check()

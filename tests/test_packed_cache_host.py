@@ -128,9 +128,9 @@ SOME = 0x1000  # a 16-byte aligned address that no call may touch
 
 
 def reserve_rows(tables=SOME, lens=SOME, off=SOME, R=4, MB=8, ring=SOME, NB=32, state=SOME, rows=SOME, new=SOME, B=2,
-                 BS=16, most=64, cu=SOME, slots=SOME, pos=SOME, bt=SOME, bl=SOME):
+                 BS=16, most=64, replace=0, cu=SOME, slots=SOME, pos=SOME, bt=SOME, bl=SOME):
     return capi.lib().memopt_reserve_rows(P(tables), P(lens), P(off), I(R), I(MB), P(ring), I(NB), P(state), P(rows),
-                                          P(new), I(B), I(BS), I64(most), P(cu), P(slots), P(pos), P(bt), P(bl), P(0))
+                                          P(new), I(B), I(BS), I64(most), I(replace), P(cu), P(slots), P(pos), P(bt), P(bl), P(0))
 
 
 @pytest.mark.parametrize("change,status", [
@@ -140,5 +140,5 @@ def reserve_rows(tables=SOME, lens=SOME, off=SOME, R=4, MB=8, ring=SOME, NB=32, 
     (dict(R=0), -1), (dict(MB=0), -1), (dict(NB=0), -1), (dict(BS=0), -1), (dict(B=8193), -3),
     (dict(R=2 ** 18 + 1), -3), (dict(NB=2 ** 27), -3), (dict(MB=2 ** 27), -3), (dict(most=2 ** 31), -3)])
 def test_reserve_rows_refuses(change, status):
-    assert reserve_rows(**change) == status
+    assert reserve_rows(**change) == reserve_rows(**change, replace=1) == status
     assert capi.lib().memopt_last_error().decode().startswith("reserve_rows:")
