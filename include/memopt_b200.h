@@ -419,12 +419,15 @@ int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens, int num_r
 /* takes n tokens out of the middle of a row (evict_topk_compact shrinks       */
 /* context_lens by them) adds n to its offset.  replace != 0: the rows begin   */
 /* anew, what they held is given back first (truncate_rows to nothing; those   */
-/* pages count as free); a refused call leaves them as they were.              */
+/* pages count as free); a refused call leaves them as they were.  attend_lens  */
+/* int32 [batch]: batch_lens, but 0 in a refused call, whose rows then attend   */
+/* over nothing (paged attention gives them zeros) and not over a context      */
+/* without the new tokens.                                                     */
 int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* position_offsets, int num_rows,
                         int max_blocks_per_seq, int32_t* free_pages, int num_blocks, int32_t* pool_state,
                         const int32_t* rows, const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
                         int replace, int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
-                        int32_t* batch_tables, int32_t* batch_lens, void* stream);
+                        int32_t* batch_tables, int32_t* batch_lens, int32_t* attend_lens, void* stream);
 /* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none;    */
 /* keep_lens, like new_lens above, must not overlap context_lens);            */
 /* the pages behind them go to the ring's end in row and page order and their */
@@ -479,6 +482,13 @@ int memopt_packed_attention(const void* query, int64_t query_stride, const void*
                             int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads, int num_kv_heads,
                             int head_dim, int window_size, int causal, void* out, void* workspace,
                             size_t workspace_bytes, void* stream);
+/* The same with zero_rest != 0: the rows of out from cu_seqlens[num_seqs] on  */
+/* are set to 0 in the same pass.  The workspace size is the same.             */
+int memopt_packed_attention_ex(const void* query, int64_t query_stride, const void* keys, int64_t key_stride,
+                               const void* values, int64_t value_stride, int dtype, const int32_t* cu_seqlens,
+                               int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads, int num_kv_heads,
+                               int head_dim, int window_size, int causal, int zero_rest, void* out, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

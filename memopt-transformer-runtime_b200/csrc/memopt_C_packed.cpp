@@ -132,26 +132,30 @@ std::vector<torch::Tensor> reserve(const char* who, torch::Tensor block_tables, 
   rows = rows.contiguous();
   new_lens = new_lens.contiguous();
   const at::cuda::CUDAGuard g(block_tables.device());
-  // One allocation behind the five outputs (an allocation each costs the host
+  // One allocation behind the outputs (an allocation each costs the host
   // more than the launch), every one 16-byte aligned.
   auto up4 = [](int64_t v) { return (v + 3) & ~int64_t(3); };
   const int64_t at_pos = up4(max_tokens), at_tables = at_pos + up4(max_tokens);
   const int64_t at_cu = at_tables + up4(static_cast<int64_t>(n.B) * n.MB), at_lens = at_cu + up4(n.B + 1);
-  const auto buf = torch::empty({at_lens + n.B}, block_tables.options());
+  const int64_t at_attend = at_lens + up4(n.B);
+  const auto buf = torch::empty({position_offsets ? at_attend + n.B : at_lens + n.B}, block_tables.options());
   auto slots = part_of(buf, 0, {max_tokens}), positions = part_of(buf, at_pos, {max_tokens});
   auto tables = part_of(buf, at_tables, {n.B, n.MB}), cu = part_of(buf, at_cu, {n.B + 1});
   auto lens = part_of(buf, at_lens, {n.B});
   auto p = [](const torch::Tensor& t) { return t.data_ptr<int32_t>(); };
-  check(position_offsets
-            ? memopt_reserve_rows(p(block_tables), p(context_lens), p(*position_offsets), n.R, n.MB, p(free_pages),
-                                  n.NB, p(pool_state), p(rows), p(new_lens), n.B, block_size, max_tokens,
-                                  replace ? 1 : 0, p(cu), p(slots), p(positions), p(tables), p(lens),
-                                  cur_stream())
-            : memopt_reserve_slots(p(block_tables), p(context_lens), n.R, n.MB, p(free_pages), n.NB, p(pool_state),
-                                   p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu), p(slots), p(positions),
-                                   p(tables), p(lens), cur_stream()),
+  if (!position_offsets) {
+    check(memopt_reserve_slots(p(block_tables), p(context_lens), n.R, n.MB, p(free_pages), n.NB, p(pool_state),
+                               p(rows), p(new_lens), n.B, block_size, max_tokens, p(cu), p(slots), p(positions),
+                               p(tables), p(lens), cur_stream()),
+          who);
+    return {cu, slots, positions, tables, lens};
+  }
+  auto attend = part_of(buf, at_attend, {n.B});
+  check(memopt_reserve_rows(p(block_tables), p(context_lens), p(*position_offsets), n.R, n.MB, p(free_pages), n.NB,
+                            p(pool_state), p(rows), p(new_lens), n.B, block_size, max_tokens, replace ? 1 : 0, p(cu),
+                            p(slots), p(positions), p(tables), p(lens), p(attend), cur_stream()),
         who);
-  return {cu, slots, positions, tables, lens};
+  return {cu, slots, positions, tables, lens, attend};
 }
 
 }  // namespace
@@ -289,7 +293,7 @@ std::vector<torch::Tensor> rotary_write_cache(torch::Tensor query, torch::Tensor
 
 torch::Tensor packed_attention(torch::Tensor query, torch::Tensor keys, torch::Tensor values,
                                torch::Tensor cu_seqlens, int64_t max_seqlen, int64_t window_size, bool causal,
-                               c10::optional<torch::Tensor> out_) {
+                               c10::optional<torch::Tensor> out_, bool zero_rest) {
   const char* who = "packed_attention";
   TORCH_CHECK(query.is_cuda(), who, ": query must be a CUDA tensor");
   TORCH_CHECK(query.dim() == 3, who, ": query must be 3-D [num_tokens, num_heads, head_dim]");
@@ -318,7 +322,7 @@ torch::Tensor packed_attention(torch::Tensor query, torch::Tensor keys, torch::T
   } else {
     out = torch::empty(query.sizes(), query.options());
   }
-  if (T == 0 || S == 0) return out;
+  if (T == 0 || (S == 0 && !zero_rest)) return out;
   auto q = packed_rows(query), k = packed_rows(keys), v = packed_rows(values);
   cu_seqlens = cu_seqlens.contiguous();
   const int window = window_size <= 0 || window_size > 0x7fffffff ? 0 : static_cast<int>(window_size);
@@ -326,10 +330,10 @@ torch::Tensor packed_attention(torch::Tensor query, torch::Tensor keys, torch::T
                                                                  causal ? 1 : 0);
   torch::Tensor ws;
   if (ws_bytes > 0) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, query.options().dtype(torch::kUInt8));
-  check(memopt_packed_attention(q.data_ptr(), row_stride(q), k.data_ptr(), row_stride(k), v.data_ptr(), row_stride(v),
-                                dtype, cu_seqlens.data_ptr<int32_t>(), S, T, static_cast<int>(max_seqlen), H, KVH, D,
-                                window, causal ? 1 : 0, out.data_ptr(), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
-                                cur_stream()),
+  check(memopt_packed_attention_ex(q.data_ptr(), row_stride(q), k.data_ptr(), row_stride(k), v.data_ptr(),
+                                   row_stride(v), dtype, cu_seqlens.data_ptr<int32_t>(), S, T,
+                                   static_cast<int>(max_seqlen), H, KVH, D, window, causal ? 1 : 0, zero_rest ? 1 : 0,
+                                   out.data_ptr(), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream()),
         who);
   return out;
 }
@@ -343,7 +347,7 @@ void bind_packed(pybind11::module_& m) {
         py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"));
   m.def("reserve_rows", &reserve_rows,
         "reserve_slots over rows that may have been evicted from: positions are index + position_offsets[row]; with "
-        "replace the rows begin anew, unless the call is refused",
+        "replace the rows begin anew, unless the call is refused; also returns the lengths to attend over, 0 if refused",
         py::arg("block_tables"), py::arg("context_lens"), py::arg("position_offsets"), py::arg("free_pages"),
         py::arg("pool_state"), py::arg("rows"), py::arg("new_lens"), py::arg("block_size"), py::arg("max_tokens"),
         py::arg("replace") = false);
@@ -359,7 +363,10 @@ void bind_packed(pybind11::module_& m) {
         py::arg("query"), py::arg("keys"), py::arg("values"), py::arg("positions"), py::arg("inv_freq"),
         py::arg("sections"), py::arg("slot_mapping"), py::arg("key_cache"), py::arg("value_cache"),
         py::arg("interleaved") = false);
-  m.def("packed_attention", &packed_attention, "Attention inside each sequence of a packed batch, grouped heads",
+  m.def("packed_attention", &packed_attention,
+        "Attention inside each sequence of a packed batch, grouped heads; rows outside every sequence are left as they "
+        "are, or with zero_rest those from cu_seqlens[-1] on become 0",
         py::arg("query"), py::arg("keys"), py::arg("values"), py::arg("cu_seqlens"), py::arg("max_seqlen"),
-        py::arg("window_size") = -1, py::arg("causal") = true, py::arg("out") = py::none());
+        py::arg("window_size") = -1, py::arg("causal") = true, py::arg("out") = py::none(),
+        py::arg("zero_rest") = false);
 }

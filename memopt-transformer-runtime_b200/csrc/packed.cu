@@ -95,6 +95,7 @@ struct Params {
   int units;        // head units: H >> gshift
   int chunk;        // head units walked together
   int window, causal;
+  int zero_rest;    // rows behind the last sequence are written as 0
   float qscale;     // log2(e) / sqrt(D)
   // Split items: key blocks of a piece, most pieces of a tile, and for every tile,
   // head unit and piece the unscaled O [D/4][128 rows] float4 and the rows' (m, l).
@@ -930,6 +931,18 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         i = cta;
         return got;
       };
+      // Index i's share of the rows behind the last sequence.  Every index of the grid
+      // passes here once, in one CTA or another, so this costs no launch.
+      const int rest = p.zero_rest ? min(max(cu[p.S], 0), p.T) : p.T;
+      const int share = rest < p.T ? static_cast<int>((static_cast<int64_t>(p.T - rest) + gridDim.x - 1) / gridDim.x) : 0;
+      auto zero_share = [&] {
+        const int64_t first = rest + static_cast<int64_t>(i) * share;
+        if (share == 0 || first >= p.T) return;
+        const int64_t row = static_cast<int64_t>(p.H) * D;
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + first * row);
+        const int64_t n = min(static_cast<int64_t>(share), p.T - first) * row / 8;
+        for (int64_t e = lane; e < n; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+      };
       // The item of index i; false when there is none.  The items are those of the
       // indexes below `end` (split: an upper bound that every miss lowers).
       uint32_t end = SPLIT ? 0xffffffffu : total;
@@ -1030,6 +1043,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         Item it{0, -1, 0, 0, 0, 0}, got = it;
         while (more) {
+          zero_share();
           bool has = find(got);
           if (SPLIT && has) {  // not a piece that this token block does not have
             const Range r = item_range<TILES, SPLIT>(p, got, 0);
@@ -1312,6 +1326,17 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
                                        int num_seqs, int64_t total_tokens, int max_seqlen, int num_heads,
                                        int num_kv_heads, int head_dim, int window_size, int causal, void* out,
                                        void* workspace, size_t workspace_bytes, void* stream) {
+  return memopt_packed_attention_ex(query, query_stride, keys, key_stride, values, value_stride, dtype, cu_seqlens,
+                                    num_seqs, total_tokens, max_seqlen, num_heads, num_kv_heads, head_dim, window_size,
+                                    causal, 0, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int memopt_packed_attention_ex(const void* query, int64_t query_stride, const void* keys,
+                                          int64_t key_stride, const void* values, int64_t value_stride, int dtype,
+                                          const int32_t* cu_seqlens, int num_seqs, int64_t total_tokens,
+                                          int max_seqlen, int num_heads, int num_kv_heads, int head_dim,
+                                          int window_size, int causal, int zero_rest, void* out, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
   if (num_seqs < 0 || total_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
     return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: invalid geometry");
   if (dtype != MEMOPT_DTYPE_F16 && dtype != MEMOPT_DTYPE_BF16)
@@ -1319,7 +1344,13 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   if (head_dim != 64 && head_dim != 128)
     return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: head_dim must be 64 or 128");
   if (total_tokens > 0x7fffff00LL) return fail(MEMOPT_ERR_UNSUPPORTED, "packed_attention: more than 2^31 tokens");
-  if (num_seqs == 0 || total_tokens == 0) return MEMOPT_OK;
+  if (total_tokens == 0 || (num_seqs == 0 && !zero_rest)) return MEMOPT_OK;
+  if (num_seqs == 0) {  // no sequence: every row is behind the last one
+    if (!out) return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: null pointer");
+    const cudaError_t e = cudaMemsetAsync(out, 0, static_cast<size_t>(total_tokens) * num_heads * head_dim * 2,
+                                          as_stream(stream));
+    return e == cudaSuccess ? MEMOPT_OK : cuda_fail(e, "packed_attention");
+  }
   if (!query || !keys || !values || !cu_seqlens || !out)
     return fail(MEMOPT_ERR_INVALID_ARG, "packed_attention: null pointer");
   if (!packed::aligned16(query) || !packed::aligned16(keys) || !packed::aligned16(values) ||
@@ -1341,6 +1372,7 @@ extern "C" int memopt_packed_attention(const void* query, int64_t query_stride, 
   p.part_o = static_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + pl.tile_slots * pl.pieces * (head_dim / 4) * 128);
   p.window = window_size > 0 ? window_size : 0, p.causal = causal ? 1 : 0;
+  p.zero_rest = zero_rest ? 1 : 0;
   p.qscale = (1.0f / sqrtf(static_cast<float>(head_dim))) * 1.4426950408889634f;
   // Head units per chunk: the chunk's keys and values fill about a quarter of L2.
   // Units that share a KV head stay together.

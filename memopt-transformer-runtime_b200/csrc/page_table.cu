@@ -58,6 +58,7 @@ struct PageArgs {
   int32_t* positions;  // [max_tokens]
   int32_t* out_tables;  // [B, MB]
   int32_t* out_lens;    // [B]
+  int32_t* attend_lens;  // [B]: out_lens, 0 where the call is refused (may be null)
 };
 
 constexpr uint32_t kNotCut = 1u << 30;  // internal refusal: the call's first launch has set the status
@@ -307,7 +308,11 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
         out[c] = v[i];
       }
     }
-    if (lane == 0) a.out_lens[b] = bad ? 0 : t.old[b] + (taken ? t.cu[b + 1] - t.cu[b] : 0);
+    if (lane == 0) {
+      const int len = bad ? 0 : t.old[b] + (taken ? t.cu[b + 1] - t.cu[b] : 0);
+      a.out_lens[b] = len;
+      if (a.attend_lens) a.attend_lens[b] = taken ? len : 0;
+    }
   }
   for (int i = blockIdx.x * kThreads + tid; i <= a.B; i += gridDim.x * kThreads) a.cu[i] = taken ? t.cu[i] : 0;
   if (bits) atomicOr(a.state + 2, static_cast<int>(bits));
@@ -488,7 +493,7 @@ extern "C" int memopt_reserve_slots(int32_t* block_tables, int32_t* context_lens
                                     int32_t* batch_tables, int32_t* batch_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
              num_blocks, block_size, batch, 0, max_tokens, nullptr, false, nullptr, cu_seqlens, slot_mapping, positions, batch_tables,
-             batch_lens};
+             batch_lens, nullptr};
   return reserve("reserve_slots", a, as_stream(stream));
 }
 
@@ -497,11 +502,11 @@ extern "C" int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens,
                                    int32_t* pool_state, const int32_t* rows, const int32_t* new_lens, int batch,
                                    int block_size, int64_t max_tokens, int replace, int32_t* cu_seqlens,
                                    int32_t* slot_mapping, int32_t* positions, int32_t* batch_tables,
-                                   int32_t* batch_lens, void* stream) {
+                                   int32_t* batch_lens, int32_t* attend_lens, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, new_lens, num_rows, max_blocks_per_seq,
              num_blocks, block_size, batch, 0, max_tokens, nullptr, replace != 0, position_offsets, cu_seqlens,
-             slot_mapping, positions, batch_tables, batch_lens};
-  if (!position_offsets) return fail(MEMOPT_ERR_INVALID_ARG, "reserve_rows: null pointer");
+             slot_mapping, positions, batch_tables, batch_lens, attend_lens};
+  if (!position_offsets || (batch > 0 && !attend_lens)) return fail(MEMOPT_ERR_INVALID_ARG, "reserve_rows: null pointer");
   return reserve("reserve_rows", a, as_stream(stream));
 }
 
@@ -509,7 +514,7 @@ extern "C" int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens
                                     int32_t* free_pages, int num_blocks, int32_t* pool_state, const int32_t* rows,
                                     const int32_t* keep_lens, int batch, int block_size, void* stream) {
   PageArgs a{block_tables, context_lens, free_pages, pool_state, rows, keep_lens, num_rows, max_blocks_per_seq,
-             num_blocks, block_size, batch, 0, 0, nullptr, false, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+             num_blocks, block_size, batch, 0, 0, nullptr, false, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   const int st = check_pages("truncate_rows", a);
   if (st != MEMOPT_OK) return st;
   if (batch == 0) return MEMOPT_OK;

@@ -55,6 +55,7 @@ class PackedBatch:
     positions: torch.Tensor     # [max_tokens] position of each new token in its sequence, evicted tokens counted
     block_tables: torch.Tensor  # [B, max_blocks_per_seq]
     context_lens: torch.Tensor  # [B] lengths with the new tokens
+    attend_lens: torch.Tensor   # [B] the same, 0 if the batch was refused
     whole: bool = False         # the new tokens are the whole sequences
 
 
@@ -112,10 +113,10 @@ class DevicePageTable:
                 raise ValueError("reserve: max_tokens is needed when new_lens is a tensor")
             max_tokens = sum(new_lens)
         r = self.ints(rows)
-        cu, slots, pos, tables, lens = self._C.reserve_rows(
+        cu, slots, pos, tables, lens, attend = self._C.reserve_rows(
             self.block_tables, self.context_lens, self.position_offsets, self.free_pages, self.pool_state, r,
             self.ints(new_lens), self.block_size, max_tokens, replace)
-        return PackedBatch(r, cu, slots, pos, tables, lens)
+        return PackedBatch(r, cu, slots, pos, tables, lens, attend)
 
     def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
         """Cuts each row to its first ``keep_lens`` tokens (None: to nothing)
@@ -326,18 +327,19 @@ class PackedKVCache:
         """Whole prompts (a batch of :meth:`admit`): rotary positions (the
         tokens' own, or ``positions`` [axes, T]), the cache write, and
         attention inside each prompt.  q [T, H, D], k and v [T, KVH, D]; rows
-        past the batch's last token come back as they are in memory."""
+        past the batch's last token, and all rows of a refused batch, are 0."""
         if not batch.whole:
             raise ValueError("PackedKVCache.prompt: the batch must come from admit (whole sequences)")
         self._need_pool()
         q, k = self._store(q, k, v, batch, positions)
-        return self._C.packed_attention(q, k, v, batch.cu_seqlens, max_seqlen, window_size, causal)
+        return self._C.packed_attention(q, k, v, batch.cu_seqlens, max_seqlen, window_size, causal, zero_rest=True)
 
     def decode(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PackedBatch, window_size: int = -1,
                positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The next tokens of each row (a batch of :meth:`extend`, the same
         number n of tokens per row): causal paged attention over the cached
-        context.  q [B * n, H, D]; the result has q's shape, in fp16."""
+        context.  q [B * n, H, D]; the result has q's shape, in fp16 (the
+        pool's type; 0 for a refused batch).  A window counts cached tokens."""
         if batch.whole:
             raise ValueError("PackedKVCache.decode: the batch must come from extend")
         B = batch.rows.numel()
@@ -350,10 +352,10 @@ class PackedKVCache:
         window = reach if window_size <= 0 else window_size
         if self.kv_format == "int4":
             out = self._C.dynamic_sparse_attention_int4(q4, self._C.get_int4_pages(), batch.block_tables,
-                                                        batch.context_lens, reach, window, True)
+                                                        batch.attend_lens, reach, window, True)
         else:
             kc, vc = self._C.get_pool_tensors()
-            out = self._C.dynamic_sparse_attention(q4, kc, vc, batch.block_tables, batch.context_lens, reach, window,
+            out = self._C.dynamic_sparse_attention(q4, kc, vc, batch.block_tables, batch.attend_lens, reach, window,
                                                    True)
         return out.reshape(q.shape)
 

@@ -382,3 +382,52 @@ def test_admission_gives_the_old_pages_back_first(rows, high):
         for name in ("block_tables", "context_lens", "free_pages", "pool_state"):
             assert torch.equal(getattr(tables[0], name), getattr(tables[1], name))
         tables[0].check()
+
+
+def test_a_refused_batch_gives_zeros():
+    """No stale memory and no attention without the new token: rows of a
+    refused batch, and rows past the last token, are zero."""
+    from memopt import DynamicAttention, PackedKVCache
+
+    H, KVH, D, BS = 4, 2, 64, 16
+    cache = PackedKVCache(6, KVH, D, BS, max_seqs=2, max_seq_len=96)
+    q, k, v = tokens(200, H, KVH, D, seed=6)
+    for _ in range(3):  # memory that the allocator hands out again
+        stale = torch.full_like(q, 9.0).contiguous()
+        del stale
+        assert not cache.prompt(q, k, v, cache.admit([0], [200]), 200).any()
+    with pytest.raises((MemoryError, RuntimeError)):
+        cache.table.check()
+    out = cache.prompt(q[:60], k[:60], v[:60], cache.admit([0], [33], 60), 33)
+    assert not out[33:].any() and out[:33].any(-1).all()
+    for n in (1, 3, 80):
+        batch = cache.extend([0, 0], n)
+        out = cache.decode(q[:2 * n], k[:2 * n], v[:2 * n], batch)
+        assert out.shape[0] == 2 * n and not out.any()
+        with pytest.raises(RuntimeError):
+            cache.table.check()
+    batch = cache.extend([0, 1])
+    assert cache.decode(q[:2], k[:2], v[:2], batch).any(-1).all()
+    assert batch.attend_lens.tolist() == batch.context_lens.tolist() == [34, 1]
+    layer = DynamicAttention(H * D, H).half().to(DEV)
+    two = PackedKVCache(6, H, D, BS, max_seqs=2, max_seq_len=96) if cache.close() is None else None
+    with torch.no_grad():
+        y = layer.forward_packed(torch.randn(200, H * D, device=DEV).half(), two, two.admit([0], [200]), 200)
+    assert not y.any()
+
+
+@pytest.mark.parametrize("H,KVH,D,lens,tail", [(4, 2, 64, [70, 0, 3], 500), (2, 1, 128, [2600], 1), (2, 1, 64, [], 2600),
+                                               (20, 20, 128, [1500, 900], 1300), (8, 2, 64, [0, 0], 77), (3, 3, 64, [1], 0)])
+def test_rows_behind_the_last_sequence_become_zero(H, KVH, D, lens, tail):
+    """zero_rest, in the whole, the two-tile and the split form; other rows as without it."""
+    T = sum(lens) + tail
+    q, k, v = make_qkv([T], H, KVH, D, torch.bfloat16, seed=8)
+    for causal in (True, False):
+        plain, out = (torch.full_like(q, 3.0) for _ in range(2))
+        C().packed_attention(q, k, v, cu_of(lens), T, -1, causal, plain)
+        C().packed_attention(q, k, v, cu_of(lens), T, -1, causal, out, zero_rest=True)
+        assert torch.equal(out[:T - tail], plain[:T - tail]) and not out[T - tail:].any()
+        assert (plain[T - tail:] == 3.0).all()
+    for cu in ([5, 2, 1], [0, -7], [0, 2 ** 31 - 1]):  # values that no table builds: inside the tensors all the same
+        C().packed_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=DEV), T, zero_rest=True)
+    torch.cuda.synchronize()

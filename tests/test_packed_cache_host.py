@@ -128,17 +128,30 @@ SOME = 0x1000  # a 16-byte aligned address that no call may touch
 
 
 def reserve_rows(tables=SOME, lens=SOME, off=SOME, R=4, MB=8, ring=SOME, NB=32, state=SOME, rows=SOME, new=SOME, B=2,
-                 BS=16, most=64, replace=0, cu=SOME, slots=SOME, pos=SOME, bt=SOME, bl=SOME):
+                 BS=16, most=64, replace=0, cu=SOME, slots=SOME, pos=SOME, bt=SOME, bl=SOME, al=SOME):
     return capi.lib().memopt_reserve_rows(P(tables), P(lens), P(off), I(R), I(MB), P(ring), I(NB), P(state), P(rows),
-                                          P(new), I(B), I(BS), I64(most), I(replace), P(cu), P(slots), P(pos), P(bt), P(bl), P(0))
+                                          P(new), I(B), I(BS), I64(most), I(replace), P(cu), P(slots), P(pos), P(bt),
+                                          P(bl), P(al), P(0))
 
 
 @pytest.mark.parametrize("change,status", [
     (dict(tables=0), -1), (dict(lens=0), -1), (dict(off=0), -1), (dict(ring=0), -1), (dict(state=0), -1),
     (dict(rows=0), -1), (dict(new=0), -1), (dict(cu=0), -1), (dict(slots=0), -1), (dict(pos=0), -1), (dict(bt=0), -1),
-    (dict(bl=0), -1), (dict(slots=SOME + 4), -1), (dict(pos=SOME + 8), -1), (dict(most=-1), -1), (dict(B=-1), -1),
+    (dict(bl=0), -1), (dict(al=0), -1), (dict(slots=SOME + 4), -1), (dict(pos=SOME + 8), -1), (dict(most=-1), -1), (dict(B=-1), -1),
     (dict(R=0), -1), (dict(MB=0), -1), (dict(NB=0), -1), (dict(BS=0), -1), (dict(B=8193), -3),
     (dict(R=2 ** 18 + 1), -3), (dict(NB=2 ** 27), -3), (dict(MB=2 ** 27), -3), (dict(most=2 ** 31), -3)])
 def test_reserve_rows_refuses(change, status):
     assert reserve_rows(**change) == reserve_rows(**change, replace=1) == status
     assert capi.lib().memopt_last_error().decode().startswith("reserve_rows:")
+
+
+def test_attention_ex_of_nothing_and_its_refusals():
+    def call(q=SOME, out=SOME, seqs=1, tokens=8, zero=1, qs=512):
+        return capi.lib().memopt_packed_attention_ex(P(q), I64(qs), P(SOME), I64(256), P(SOME), I64(256), I(0), P(SOME),
+                                                     I(seqs), I64(tokens), I(8), I(4), I(2), I(128), I(0), I(1), I(zero),
+                                                     P(out), P(0), ctypes.c_size_t(0), P(0))
+
+    assert call(tokens=0) == call(seqs=0, zero=0) == 0
+    for zero in (0, 1):
+        assert call(q=0, zero=zero) == call(qs=516, zero=zero) == call(out=0, zero=zero) == -1
+    assert call(seqs=0, out=0) == -1
