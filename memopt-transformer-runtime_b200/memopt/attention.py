@@ -153,8 +153,19 @@ class DynamicAttention(nn.Module):
         lengths (``max_seqlen``: the longest) and attend inside each prompt;
         with a batch of ``cache.extend`` the next tokens of each row, attending
         over its cached context.  ``positions`` [axes, num_tokens] replaces the
-        tokens' own positions where the cache has rotary positions.  The
-        attention carries no gradient."""
+        tokens' own positions where the cache has rotary positions.
+
+        The attention carries no gradient: while gradients are recorded, an
+        ``x`` that requires one is refused, and a layer whose q, k and v
+        projections do warns that only ``out_proj`` gets one.  Serve under
+        ``torch.no_grad()``."""
+        if torch.is_grad_enabled():
+            if x.requires_grad:
+                raise RuntimeError("forward_packed: the attention has no gradient; detach x or call it under "
+                                   "torch.no_grad()")
+            if any(p.weight.requires_grad for p in (self.q_proj, self.k_proj, self.v_proj)):
+                warnings.warn("forward_packed: the attention has no gradient, q_proj, k_proj and v_proj get none; call "
+                              "it under torch.no_grad()", RuntimeWarning, stacklevel=2)
         T = x.shape[0]
         shape = (T, self.num_heads, self.head_dim)
         q, k, v = (p(x).detach().reshape(shape) for p in (self.q_proj, self.k_proj, self.v_proj))

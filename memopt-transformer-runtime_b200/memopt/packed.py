@@ -20,7 +20,7 @@ and everything that depends on the lengths is built on the GPU:
   attention).
 
 These operators serve; they carry no gradient and refuse inputs that ask for
-one.
+one while gradients are recorded (serve under ``torch.no_grad()``).
 """
 from __future__ import annotations
 
@@ -307,6 +307,14 @@ class PackedKVCache:
         self.table.truncate(rows)
 
     # ---- data path -------------------------------------------------------------
+    @staticmethod
+    def _no_grad(*tensors: torch.Tensor) -> None:
+        """Before anything is written: paged attention and the cache write
+        would drop the gradient in silence."""
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+            raise RuntimeError("PackedKVCache: the operators have no gradient; detach their inputs or call them under "
+                               "torch.no_grad()")
+
     def _store(self, q, k, v, batch: PackedBatch, positions):
         if self.rotary is not None:
             pos = batch.positions if positions is None else positions
@@ -330,6 +338,7 @@ class PackedKVCache:
         past the batch's last token, and all rows of a refused batch, are 0."""
         if not batch.whole:
             raise ValueError("PackedKVCache.prompt: the batch must come from admit (whole sequences)")
+        self._no_grad(q, k, v)
         self._need_pool()
         q, k = self._store(q, k, v, batch, positions)
         return self._C.packed_attention(q, k, v, batch.cu_seqlens, max_seqlen, window_size, causal, zero_rest=True)
@@ -345,6 +354,7 @@ class PackedKVCache:
         B = batch.rows.numel()
         if B == 0 or q.shape[0] % B != 0:
             raise ValueError(f"PackedKVCache.decode: {q.shape[0]} tokens for {B} rows")
+        self._no_grad(q, k, v)
         self._need_pool()
         q, _ = self._store(q, k, v, batch, positions)
         q4 = q.to(torch.float16).contiguous().reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])

@@ -431,3 +431,42 @@ def test_rows_behind_the_last_sequence_become_zero(H, KVH, D, lens, tail):
     for cu in ([5, 2, 1], [0, -7], [0, 2 ** 31 - 1]):  # values that no table builds: inside the tensors all the same
         C().packed_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=DEV), T, zero_rest=True)
     torch.cuda.synchronize()
+
+
+# ---- gradients ---------------------------------------------------------------------
+@pytest.mark.parametrize("rotary", [False, True])
+def test_inputs_that_require_a_gradient_are_refused(rotary):
+    """None is cut off in silence, and a refused call writes nothing."""
+    from memopt import DynamicAttention, PackedKVCache, RotaryPositions
+
+    H, D = 2, 64
+    cache = PackedKVCache(7, H, D, 16, max_seqs=1, max_seq_len=96, rotary=RotaryPositions(D) if rotary else None)
+    layer = DynamicAttention(H * D, H).half().to(DEV)
+    x = torch.randn(20, H * D, device=DEV).half().requires_grad_(True)
+    q, k, v = tokens(20, H, H, D)
+    for pool in C().get_pool_tensors():
+        pool.fill_(7.0)
+    batch = cache.admit([0], [20])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer.forward_packed(x, cache, batch, 20)
+    for i in range(3):
+        args = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            cache.prompt(*args, batch, 20)
+    assert all((p == 7.0).all() for p in C().get_pool_tensors())
+    with torch.no_grad():
+        assert not layer.forward_packed(x, cache, batch, 20).requires_grad
+    step = cache.extend([0])
+    before = [p.clone() for p in C().get_pool_tensors()]
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer.forward_packed(x[:1], cache, step)
+    for i in range(3):
+        args = [t[:1].clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            cache.decode(*args, step)
+    assert all(torch.equal(a, b) for a, b in zip(before, C().get_pool_tensors()))
+    # The layer's own projections: out_proj trains, and the caller is told that the others do not.
+    with pytest.warns(RuntimeWarning, match="no gradient"):
+        y = layer.forward_packed(x[:1].detach(), cache, step)
+    y.float().sum().backward()
+    assert layer.out_proj.weight.grad is not None and layer.q_proj.weight.grad is None
