@@ -153,7 +153,8 @@ class DynamicAttention(nn.Module):
         lengths (``max_seqlen``: the longest) and attend inside each prompt;
         with a batch of ``cache.extend`` the next tokens of each row, attending
         over its cached context.  ``positions`` [axes, num_tokens] replaces the
-        tokens' own positions where the cache has rotary positions.
+        tokens' own positions where the cache has rotary positions.  The
+        layer's scheduler is not used here (``cache.evict`` evicts).
 
         The attention carries no gradient: while gradients are recorded, an
         ``x`` that requires one is refused, and a layer whose q, k and v
@@ -166,6 +167,9 @@ class DynamicAttention(nn.Module):
             if any(p.weight.requires_grad for p in (self.q_proj, self.k_proj, self.v_proj)):
                 warnings.warn("forward_packed: the attention has no gradient, q_proj, k_proj and v_proj get none; call "
                               "it under torch.no_grad()", RuntimeWarning, stacklevel=2)
+        if self.scheduler is not None:
+            warnings.warn("forward_packed: the layer's scheduler is not used on packed batches; evict through the cache",
+                          RuntimeWarning, stacklevel=2)
         T = x.shape[0]
         shape = (T, self.num_heads, self.head_dim)
         q, k, v = (p(x).detach().reshape(shape) for p in (self.q_proj, self.k_proj, self.v_proj))

@@ -155,3 +155,20 @@ def test_attention_ex_of_nothing_and_its_refusals():
     for zero in (0, 1):
         assert call(q=0, zero=zero) == call(qs=516, zero=zero) == call(out=0, zero=zero) == -1
     assert call(seqs=0, out=0) == -1
+
+
+def test_layer_says_that_its_scheduler_is_not_used():
+    """forward(kv_cache=) obeys the layer's scheduler; a packed batch has none of its scores and says so."""
+    import warnings
+    from types import SimpleNamespace
+
+    from memopt import DynamicAttention, MemoryScheduler
+
+    cache = SimpleNamespace(prompt=lambda q, *_: q)
+    batch, x = SimpleNamespace(whole=True), torch.randn(3, 128)
+    with torch.no_grad():
+        with pytest.warns(RuntimeWarning, match="scheduler"):
+            DynamicAttention(128, 2, scheduler=MemoryScheduler()).forward_packed(x, cache, batch, 3)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            DynamicAttention(128, 2).forward_packed(x, cache, batch, 3)
