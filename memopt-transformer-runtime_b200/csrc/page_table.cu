@@ -84,7 +84,7 @@ __device__ __forceinline__ Batch carve(uint8_t* smem, int B) {
   return t;
 }
 
-size_t batch_smem(int B, int R) {
+constexpr size_t batch_smem(int B, int R) {
   return (static_cast<size_t>(5) * B + 2) * 4 + static_cast<size_t>((R + 31) / 32) * 4;
 }
 
@@ -452,7 +452,12 @@ int launch_pages(K small, K large, const char* what, const PageArgs& a, cudaStre
   const K kern = a.B > 256 ? large : small;
   const size_t smem = batch_smem(a.B, a.R);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // The most that any call needs, so that a call on another host thread does not
+    // lower this one's limit before its launch.
+    constexpr size_t kMost = batch_smem(kMaxBatch, kMaxRows);
+    static_assert(kMost <= 227 * 1024, "shared memory");
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMost));
     if (e != cudaSuccess) return cuda_fail(e, what);
   }
   const int64_t per_cta = threads * kTokensPerThread, rows = threads / 32;

@@ -470,3 +470,38 @@ def test_inputs_that_require_a_gradient_are_refused(rotary):
         y = layer.forward_packed(x[:1].detach(), cache, step)
     y.float().sum().backward()
     assert layer.out_proj.weight.grad is not None and layer.q_proj.weight.grad is None
+
+
+# ---- page tables: calls at once, arguments of every kind -----------------------------
+def test_page_calls_of_two_host_threads():
+    """Batches of different sizes from two threads: neither lowers the shared
+    memory that the other's launch asks for."""
+    lib, bad = capi.lib(), []
+
+    def work(B, calls):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            i32 = dict(dtype=torch.int32, device=DEV)
+            tables, lens = torch.full((B, 1), -1, **i32), torch.zeros(B, **i32)
+            ring, state = torch.arange(B, **i32), torch.tensor([0, B, 0, 0], **i32)
+            rows, one = torch.arange(B, **i32), torch.ones(B, **i32)
+            out = [torch.empty(B + 4, **i32) for _ in range(3)] + [torch.empty(B, 1, **i32), torch.empty(B, **i32)]
+            p, s = capi.ptr, capi.stream()
+            I, I64 = ctypes.c_int, ctypes.c_int64
+            for _ in range(calls):
+                st = lib.memopt_reserve_slots(p(tables), p(lens), I(B), I(1), p(ring), I(B), p(state), p(rows), p(one),
+                                              I(B), I(16), I64(B), *(p(t) for t in out), s)
+                st2 = lib.memopt_truncate_rows(p(tables), p(lens), I(B), I(1), p(ring), I(B), p(state), p(rows),
+                                               capi.P(0), I(B), I(16), s)
+                if st or st2:
+                    bad.append((B, st, st2))
+                    return
+            torch.cuda.current_stream().synchronize()
+            if state.tolist()[1:] != [B, 0, 0]:
+                bad.append((B, state.tolist()))
+
+    threads = [threading.Thread(target=work, args=a) for a in ((8192, 4000), (4000, 4000), (6000, 4000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
