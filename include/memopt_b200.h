@@ -388,6 +388,7 @@ int memopt_paged_attention_int4(const void* query, const uint8_t* kv_pages,
 /* [num_blocks] is a ring of free pages; pool_state int32 [4] = index of the  */
 /* oldest free page, number of free pages, status bits, internal (0).  A new  */
 /* state has every page in the ring, lengths 0 and state {0, num_blocks, 0, 0}. */
+/* What a call updates or writes must not overlap anything else it is given.   */
 /* The calls are asynchronous; a call that cannot be done changes nothing but  */
 /* the status word, where it sets (and keeps) the bits that say why:          */
 #define MEMOPT_PAGES_EXHAUSTED   1  /* more new pages than free ones           */
@@ -428,8 +429,7 @@ int memopt_reserve_rows(int32_t* block_tables, int32_t* context_lens, int32_t* p
                         const int32_t* rows, const int32_t* new_lens, int batch, int block_size, int64_t max_tokens,
                         int replace, int32_t* cu_seqlens, int32_t* slot_mapping, int32_t* positions,
                         int32_t* batch_tables, int32_t* batch_lens, int32_t* attend_lens, void* stream);
-/* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none;    */
-/* keep_lens, like new_lens above, must not overlap context_lens);            */
+/* Cuts table row rows[b] to its first keep_lens[b] tokens (NULL: to none);   */
 /* the pages behind them go to the ring's end in row and page order and their */
 /* table entries become -1.  With freed page lists as block_tables, their     */
 /* counts as context_lens and block_size 1 it returns those pages.            */

@@ -30,6 +30,7 @@ void int32_inplace(const torch::Tensor& t, const char* who, const char* name, in
 // The bytes that a tensor spans, and whether two such spans meet.
 struct Span {
   const char *begin = nullptr, *end = nullptr;
+  Span() = default;
   explicit Span(const torch::Tensor& t) {
     const auto sizes = t.sizes(), strides = t.strides();
     int64_t last = 0;
@@ -91,9 +92,11 @@ void packed_check(const torch::Tensor& t, const char* who, const char* name, con
 struct PageTensors {
   int R, MB, NB, B;
 };
+// What a call updates meets nothing else that it takes: lens are the new or kept
+// lengths, offsets the position offsets (null: none).
 PageTensors page_checks(const char* who, const torch::Tensor& block_tables, const torch::Tensor& context_lens,
-                        const torch::Tensor& free_pages, const torch::Tensor& pool_state, const torch::Tensor& rows,
-                        int block_size) {
+                        const torch::Tensor* offsets, const torch::Tensor& free_pages, const torch::Tensor& pool_state,
+                        const torch::Tensor& rows, const torch::Tensor* lens, int block_size) {
   TORCH_CHECK(block_tables.is_cuda(), who, ": block_tables must be a CUDA tensor");
   const auto dev = block_tables.device();
   int32_inplace(block_tables, who, "block_tables", 2, dev);
@@ -104,8 +107,18 @@ PageTensors page_checks(const char* who, const torch::Tensor& block_tables, cons
   TORCH_CHECK(context_lens.size(0) == block_tables.size(0), who, ": context_lens length != block_tables rows");
   TORCH_CHECK(pool_state.size(0) == 4, who, ": pool_state must hold 4 values (head, count, status, ticket)");
   TORCH_CHECK(block_size > 0, who, ": block_size must be > 0");
-  TORCH_CHECK(!overlap(rows, block_tables) && !overlap(rows, context_lens), who,
-              ": rows must not overlap what the call updates");
+  if (offsets) {
+    int32_inplace(*offsets, who, "position_offsets", 1, dev);
+    TORCH_CHECK(offsets->size(0) == block_tables.size(0), who, ": position_offsets length != block_tables rows");
+  }
+  TORCH_CHECK(!lens || lens->size(0) == rows.size(0), who, ": new_lens / keep_lens length != rows length");
+  const Span none;
+  const Span all[] = {Span(block_tables), Span(context_lens), Span(free_pages), Span(pool_state),
+                      offsets ? Span(*offsets) : none, Span(rows), lens ? Span(*lens) : none};
+  constexpr int kUpdated = 5, kAll = 7;
+  for (int i = 0; i < kUpdated; ++i)
+    for (int j = i + 1; j < kAll; ++j)
+      TORCH_CHECK(!all[i].meets(all[j]), who, ": tensors that the call updates must not overlap the others");
   return {to_int(block_tables.size(0), who, "table rows"), to_int(block_tables.size(1), who, "table width"),
           to_int(free_pages.size(0), who, "number of pages"), to_int(rows.size(0), who, "batch")};
 }
@@ -118,17 +131,10 @@ std::vector<torch::Tensor> reserve(const char* who, torch::Tensor block_tables, 
                                    const torch::Tensor* position_offsets, torch::Tensor free_pages,
                                    torch::Tensor pool_state, torch::Tensor rows, torch::Tensor new_lens, int block_size,
                                    int64_t max_tokens, bool replace) {
-  const PageTensors n = page_checks(who, block_tables, context_lens, free_pages, pool_state, rows, block_size);
   int32_cuda(new_lens, who, "new_lens", 1, block_tables.device());
-  TORCH_CHECK(new_lens.size(0) == n.B, who, ": new_lens length != rows length");
-  TORCH_CHECK(!overlap(new_lens, context_lens), who, ": new_lens must not overlap context_lens");
+  const PageTensors n = page_checks(who, block_tables, context_lens, position_offsets, free_pages, pool_state, rows,
+                                    &new_lens, block_size);
   TORCH_CHECK(max_tokens >= 0 && max_tokens <= 0x7fffffff, who, ": max_tokens out of range");
-  if (position_offsets) {
-    int32_inplace(*position_offsets, who, "position_offsets", 1, block_tables.device());
-    TORCH_CHECK(position_offsets->size(0) == n.R, who, ": position_offsets length != block_tables rows");
-    for (const auto* t : {&block_tables, &context_lens, &free_pages, &pool_state, &rows, &new_lens})
-      TORCH_CHECK(!overlap(*position_offsets, *t), who, ": position_offsets must not overlap the other tensors");
-  }
   rows = rows.contiguous();
   new_lens = new_lens.contiguous();
   const at::cuda::CUDAGuard g(block_tables.device());
@@ -179,14 +185,11 @@ void truncate_rows(torch::Tensor block_tables, torch::Tensor context_lens, torch
                    torch::Tensor pool_state, torch::Tensor rows, c10::optional<torch::Tensor> keep_lens,
                    int block_size) {
   const char* who = "truncate_rows";
-  const PageTensors n = page_checks(who, block_tables, context_lens, free_pages, pool_state, rows, block_size);
+  if (keep_lens.has_value()) int32_cuda(*keep_lens, who, "keep_lens", 1, block_tables.device());
+  const PageTensors n = page_checks(who, block_tables, context_lens, nullptr, free_pages, pool_state, rows,
+                                    keep_lens.has_value() ? &*keep_lens : nullptr, block_size);
   torch::Tensor keep;
-  if (keep_lens.has_value()) {
-    int32_cuda(*keep_lens, who, "keep_lens", 1, block_tables.device());
-    TORCH_CHECK(keep_lens->size(0) == n.B, who, ": keep_lens length != rows length");
-    TORCH_CHECK(!overlap(*keep_lens, context_lens), who, ": keep_lens must not overlap context_lens");
-    keep = keep_lens->contiguous();
-  }
+  if (keep_lens.has_value()) keep = keep_lens->contiguous();
   rows = rows.contiguous();
   const at::cuda::CUDAGuard g(block_tables.device());
   check(memopt_truncate_rows(block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(), n.R, n.MB,

@@ -505,3 +505,34 @@ def test_page_calls_of_two_host_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_page_tensors_that_overlap_are_refused():
+    """What a call updates must not be what it reads: each pair is refused."""
+    i32 = dict(dtype=torch.int32, device=DEV)
+    names = ("block_tables", "context_lens", "free_pages", "pool_state", "rows", "lens")
+
+    def args():
+        return {"block_tables": torch.full((4, 4), -1, **i32), "context_lens": torch.zeros(4, **i32),
+                "free_pages": torch.arange(8, **i32), "pool_state": torch.tensor([0, 8, 0, 0], **i32),
+                "rows": torch.arange(4, **i32), "lens": torch.zeros(4, **i32)}
+
+    def call(a):
+        C().reserve_slots(*(a[n] for n in names), 16, 4)
+        C().truncate_rows(*(a[n] for n in names), 16)
+
+    call(args())
+    a = args()
+    a["lens"] = a["rows"] = torch.zeros(4, **i32)  # both are only read (and refused on the device: a row twice)
+    call(a)
+    for i, one in enumerate(names):
+        for two in names[i + 1:]:
+            if (one, two) == ("rows", "lens"):
+                continue
+            buf, a = torch.zeros(40, **i32), args()
+            a[one] = buf[: a[one].numel()].view(a[one].shape)
+            a[two] = buf[a[one].numel() - 1:][: a[two].numel()].view(a[two].shape)  # one value in common
+            for f, n in ((C().reserve_slots, (16, 4)), (C().truncate_rows, (16,))):
+                with pytest.raises(RuntimeError, match="overlap"):
+                    f(*(a[x] for x in names), *n)
+            assert not buf.any()
