@@ -89,10 +89,19 @@ class DevicePageTable:
         self.pool_state = torch.tensor([0, len(ring), 0, 0], dtype=torch.int32, device=self.device)
 
     def ints(self, values: Ints) -> torch.Tensor:
-        """Whole numbers as an int32 tensor on the table's device."""
-        if isinstance(values, torch.Tensor):
-            return values.to(device=self.device, dtype=torch.int32)
-        return torch.tensor(list(values), dtype=torch.int32, device=self.device)
+        """Whole numbers as an int32 tensor on the table's device.  Those of
+        the host are copied from pinned memory, so the call does not wait for
+        the stream; a graph would replay the copy of what is no longer there,
+        so they are refused during a capture."""
+        given = isinstance(values, torch.Tensor)
+        pin = self.device.type == "cuda" and not (given and values.is_cuda)
+        if pin and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("DevicePageTable: a captured call takes its rows and lengths as tensors of the GPU")
+        if not given:
+            values = torch.tensor(list(values), dtype=torch.int32, pin_memory=pin)
+        elif pin:
+            values = values.to(torch.int32).pin_memory()
+        return values.to(device=self.device, dtype=torch.int32, non_blocking=True)
 
     def reserve(self, rows: Ints, new_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:
         """Appends ``new_lens[b]`` tokens to row ``rows[b]``.  ``max_tokens``

@@ -536,3 +536,44 @@ def test_page_tensors_that_overlap_are_refused():
                 with pytest.raises(RuntimeError, match="overlap"):
                     f(*(a[x] for x in names), *n)
             assert not buf.any()
+
+
+def test_lists_do_not_wait_for_the_stream():
+    """Rows and lengths given as Python numbers or as tensors of the host."""
+    from memopt import PackedKVCache
+
+    cache = PackedKVCache(20, 2, 64, 16, max_seqs=3, max_seq_len=96)
+    long = torch.tensor([3, 4])
+    cache.admit([0, 1], [3, 4])  # warm-up
+    cache.table.truncate(long - 3, long - 3)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(1_000_000_000)  # half a second
+    batches = [cache.admit([0, 1], [3, 4])] + [cache.extend([i % 3, (i + 1) % 3], 1 + i % 2) for i in range(6)]
+    cache.table.truncate([0, 2], [2, 1])
+    cache.table.reserve(long - 3, long, 7)
+    cache.finish([1])
+    done.record()
+    assert not done.query()
+    torch.cuda.synchronize()
+    cache.table.check()
+    assert batches[0].positions.tolist() == [0, 1, 2, 0, 1, 2, 3]
+    assert cache.table.context_lens.tolist() == [5, 0, 1]
+
+
+def test_numbers_of_the_host_cannot_be_captured():
+    """A graph would replay what the list held once: refused, tensors of the GPU are the way."""
+    from memopt import DevicePageTable
+
+    table = DevicePageTable(20, 16, 3, 96)
+    rows, one = (torch.arange(2, dtype=torch.int32, device=DEV) + i for i in (0, 1))
+    host, graph = rows.long().cpu(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: table.reserve([0, 1], one, 3), lambda: table.reserve(rows, [1, 2]),
+                     lambda: table.truncate([0]), lambda: table.reserve(host, one, 3)):
+            with pytest.raises(RuntimeError, match="tensors of the GPU"):
+                call()
+        table.reserve(rows, one.long(), 3)
+    graph.replay()
+    assert table.context_lens.tolist() == [1, 2, 0]
+    table.check()
