@@ -43,6 +43,7 @@ _STATUS = (
 )
 
 Ints = Union[torch.Tensor, Sequence[int]]
+_WHOLE = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
 @dataclass
@@ -89,7 +90,8 @@ class DevicePageTable:
         self.pool_state = torch.tensor([0, len(ring), 0, 0], dtype=torch.int32, device=self.device)
 
     def ints(self, values: Ints) -> torch.Tensor:
-        """Whole numbers as an int32 tensor on the table's device.  Those of
+        """Whole numbers as an int32 tensor on the table's device; what passes
+        32 bits stays out of any range and is refused there.  Those of
         the host are copied from pinned memory, so the call does not wait for
         the stream; a graph would replay the copy of what is no longer there,
         so they are refused during a capture."""
@@ -99,7 +101,11 @@ class DevicePageTable:
             raise RuntimeError("DevicePageTable: a captured call takes its rows and lengths as tensors of the GPU")
         if not given:
             values = torch.tensor(list(values), dtype=torch.int32, pin_memory=pin)
-        elif pin:
+        elif values.dtype not in _WHOLE:
+            raise TypeError(f"DevicePageTable: rows and lengths are whole numbers, not {values.dtype}")
+        elif values.dtype == torch.int64:
+            values = values.clamp(-(1 << 31), (1 << 31) - 1)
+        if given and pin:
             values = values.to(torch.int32).pin_memory()
         return values.to(device=self.device, dtype=torch.int32, non_blocking=True)
 

@@ -577,3 +577,28 @@ def test_numbers_of_the_host_cannot_be_captured():
     graph.replay()
     assert table.context_lens.tolist() == [1, 2, 0]
     table.check()
+
+
+def test_whole_numbers_past_32_bits_are_refused():
+    """They are not cut to 32 bits, which would make another row of them."""
+    from memopt import DevicePageTable
+
+    table = DevicePageTable(20, 16, 3, 96)
+    far = 2 ** 32
+    for dev in (DEV, "cpu"):
+        t = lambda *values: torch.tensor(values, device=dev)
+        for call in (lambda: table.reserve(t(far), t(1), 1), lambda: table.reserve(t(0), t(far + 1), 9),
+                     lambda: table.reserve(t(0), t(-far + 1), 9), lambda: table.truncate(t(far + 1)),
+                     lambda: table.truncate(t(0), t(far))):
+            call()
+            with pytest.raises(RuntimeError):
+                table.check()
+            assert table.context_lens.tolist() == [0, 0, 0] and table.free_count() == 20
+    for bad in (torch.tensor([1.0], device=DEV), torch.tensor([1.5]), torch.tensor([True], device=DEV)):
+        with pytest.raises(TypeError, match="whole numbers"):
+            table.reserve(bad, [1])
+        with pytest.raises(TypeError, match="whole numbers"):
+            table.truncate([0], bad)
+    table.reserve(torch.tensor([2], dtype=torch.uint8, device=DEV), torch.tensor([3], dtype=torch.int16), 3)
+    table.check()
+    assert table.context_lens.tolist() == [0, 0, 3]
