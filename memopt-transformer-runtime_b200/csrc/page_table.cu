@@ -88,8 +88,13 @@ constexpr size_t batch_smem(int B, int R) {
   return (static_cast<size_t>(5) * B + 2) * 4 + static_cast<size_t>((R + 31) / 32) * 4;
 }
 
-__device__ __forceinline__ int over_bs(int x, const PageArgs& a) { return a.shift >= 0 ? x >> a.shift : x / a.BS; }
-__device__ __forceinline__ int pages_of(int tokens, const PageArgs& a) { return over_bs(tokens + a.BS - 1, a); }
+// x >= 0; unsigned, as a length and a block size may add up to more than 2^31.
+__device__ __forceinline__ int over_bs(uint32_t x, const PageArgs& a) {
+  return static_cast<int>(a.shift >= 0 ? x >> a.shift : x / static_cast<uint32_t>(a.BS));
+}
+__device__ __forceinline__ int pages_of(int tokens, const PageArgs& a) {
+  return over_bs(static_cast<uint32_t>(tokens) + a.BS - 1, a);
+}
 
 // Reads the batch, checks it and scans it.  Returns the status bits of the
 // refusal (0: accepted), the same in every thread.  total_tokens and
@@ -432,6 +437,8 @@ int check_pages(const char* who, const PageArgs& a) {
   if (a.R > kMaxRows) return fail(MEMOPT_ERR_UNSUPPORTED, w + ": more than 262144 table rows");
   if (static_cast<int64_t>(a.NB) * a.BS > 0x7fffffffLL || static_cast<int64_t>(a.MB) * a.BS > 0x7fffffffLL)
     return fail(MEMOPT_ERR_UNSUPPORTED, w + ": slots past 2^31 (the slot mapping is int32)");
+  if (a.MB > 0x7fffffff - 1024)  // a lane's index of an entry runs up to 32 * kInFlight past the row
+    return fail(MEMOPT_ERR_UNSUPPORTED, w + ": a block table row near 2^31 entries");
   if (a.max_tokens > 0x7fffffffLL) return fail(MEMOPT_ERR_UNSUPPORTED, w + ": max_tokens past 2^31");
   if (!a.tables || !a.lens || !a.ring || !a.state || (a.B > 0 && !a.rows))
     return fail(MEMOPT_ERR_INVALID_ARG, w + ": null pointer");

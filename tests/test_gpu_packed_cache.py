@@ -602,3 +602,17 @@ def test_whole_numbers_past_32_bits_are_refused():
     table.reserve(torch.tensor([2], dtype=torch.uint8, device=DEV), torch.tensor([3], dtype=torch.int16), 3)
     table.check()
     assert table.context_lens.tolist() == [0, 0, 3]
+
+
+def test_page_counts_of_very_large_blocks():
+    """Lengths and block sizes whose sum passes 2^31 still count their pages."""
+    i32 = dict(dtype=torch.int32, device=DEV)
+    for bs in (1_500_000_000, 1 << 30):
+        tables, lens, ring = torch.zeros(1, 1, **i32), torch.tensor([1_000_000_000], **i32), torch.full((1,), -1, **i32)
+        state, row = torch.tensor([0, 0, 0, 0], **i32), torch.zeros(1, **i32)
+        C().truncate_rows(tables, lens, ring, state, row, torch.tensor([5], **i32), bs)
+        assert state.tolist() == [0, 0, 0, 0] and lens.tolist() == [5] and tables.tolist() == [[0]]
+        cu, slots, pos, bt, bl = C().reserve_slots(tables, lens, ring, state, row, torch.tensor([3], **i32), bs, 3)
+        assert slots.tolist() == pos.tolist() == [5, 6, 7] and bl.tolist() == [8]
+        C().truncate_rows(tables, lens, ring, state, row, None, bs)
+        assert state.tolist() == [0, 1, 0, 0] and ring.tolist() == [0] and tables.tolist() == [[-1]]

@@ -172,3 +172,12 @@ def test_layer_says_that_its_scheduler_is_not_used():
         with warnings.catch_warnings():
             warnings.simplefilter("error")
             DynamicAttention(128, 2).forward_packed(x, cache, batch, 3)
+
+
+@pytest.mark.parametrize("MB", [2 ** 31 - 1, 2 ** 31 - 1024])
+def test_tables_near_2_to_the_31_are_refused(MB):
+    """A lane's index of an entry runs up to 256 past the row's end."""
+    assert reserve_rows(MB=MB, BS=1) == -3
+    lib = capi.lib()
+    assert lib.memopt_truncate_rows(P(SOME), P(SOME), I(4), I(MB), P(SOME), I(32), P(SOME), P(SOME), P(0), I(2), I(1),
+                                    P(0)) == -3
