@@ -106,7 +106,9 @@ class DevicePageTable:
         elif values.dtype == torch.int64:
             values = values.clamp(-(1 << 31), (1 << 31) - 1)
         if given and pin:
-            values = values.to(torch.int32).pin_memory()
+            values = values.to(torch.int32)
+            # pin_memory gives pinned memory back as it is, and the caller may write there after the call
+            values = (values.clone() if values.is_pinned() else values).pin_memory()
         return values.to(device=self.device, dtype=torch.int32, non_blocking=True)
 
     def reserve(self, rows: Ints, new_lens: Ints, max_tokens: Optional[int] = None) -> PackedBatch:

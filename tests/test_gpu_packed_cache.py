@@ -616,3 +616,22 @@ def test_page_counts_of_very_large_blocks():
         assert slots.tolist() == pos.tolist() == [5, 6, 7] and bl.tolist() == [8]
         C().truncate_rows(tables, lens, ring, state, row, None, bs)
         assert state.tolist() == [0, 1, 0, 0] and ring.tolist() == [0] and tables.tolist() == [[-1]]
+
+
+def test_pinned_numbers_may_change_after_the_call():
+    """The copy is taken within the call, whatever memory the numbers lie in."""
+    from memopt import DevicePageTable
+
+    for dtype in (torch.int32, torch.int64, torch.int16):
+        table = DevicePageTable(20, 16, 3, 96)
+        rows, lens = (torch.tensor(x, dtype=dtype).pin_memory() for x in ([0, 2], [5, 20]))
+        table.reserve(rows, lens, 25)  # warm-up
+        table.truncate(rows)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(300_000_000)
+        batch = table.reserve(rows, lens, 25)
+        rows.fill_(1)
+        lens.fill_(3)
+        assert batch.context_lens.tolist() == [5, 20] and batch.rows.tolist() == [0, 2]
+        table.check()
+        assert table.context_lens.tolist() == [5, 0, 20]
