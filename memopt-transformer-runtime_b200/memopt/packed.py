@@ -395,8 +395,10 @@ class PackedKVCache:
         self._need_pool()
         t = self.table
         before = t.context_lens.clone()
-        kept, count, freed, freed_count = self._C.evict_topk_compact(scores, t.block_tables, t.context_lens,
-                                                                     float(retain_ratio), int(num_sink_tokens))
-        t.position_offsets += before - t.context_lens
+        try:
+            kept, count, freed, freed_count = self._C.evict_topk_compact(scores, t.block_tables, t.context_lens,
+                                                                         float(retain_ratio), int(num_sink_tokens))
+        finally:  # a failed one may have shrunk the lengths too
+            t.position_offsets += before - t.context_lens
         t.release_pages(freed, freed_count)
         return kept, count

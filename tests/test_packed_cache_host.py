@@ -181,3 +181,17 @@ def test_tables_near_2_to_the_31_are_refused(MB):
     lib = capi.lib()
     assert lib.memopt_truncate_rows(P(SOME), P(SOME), I(4), I(MB), P(SOME), I(32), P(SOME), P(SOME), P(0), I(2), I(1),
                                     P(0)) == -3
+
+
+def test_an_eviction_that_fails_keeps_the_positions(pool):
+    """A row move that ran out of time leaves the lengths shrunk: the positions still go on from the true length."""
+    def shrink_and_fail(scores, tables, lens, ratio, sinks):
+        lens.copy_(torch.tensor([3, 0], dtype=torch.int32))
+        raise RuntimeError("a bounded device wait ran out")
+
+    cache = cache_of(8)
+    cache.table.context_lens.copy_(torch.tensor([9, 4], dtype=torch.int32))
+    pool.evict_topk_compact = shrink_and_fail
+    with pytest.raises(RuntimeError, match="bounded"):
+        cache.evict(torch.zeros(2, 2, 9), 0.5)
+    assert (cache.table.position_offsets + cache.table.context_lens).tolist() == [9, 4]
