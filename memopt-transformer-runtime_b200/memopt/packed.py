@@ -56,8 +56,8 @@ class PackedBatch:
     positions: torch.Tensor     # [max_tokens] position of each new token in its sequence, evicted tokens counted
     block_tables: torch.Tensor  # [B, max_blocks_per_seq]
     context_lens: torch.Tensor  # [B] lengths with the new tokens
-    attend_lens: torch.Tensor   # [B] the same, 0 if the batch was refused
     whole: bool = False         # the new tokens are the whole sequences
+    attend_lens: Optional[torch.Tensor] = None  # [B] context_lens, 0 if the batch was refused
 
 
 class DevicePageTable:
@@ -133,7 +133,7 @@ class DevicePageTable:
         cu, slots, pos, tables, lens, attend = self._C.reserve_rows(
             self.block_tables, self.context_lens, self.position_offsets, self.free_pages, self.pool_state, r,
             self.ints(new_lens), self.block_size, max_tokens, replace)
-        return PackedBatch(r, cu, slots, pos, tables, lens, attend)
+        return PackedBatch(r, cu, slots, pos, tables, lens, attend_lens=attend)
 
     def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
         """Cuts each row to its first ``keep_lens`` tokens (None: to nothing)
@@ -377,13 +377,13 @@ class PackedKVCache:
         q4 = q.to(torch.float16).contiguous().reshape(B, q.shape[0] // B, q.shape[1], q.shape[2])
         reach = batch.block_tables.shape[1] * self.block_size
         window = reach if window_size <= 0 else window_size
+        lens = batch.context_lens if batch.attend_lens is None else batch.attend_lens
         if self.kv_format == "int4":
-            out = self._C.dynamic_sparse_attention_int4(q4, self._C.get_int4_pages(), batch.block_tables,
-                                                        batch.attend_lens, reach, window, True)
+            out = self._C.dynamic_sparse_attention_int4(q4, self._C.get_int4_pages(), batch.block_tables, lens,
+                                                        reach, window, True)
         else:
             kc, vc = self._C.get_pool_tensors()
-            out = self._C.dynamic_sparse_attention(q4, kc, vc, batch.block_tables, batch.attend_lens, reach, window,
-                                                   True)
+            out = self._C.dynamic_sparse_attention(q4, kc, vc, batch.block_tables, lens, reach, window, True)
         return out.reshape(q.shape)
 
     def evict(self, scores: torch.Tensor, retain_ratio: float, num_sink_tokens: int = 4):

@@ -195,3 +195,12 @@ def test_an_eviction_that_fails_keeps_the_positions(pool):
     with pytest.raises(RuntimeError, match="bounded"):
         cache.evict(torch.zeros(2, 2, 9), 0.5)
     assert (cache.table.position_offsets + cache.table.context_lens).tolist() == [9, 4]
+
+
+def test_packed_batch_of_six_tensors():
+    from memopt import PackedBatch
+
+    t = torch.zeros(2, dtype=torch.int32)
+    for whole in ((), (True,)):
+        batch = PackedBatch(t, t, t, t, t, t, *whole)
+        assert batch.whole == bool(whole) and batch.attend_lens is None
