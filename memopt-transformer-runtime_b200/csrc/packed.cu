@@ -323,6 +323,19 @@ __device__ __noinline__ void row_by_row(const Params& p, int64_t row, int h, int
   }
 }
 
+// Index i's share of the rows behind the last sequence, which end at row `rest`.
+// Every index of the grid passes through one scheduler or another once, so this
+// costs no launch (and out of line no instructions where there are no such rows).
+template <typename T, int D>
+__device__ __noinline__ void zero_share(const Params& p, int rest, uint32_t i) {
+  rest = max(rest, 0);
+  const int64_t share = (static_cast<int64_t>(p.T - rest) + gridDim.x - 1) / gridDim.x, first = rest + i * share;
+  if (first >= p.T) return;
+  const int64_t row = static_cast<int64_t>(p.H) * D, n = min(share, p.T - first) * row / 8;
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + first * row);
+  for (int64_t e = threadIdx.x & 31; e < n; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+}
+
 // Barriers: items (2 slots: filled by the scheduler, read by the warps that
 // work on it), Q (filled by TMA, free by commit), K/V ring, and per tile: scores
 // ready (commit), first and second part of P ready (4 warps), P.V done
@@ -931,18 +944,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         i = cta;
         return got;
       };
-      // Index i's share of the rows behind the last sequence.  Every index of the grid
-      // passes here once, in one CTA or another, so this costs no launch.
-      const int rest = p.zero_rest ? min(max(cu[p.S], 0), p.T) : p.T;
-      const int share = rest < p.T ? static_cast<int>((static_cast<int64_t>(p.T - rest) + gridDim.x - 1) / gridDim.x) : 0;
-      auto zero_share = [&] {
-        const int64_t first = rest + static_cast<int64_t>(i) * share;
-        if (share == 0 || first >= p.T) return;
-        const int64_t row = static_cast<int64_t>(p.H) * D;
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + first * row);
-        const int64_t n = min(static_cast<int64_t>(share), p.T - first) * row / 8;
-        for (int64_t e = lane; e < n; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
-      };
+      const bool zero = p.zero_rest && cu[p.S] < p.T;  // there are rows behind the last sequence
       // The item of index i; false when there is none.  The items are those of the
       // indexes below `end` (split: an upper bound that every miss lowers).
       uint32_t end = SPLIT ? 0xffffffffu : total;
@@ -1043,7 +1045,7 @@ packed_attention_kernel(const __grid_constant__ Params p, const __grid_constant_
         }
         Item it{0, -1, 0, 0, 0, 0}, got = it;
         while (more) {
-          zero_share();
+          if (zero) zero_share<T, D>(p, cu[p.S], i);
           bool has = find(got);
           if (SPLIT && has) {  // not a piece that this token block does not have
             const Range r = item_range<TILES, SPLIT>(p, got, 0);

@@ -99,7 +99,7 @@ __device__ __forceinline__ int pages_of(int tokens, const PageArgs& a) {
 // Reads the batch, checks it and scans it.  Returns the status bits of the
 // refusal (0: accepted), the same in every thread.  total_tokens and
 // total_pages are the sums (64-bit: refused sums may exceed an int).
-template <int kThreads, bool kReserve>
+template <int kThreads, bool kReserve, bool kRows>
 __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total_tokens, int64_t& total_pages) {
   __shared__ uint32_t s_status;
   constexpr int kWarps = kThreads / 32;
@@ -122,7 +122,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
       } else {
         if (atomicOr(&t.seen[row >> 5], 1u << (row & 31)) & (1u << (row & 31))) bits |= MEMOPT_PAGES_BAD_ROW;
         old = a.lens[row];
-        if (kReserve && a.offsets) off = a.offsets[row];
+        if (kReserve && kRows) off = a.offsets[row];
         if (old < 0 || old > cap) {
           bits |= MEMOPT_PAGES_CORRUPT;
           old = 0;
@@ -133,7 +133,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
         bits |= MEMOPT_PAGES_BAD_LENGTH;
         n = 0;
       }
-      if (kReserve && a.fresh && old > 0) {
+      if (kReserve && kRows && a.fresh && old > 0) {
         bits |= kNotCut;
         n = 0;
       }
@@ -148,7 +148,7 @@ __device__ uint32_t scan_batch(const PageArgs& a, const Batch& t, int64_t& total
       }
       t.row[b] = row;
       t.old[b] = old;
-      t.off[b] = old > 0 ? off : 0;
+      if (kReserve && kRows) t.off[b] = old > 0 ? off : 0;
     }
     // Block-wide exclusive scan of (n, p): within the warp, then over the warps.
     int64_t sn = n, sp = p;
@@ -214,7 +214,10 @@ __device__ bool arrive_last(int32_t* ticket) {
   return s_last != 0;
 }
 
-template <int kThreads>
+// kRows: with position offsets, lengths to attend over and perhaps rows that begin
+// anew (reserve_rows).  In kernels of their own, as is truncate with a next batch
+// (kNext): code that a short kernel fetches and does not use costs it 0.2 to 0.5 us.
+template <int kThreads, bool kRows>
 __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
   constexpr int kWarps = kThreads / 32;
   extern __shared__ uint8_t smem[];
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
   after_previous();
   const int head = a.state[0], count = a.state[1];
   int64_t tokens, pages;
-  uint32_t status = scan_batch<kThreads, true>(a, t, tokens, pages);
+  uint32_t status = scan_batch<kThreads, true, kRows>(a, t, tokens, pages);
   if (head < 0 || head >= a.NB || count < 0 || count > a.NB) status |= MEMOPT_PAGES_CORRUPT;
   if (status == 0 && pages > count) status |= MEMOPT_PAGES_EXHAUSTED;
   const bool taken = status == 0;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
           page = at < had ? a.tables[static_cast<int64_t>(t.row[b]) * a.MB + at] : ring_at(t.page[b] + at - had);
           page_at = at;
         }
-        pos[k] = p + t.off[b];
+        pos[k] = kRows ? p + t.off[b] : p;
         if (page >= 0 && page < a.NB) slot[k] = page * a.BS + (p - at * a.BS);
         else bits |= MEMOPT_PAGES_CORRUPT;
       }
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
     if (lane == 0) {
       const int len = bad ? 0 : t.old[b] + (taken ? t.cu[b + 1] - t.cu[b] : 0);
       a.out_lens[b] = len;
-      if (a.attend_lens) a.attend_lens[b] = taken ? len : 0;
+      if (kRows) a.attend_lens[b] = taken ? len : 0;
     }
   }
   for (int i = blockIdx.x * kThreads + tid; i <= a.B; i += gridDim.x * kThreads) a.cu[i] = taken ? t.cu[i] : 0;
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
     if (taken) {
       for (int b = tid; b < a.B; b += kThreads) {
         a.lens[t.row[b]] = t.old[b] + (t.cu[b + 1] - t.cu[b]);
-        if (a.offsets && t.old[b] == 0) a.offsets[t.row[b]] = 0;
+        if (kRows && t.old[b] == 0) a.offsets[t.row[b]] = 0;
       }
     }
     if (tid == 0) {
@@ -334,7 +337,8 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const PageArgs a) {
         a.state[0] = static_cast<int32_t>((head + pages) % a.NB);
         a.state[1] = static_cast<int32_t>(count - pages);
       }
-      if (status & ~kNotCut) atomicOr(a.state + 2, static_cast<int>(status & ~kNotCut));
+      if (kRows) status &= ~kNotCut;
+      if (status) atomicOr(a.state + 2, static_cast<int>(status));
       a.state[3] = 0;
     }
   }
@@ -374,7 +378,7 @@ __device__ uint32_t next_batch_fits(const PageArgs& a, int64_t free_pages) {
   return bits;
 }
 
-template <int kThreads>
+template <int kThreads, bool kNext>
 __global__ void __launch_bounds__(kThreads) truncate_kernel(const PageArgs a) {
   constexpr int kWarps = kThreads / 32;
   extern __shared__ uint8_t smem[];
@@ -384,10 +388,10 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(const PageArgs a) {
   after_previous();
   const int head = a.state[0], count = a.state[1];
   int64_t kept, pages;
-  uint32_t status = scan_batch<kThreads, false>(a, t, kept, pages);
+  uint32_t status = scan_batch<kThreads, false, false>(a, t, kept, pages);
   if (head < 0 || head >= a.NB || count < 0 || count > a.NB || (status == 0 && count + pages > a.NB))
     status |= MEMOPT_PAGES_CORRUPT;
-  if (a.next) status |= next_batch_fits<kThreads>(a, count + pages);
+  if (kNext) status |= next_batch_fits<kThreads>(a, count + pages);
   uint32_t bits = 0;
   if (status == 0) {
     const int nwarps = gridDim.x * kWarps;
@@ -487,10 +491,11 @@ int reserve(const char* who, PageArgs a, cudaStream_t s) {
   if (a.fresh && a.B > 0) {
     PageArgs cut = a;
     cut.amount = nullptr, cut.next = a.amount;
-    const int st2 = launch_pages(truncate_kernel<256>, truncate_kernel<1024>, "truncate_kernel launch", cut, s);
+    const int st2 = launch_pages(truncate_kernel<256, true>, truncate_kernel<1024, true>, "truncate_kernel launch", cut, s);
     if (st2 != MEMOPT_OK) return st2;
   }
-  return launch_pages(reserve_kernel<256>, reserve_kernel<1024>, "reserve_kernel launch", a, s);
+  return a.offsets ? launch_pages(reserve_kernel<256, true>, reserve_kernel<1024, true>, "reserve_kernel launch", a, s)
+                   : launch_pages(reserve_kernel<256, false>, reserve_kernel<1024, false>, "reserve_kernel launch", a, s);
 }
 
 }  // namespace
@@ -531,5 +536,5 @@ extern "C" int memopt_truncate_rows(int32_t* block_tables, int32_t* context_lens
   if (st != MEMOPT_OK) return st;
   if (batch == 0) return MEMOPT_OK;
   a.shift = log2_of(block_size);
-  return launch_pages(truncate_kernel<256>, truncate_kernel<1024>, "truncate_kernel launch", a, as_stream(stream));
+  return launch_pages(truncate_kernel<256, false>, truncate_kernel<1024, false>, "truncate_kernel launch", a, as_stream(stream));
 }

@@ -46,6 +46,12 @@ Ints = Union[torch.Tensor, Sequence[int]]
 _WHOLE = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
+def _device(device: Optional[torch.device]) -> torch.device:
+    """With its index, as tensors have it; the current CUDA device by default."""
+    dev = torch.device("cuda" if device is None else device)
+    return torch.device("cuda", torch.cuda.current_device()) if dev.type == "cuda" and dev.index is None else dev
+
+
 @dataclass
 class PackedBatch:
     """What ``reserve`` built for a batch of rows (device tensors, int32)."""
@@ -77,7 +83,7 @@ class DevicePageTable:
         self._C = memopt_C
         self.num_blocks, self.block_size, self.max_seqs = num_blocks, block_size, max_seqs
         self.max_seq_len = max_seq_len
-        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.device = _device(device)
         width = (max_seq_len + block_size - 1) // block_size
 
         def int32(value, *shape):
@@ -96,6 +102,8 @@ class DevicePageTable:
         the stream; a graph would replay the copy of what is no longer there,
         so they are refused during a capture."""
         given = isinstance(values, torch.Tensor)
+        if given and values.dtype == torch.int32 and values.device == self.device:
+            return values
         pin = self.device.type == "cuda" and not (given and values.is_cuda)
         if pin and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("DevicePageTable: a captured call takes its rows and lengths as tensors of the GPU")
@@ -273,9 +281,7 @@ class PackedKVCache:
         if rotary is not None and rotary.head_dim != head_dim:
             raise ValueError("PackedKVCache: rotary.head_dim differs from head_dim")
         self.num_heads, self.head_dim, self.block_size, self.rotary = num_heads, head_dim, block_size, rotary
-        dev = torch.device("cuda" if device is None else device)
-        if dev.type == "cuda" and dev.index is None:
-            dev = torch.device("cuda", torch.cuda.current_device())
+        dev = _device(device)
         with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():
             pages, total = _take_pages(memopt_C, num_blocks, (block_size, num_heads, head_dim, kv_format, dev))
         self._generation = memopt_C.pool_generation()
