@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import contextlib
 import gc
+import threading
 import weakref
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple, Union
@@ -221,6 +222,7 @@ class RotaryPositions:
 
 
 _caches: "weakref.WeakSet[PackedKVCache]" = weakref.WeakSet()
+_taking = threading.Lock()
 
 
 def _pool_kind(C) -> Optional[tuple]:
@@ -249,10 +251,14 @@ def _take_pages(C, num_blocks: int, kind: tuple) -> Tuple[List[int], int]:
                                f"{num_blocks} free pages of this kind; call memopt_C.init_pool with the pages of all "
                                "caches before the first one is made, or close the other one")
         C.init_pool(num_blocks, *kind[:3], kv_format=kind[3])
-        if C.free_blocks_count() < num_blocks:
-            raise RuntimeError(f"PackedKVCache: the pool has {C.free_blocks_count()} free pages, {num_blocks} are asked "
-                               "for; the others are held through allocate_block")
-    return [C.allocate_block() for _ in range(num_blocks)], _pool_kind(C)[1]
+    pages: List[int] = []
+    while len(pages) < num_blocks and (page := C.allocate_block()) >= 0:
+        pages.append(page)
+    if len(pages) < num_blocks:
+        _give_back(C, C.pool_generation(), pages)
+        raise RuntimeError(f"PackedKVCache: the pool has {len(pages)} free pages, {num_blocks} are asked for; the others "
+                           "are held through allocate_block")
+    return pages, _pool_kind(C)[1]
 
 
 def _give_back(C, generation: int, pages: List[int]) -> None:
@@ -283,11 +289,12 @@ class PackedKVCache:
         self.num_heads, self.head_dim, self.block_size, self.rotary = num_heads, head_dim, block_size, rotary
         dev = _device(device)
         with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():
-            pages, total = _take_pages(memopt_C, num_blocks, (block_size, num_heads, head_dim, kv_format, dev))
-        self._generation = memopt_C.pool_generation()
-        self._pages = weakref.finalize(self, _give_back, memopt_C, self._generation, pages)
-        self._pages.atexit = False
-        _caches.add(self)
+            with _taking:
+                pages, total = _take_pages(memopt_C, num_blocks, (block_size, num_heads, head_dim, kv_format, dev))
+                self._generation = memopt_C.pool_generation()
+                self._pages = weakref.finalize(self, _give_back, memopt_C, self._generation, pages)
+                self._pages.atexit = False
+                _caches.add(self)
         self.table = DevicePageTable(total, block_size, max_seqs, max_seq_len, dev, pages)
 
     def close(self) -> None:

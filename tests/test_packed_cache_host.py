@@ -204,3 +204,33 @@ def test_packed_batch_of_six_tensors():
     for whole in ((), (True,)):
         batch = PackedBatch(t, t, t, t, t, t, *whole)
         assert batch.whole == bool(whole) and batch.attend_lens is None
+
+
+def test_caches_made_by_several_threads(pool):
+    """Each takes its own pages; one that finds none any more leaves nothing behind."""
+    import threading
+
+    plain, taken = pool.allocate_block, []
+    pool.init_pool(40, 16, 2, 64)
+
+    def slow():
+        import time
+
+        page = plain()
+        time.sleep(1e-4)
+        return page
+
+    pool.allocate_block = slow
+    threads = [threading.Thread(target=lambda: taken.append(cache_of(10))) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(p for c in taken for p in c.table.free_pages[:10].tolist()) == list(range(40))
+    taken.clear()
+    assert sorted(pool.free) == list(range(40))
+    # Somebody else's allocate_block in between.
+    pool.allocate_block = lambda: -1 if len(pool.free) == 37 else plain()
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache_of(10)
+    assert sorted(pool.free) == list(range(40))
