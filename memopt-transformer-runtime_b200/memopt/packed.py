@@ -286,6 +286,8 @@ class PackedKVCache:
         self._C = memopt_C
         if rotary is not None and rotary.head_dim != head_dim:
             raise ValueError("PackedKVCache: rotary.head_dim differs from head_dim")
+        if num_blocks <= 0:
+            raise ValueError("PackedKVCache: num_blocks must be > 0")
         self.num_heads, self.head_dim, self.block_size, self.rotary = num_heads, head_dim, block_size, rotary
         dev = _device(device)
         with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():

@@ -234,3 +234,11 @@ def test_caches_made_by_several_threads(pool):
     with pytest.raises(RuntimeError, match="free pages"):
         cache_of(10)
     assert sorted(pool.free) == list(range(40))
+
+
+def test_a_cache_without_pages_is_refused(pool):
+    pool.init_pool(5, 16, 2, 64)
+    for n in (0, -1):
+        with pytest.raises(ValueError, match="num_blocks"):
+            cache_of(n)
+    assert pool.generation == 1 and len(pool.free) == 5
