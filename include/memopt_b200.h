@@ -390,7 +390,10 @@ int memopt_paged_attention_int4(const void* query, const uint8_t* kv_pages,
 /* state has every page in the ring, lengths 0 and state {0, num_blocks, 0, 0}. */
 /* What a call updates or writes must not overlap anything else it is given.   */
 /* The calls are asynchronous; a call that cannot be done changes nothing but  */
-/* the status word, where it sets (and keeps) the bits that say why:          */
+/* the status word, where it sets (and keeps) the bits that say why.  Only     */
+/* damaged page ids do not stop a call, as they are met while it is under way: */
+/* one outside the pool gives its tokens no slot (-1) and is passed on as it   */
+/* is, table to ring or ring to table, so that the counts stay right.          */
 #define MEMOPT_PAGES_EXHAUSTED   1  /* more new pages than free ones           */
 #define MEMOPT_PAGES_ROW_FULL    2  /* a row would exceed max_blocks_per_seq   */
 #define MEMOPT_PAGES_BAD_ROW     4  /* a row out of range, or twice in a batch */

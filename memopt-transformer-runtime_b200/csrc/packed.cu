@@ -37,7 +37,7 @@
 // only when the running maximum grows by more than 2^8 (weights stay <= 2^8 and
 // the sums fp32), which is rare.  Weights are rounded to 16 bits for P V, as its A
 // operand has to be of V's type; the row sum adds them in fp32.  Against 64 bits a
-// result is off by 9 to 32% more than with fp32 weights (fp16 2.1e-4 to 2.7e-4 over
+// result is off by 9 to 38% more than with fp32 weights (fp16 2.1e-4 to 2.9e-4 over
 // an output, bf16 2.1e-3; the rounding of the result alone 1.9e-4 and 1.65e-3).
 //
 // What bounds it: for each tile and block 1024 cycles of the tensor pipe (D = 128)
@@ -45,7 +45,8 @@
 // pair of blocks (70% of the tensor pipe); in long runs the power cap (1000 W,
 // 1.4 GHz).  148 heads x 8192 tokens, not causal: 3.82-3.94 ms = 1290-1330 TFLOP/s,
 // 0.92-0.95 of the measured sustained cuBLAS rate; 2 x 8192 causal, 32 heads:
-// 1.05 ms = 1040.  A quarter of the exponentials on the FMA pipe saves 3% of the
+// 1.02-1.08 ms = 1020-1080, of which about an eighth is the ends of its 13.8 items an
+// SM (the warps that compute weights also scale and store).  A quarter of the exponentials on the FMA pipe saves 3% of the
 // cycles and costs as much power: equal or slower by the clock, not kept.
 //
 // Masked scores are replaced, so a hidden key never matters.  A hidden value
@@ -1208,12 +1209,12 @@ Plan plan_of(int S, int64_t T, int max_seqlen, int H, int KVH, int D, int window
   const int64_t tokens = 128 >> pl.gshift;
   auto most_items = [&](int tiles) { return (T / (tokens * tiles) + S) * pl.units; };
   // Two tiles an item halve the K/V traffic and pay where the walk over the keys is
-  // long and the items are many: 2 x 8192 tokens, 32 heads 0.91 ms against 0.98 with
-  // one tile, 4 prompts up to 7696 with 4/1 heads 140 us against 162, 12 x 800 with
-  // 32/8 heads of 64 dims 82 against 92.  One tile, two CTAs to an SM, hides an item's
-  // ends better and makes twice the items: 32 x 512 tokens 128 against 132, 64 x 32
-  // 14.5 against 20.0, 12 x 800 with heads of 128 dims 98 against 106, one prompt of
-  // 1000 24 against 29.
+  // long and the items are many: 2 x 8192 tokens, 32/32 heads 1.02 ms against 1.10 with
+  // one tile, 32/8 heads 0.98 against 1.07, 12 x 800 with 32/8 heads of 64 dims 71.5
+  // against 80.8 us.  One tile, two CTAs to an SM, hides an item's ends better and makes
+  // twice the items: 32 x 512 tokens, 32/8 heads of 128 dims 114 against 118, 64 x 32
+  // 13.2 against 18.4, one prompt of 1000 20.9 against 25.7.  (Just above the border it
+  // would be the better form still: 12 x 800 of 128 dims 88 against 96.)
   pl.tiles = T >= 768LL * S && most_items(2) >= 2 * sm_count() ? 2 : 1;
   // Few rows with long walks: the longest item would go on alone, so items are split
   // into pieces of `split` key blocks.  With the longest sequence as hinted and the

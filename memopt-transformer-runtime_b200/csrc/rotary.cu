@@ -20,8 +20,8 @@
 // tokens: its warps put their first loads in flight, the threads compute the
 // (cos, sin) of the tokens' pairs once into shared memory, and every step reads
 // them there.  Small CTAs of two warps, each with one batch of loads: on 32768
-// tokens x 64 heads of 128 with the cache (1.88 GB) 297 us = 6.33 TB/s, against
-// 306 to 349 us with four or eight warps, 2 to 4 steps in flight or up to four
+// tokens x 64 heads of 128 with the cache (1.88 GB) 297 to 339 us between boards
+// (6.33 to 5.54 TB/s); on the fastest of them 297 against 306 to 349 us with four or eight warps, 2 to 4 steps in flight or up to four
 // batches a warp; holding (cos, sin) in registers for all heads of a token and a
 // grid of resident warps took 316 us (28.6 against 25.6 us on 4099 tokens).
 #include <algorithm>

@@ -68,8 +68,8 @@ class PackedBatch:
 
 
 class DevicePageTable:
-    """Block tables and free pages in device memory, one sequence per row.
-    ``pages``: those of the pool's ``num_blocks`` pages that the table may
+    """Block tables and free pages in device memory, one sequence per row of
+    up to ``max_seq_len`` tokens (rounded up to whole pages).  ``pages``: those of the pool's ``num_blocks`` pages that the table may
     hand out, in this order (all of them by default)."""
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_len: int,
@@ -146,7 +146,8 @@ class DevicePageTable:
 
     def truncate(self, rows: Ints, keep_lens: Optional[Ints] = None) -> None:
         """Cuts each row to its first ``keep_lens`` tokens (None: to nothing)
-        and gives the pages behind them back."""
+        and gives the pages behind them back.  Positions go on from there:
+        those of the tokens cut off are given out again."""
         keep = None if keep_lens is None else self.ints(keep_lens)
         self._C.truncate_rows(self.block_tables, self.context_lens, self.free_pages, self.pool_state,
                               self.ints(rows), keep, self.block_size)
@@ -276,7 +277,9 @@ class PackedKVCache:
     format) that has so many free pages is used as it is, otherwise it is
     initialised with ``num_blocks`` pages: for several caches, one per layer,
     call ``memopt_C.init_pool`` with the pages of all of them first.  While a
-    cache lives in the pool another one does not replace it."""
+    cache lives in the pool another one does not replace it.  The pool holds
+    fp16 or INT4 whatever the inputs' type: bf16 keys and values past 65504
+    are infinite there."""
 
     def __init__(self, num_blocks: int, num_heads: int, head_dim: int, block_size: int = 16, max_seqs: int = 256,
                  max_seq_len: int = 32768, kv_format: str = "fp16", rotary: Optional[RotaryPositions] = None,
@@ -367,7 +370,10 @@ class PackedKVCache:
         """Whole prompts (a batch of :meth:`admit`): rotary positions (the
         tokens' own, or ``positions`` [axes, T]), the cache write, and
         attention inside each prompt.  q [T, H, D], k and v [T, KVH, D]; rows
-        past the batch's last token, and all rows of a refused batch, are 0."""
+        past the batch's last token, and all rows of a refused batch, are 0.
+        A window is the last ``window_size`` tokens up to the row's own
+        (causal), or of the whole prompt for every row (not causal: what a
+        decode step sees, not a band around the row)."""
         if not batch.whole:
             raise ValueError("PackedKVCache.prompt: the batch must come from admit (whole sequences)")
         self._no_grad(q, k, v)
