@@ -635,3 +635,103 @@ def test_pinned_numbers_may_change_after_the_call():
         assert batch.context_lens.tolist() == [5, 20] and batch.rows.tolist() == [0, 2]
         table.check()
         assert table.context_lens.tolist() == [5, 0, 20]
+
+
+# ---- together, in graphs and on two streams -----------------------------------------------
+@pytest.mark.parametrize("kv_format", ["fp16", "int4"])
+def test_admission_prompt_and_steps_in_a_graph(kv_format):
+    """Captured once and replayed with other rows, lengths and inputs, refused
+    batches among them: what the same calls give one by one."""
+    from memopt import PackedKVCache, RotaryPositions
+
+    H, KVH, D, T = 4, 2, 64, 120
+    gc.collect()
+    C().init_pool(40, 16, KVH, D, kv_format=kv_format)
+    rot = RotaryPositions(D, sections=[16, 16])
+    one, two = (PackedKVCache(20, KVH, D, 16, max_seqs=4, max_seq_len=112, kv_format=kv_format, rotary=rot) for _ in range(2))
+    q, k, v = tokens(T, H, KVH, D, seed=1)
+    rows, lens = torch.tensor([0, 2], dtype=torch.int32, device=DEV), torch.tensor([60, 50], dtype=torch.int32, device=DEV)
+
+    def step(cache):
+        out = [cache.prompt(q, k, v, cache.admit(rows, lens, T), T)]
+        out += [cache.decode(q[:2 * n], k[:2 * n], v[:2 * n], cache.extend(rows, n)) for n in (1, 3)]
+        return out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(one)  # warm-up: the paged attention's workspace of this stream
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(one)
+        for i, (r, n) in enumerate((((0, 2), (60, 50)), ((1, 3), (1, 112)), ((1, 0), (100, 20)), ((2, 2), (5, 5)),
+                                    ((2, 3), (0, 70)), ((0, 1), (90, 40)))):
+            rows.copy_(torch.tensor(r))
+            lens.copy_(torch.tensor(n))
+            for x, y in zip((q, k, v), tokens(T, H, KVH, D, seed=10 + i)):
+                x.copy_(y)
+            if i == 0:
+                step(two)  # the warm-up's turn, so that both tables have the same past
+            graph.replay()
+            want = step(two)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            for name in ("context_lens", "position_offsets"):
+                assert torch.equal(getattr(one.table, name), getattr(two.table, name))
+            assert torch.equal(one.table.pool_state, two.table.pool_state)
+            if r == (2, 2):
+                assert not any(x.any() for x in got)
+    side.synchronize()
+    torch.cuda.current_stream().wait_stream(side)
+
+
+def test_two_caches_on_two_streams():
+    """Prompts and steps of two layers at once: as one after the other."""
+    from memopt import PackedKVCache, RotaryPositions
+
+    H, KVH, D, lens = 8, 2, 128, [300, 1, 77]
+
+    def layers():
+        gc.collect()
+        C().init_pool(120, 16, KVH, D)
+        return [PackedKVCache(60, KVH, D, 16, max_seqs=3, max_seq_len=320, rotary=RotaryPositions(D)) for _ in range(2)]
+
+    data = [[tokens(n, H, KVH, D, seed=5 * i + j) for j, n in enumerate((378, 3, 3, 6))] for i in range(2)]
+
+    def run(cache, i):
+        out = [cache.prompt(*data[i][0], cache.admit([0, 1, 2], lens), 300)]
+        for x in data[i][1:]:
+            out.append(cache.decode(*x, cache.extend([0, 1, 2], x[0].shape[0] // 3)))
+        return out
+
+    caches = layers()
+    want = [run(c, i) for i, c in enumerate(caches)]
+    torch.cuda.synchronize()
+    del caches
+    caches, streams, got = layers(), [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got.append(run(caches[i], i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+        caches[i].table.check()
+
+
+def test_position_offsets_that_overlap_are_refused():
+    i32 = dict(dtype=torch.int32, device=DEV)
+    names = ("block_tables", "context_lens", "position_offsets", "free_pages", "pool_state", "rows", "lens")
+    for other in names:
+        if other == "position_offsets":
+            continue
+        a = {"block_tables": torch.full((4, 4), -1, **i32), "context_lens": torch.zeros(4, **i32),
+             "position_offsets": torch.zeros(4, **i32), "free_pages": torch.arange(8, **i32),
+             "pool_state": torch.tensor([0, 8, 0, 0], **i32), "rows": torch.arange(4, **i32),
+             "lens": torch.zeros(4, **i32)}
+        a["position_offsets"] = a[other].view(-1)[:4]
+        with pytest.raises(RuntimeError, match="overlap"):
+            C().reserve_rows(*(a[n] for n in names), 16, 4)
+    with pytest.raises(RuntimeError, match="position_offsets"):
+        a["position_offsets"] = torch.zeros(3, **i32)
+        C().reserve_rows(*(a[n] for n in names), 16, 4)
