@@ -216,19 +216,19 @@ def test_rotary_positions_after_an_eviction(sections):
         at[r], true[r] = at[r][: len(at[r]) - n], true[r] - n
 
     step(1, 2)
-    for round, ratio in enumerate((0.5, 0.7)):  # twice, so that offsets add up
-        g = torch.Generator(device=DEV).manual_seed(round)
+    for part, ratio in enumerate((0.5, 0.7)):  # twice, so that offsets add up
+        g = torch.Generator(device=DEV).manual_seed(part)
         for r, kept in zip(rows, evicted(cache, rows, torch.rand(4, KVH, 256, generator=g, device=DEV), ratio)):
             assert len(kept) < len(at[r]) or len(at[r]) < 7
             raw[r] = tuple(x[kept] for x in raw[r])
             at[r] = [at[r][i] for i in kept]
         for i in range(3):
-            step(1, 10 * round + i + 3)
-        step(5, 40 + round)
+            step(1, 10 * part + i + 3)
+        step(5, 40 + part)
         cache.table.truncate(rows, [len(at[r]) - 4 for r in rows])  # four of five drafts rejected
         for r in rows:
             cut(r, 4)
-        step(1, 50 + round)
+        step(1, 50 + part)
     # A row that begins anew begins at 0; the others keep their offsets.
     cache.finish([2])
     q, k, v = tokens(30, H, KVH, D, seed=60)
